@@ -14,6 +14,7 @@ Where ``own`` is false, ``run`` computes them with elementary torch operations
 in 32 bits (64 for the sums over rows), rounded once to the output's type.
 """
 
+import functools
 import math
 import sys
 from pathlib import Path
@@ -33,6 +34,7 @@ MAX_PRODUCT = 8192 * 4096 * 8192
 MAX_LOGITS = 4096 * 128000
 
 
+@functools.lru_cache(maxsize=None)
 def framework():
     package = str(Path(__file__).resolve().parent.parent / "alpha-yoo-for-great-kingdom_b200")
     if package not in sys.path:
