@@ -1,0 +1,864 @@
+// gk_policy_loss.cu - the policy loss of a training step and its gradient.
+//
+// For a row of logits z with legal entries L (all of them without a mask),
+//   log p_j = z_j - M - log S,  M = max_L z,  S = sum_L exp(z_j - M),
+// the row's loss has up to three terms:
+//   clipped ratio   -min(q A, clip(q, lo, hi) A),  q = exp(log p_a - old)
+//   KL estimate     kl_weight (e^d - d - 1),       d = reference - log p_a
+//   target          target_weight sum_j t_j (log t_j - log p_j)
+// and its gradient is, with c the derivative by log p_a and T = sum_j t_j,
+//   dz_j = (target_weight T - c) p_j - target_weight t_j + c [j = a].
+// The loss is the sum of the rows divided by the denominator.
+//
+// The row statistics, the row terms and the gradient are fp32 (row sums are
+// added in double); the gradient is rounded once to the logits' type. exp of
+// 16-bit logits uses the hardware's 2^x (relative error about 2^-22, far below
+// the 2^-9 of the rounded result); fp32 logits use expf.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cfloat>
+#include <cstdint>
+#include <type_traits>
+
+#include "../../include/gk.h"
+#include "gk_launch.cuh"
+
+namespace gk {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kRowWarps = 8;        // rows per block of the short-row kernel
+constexpr int kShortRow = 256;      // longest row that one warp keeps in registers
+constexpr int kLongThreads = 256;   // threads per CTA of the long-row kernel
+constexpr int kMaxCluster = 8;
+
+struct None {};
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) {
+    return v;
+}
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) {
+    return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// exp(x - m) for many x of one row. For 16-bit logits it is 2^(x s - m s),
+// one multiply-add and one 2^x; `correct` undoes the rounding of m s, which
+// all terms share. The difference of two values whose product with log2 e
+// would overflow is either 0 or below -1e35, so any small scale serves there.
+template <typename T>
+struct Exp {
+    float scale, offset, correct;
+    __device__ __forceinline__ explicit Exp(float m) {
+        scale = fabsf(m) < 1e38f ? 1.4426950408889634f : 1e-30f;
+        offset = m * scale;
+        const float rest = fmaf(m, scale, -offset);
+        correct = fabsf(rest) < 1.0f ? ex2(-rest) : 1.0f;
+    }
+    __device__ __forceinline__ float operator()(float x) const { return ex2(fmaf(x, scale, -offset)); }
+};
+template <>
+struct Exp<float> {
+    float m;
+    static constexpr float correct = 1.0f;
+    __device__ __forceinline__ explicit Exp(float top) : m(top) {}
+    __device__ __forceinline__ float operator()(float x) const { return expf(x - m); }
+};
+
+// Elements of one 16-byte vector of logits.
+template <typename T>
+constexpr int kVec = 16 / (int)sizeof(T);
+
+template <int BYTES>
+struct Raw;
+template <>
+struct Raw<1> {
+    using type = uint8_t;
+};
+template <>
+struct Raw<4> {
+    using type = uint32_t;
+};
+template <>
+struct Raw<8> {
+    using type = uint2;
+};
+template <>
+struct Raw<16> {
+    using type = uint4;
+};
+
+// V consecutive entries of a row, masked ones as -inf, with a bit an entry for the legal ones.
+template <typename TL, int V>
+struct Group {
+    alignas(V > 1 ? 16 : alignof(TL)) TL raw[V];
+    uint32_t legal;
+    __device__ __forceinline__ float x(int i) const { return to_f(raw[i]); }
+    __device__ __forceinline__ float top() const {
+        if constexpr (V == 8) {  // 16-bit logits: in pairs, which keeps them packed
+            using P = typename std::conditional<std::is_same<TL, __half>::value, __half2, __nv_bfloat162>::type;
+            const P* v = reinterpret_cast<const P*>(raw);
+            const P m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+            return fmaxf(to_f(m.x), to_f(m.y));
+        } else {
+            float m = x(0);
+#pragma unroll
+            for (int i = 1; i < V; ++i) m = fmaxf(m, x(i));
+            return m;
+        }
+    }
+    // All V entries lie in the row; `from` is 16-byte aligned if V > 1.
+    __device__ __forceinline__ void load(const TL* from, const uint8_t* mask) {
+        legal = (1u << V) - 1u;
+        if constexpr (V > 1)
+            *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(from);
+        else
+            raw[0] = *from;
+        if (mask != nullptr) {
+            alignas(V) uint8_t m[V];
+            using R = typename Raw<V>::type;
+            *reinterpret_cast<R*>(m) = __ldg(reinterpret_cast<const R*>(mask));
+            legal = 0u;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                legal |= (m[i] != 0 ? 1u : 0u) << i;
+                if (m[i] == 0) raw[i] = from_f<TL>(-INFINITY);
+            }
+        }
+    }
+    // The group at the row's start or end: entries outside [0, cols) count as masked.
+    __device__ __forceinline__ void load_edge(const TL* lrow, const uint8_t* mrow, int first, int cols) {
+        legal = 0u;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int j = first + i;
+            const bool in = j >= 0 && j < cols && (mrow == nullptr || mrow[j] != 0);
+            legal |= (in ? 1u : 0u) << i;
+            raw[i] = in ? lrow[j] : from_f<TL>(-INFINITY);
+        }
+    }
+};
+
+// The same entries of the target, 0 where `legal` has no bit.
+template <typename TT, int V>
+__device__ __forceinline__ void load_target(const TT* trow, uint32_t legal, int first, bool edge, float (&t)[V]) {
+    if constexpr (std::is_same<TT, None>::value) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[i] = 0.0f;
+    } else {
+        if (V > 1 && !edge) {
+            if constexpr (V > 1) {
+                alignas(16) TT tv[V];
+#pragma unroll
+                for (int k = 0; k < (int)(V * sizeof(TT) / 16); ++k)
+                    reinterpret_cast<uint4*>(tv)[k] = __ldg(reinterpret_cast<const uint4*>(trow + first) + k);
+#pragma unroll
+                for (int i = 0; i < V; ++i) t[i] = (legal >> i) & 1u ? to_f(tv[i]) : 0.0f;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) t[i] = (legal >> i) & 1u ? to_f(trow[first + i]) : 0.0f;
+        }
+    }
+}
+
+template <typename TL, int V>
+__device__ __forceinline__ void store_group(TL* grow, int first, int cols, bool edge, const float (&g)[V]) {
+    if (V > 1 && !edge) {
+        if constexpr (V > 1) {
+            alignas(16) TL raw[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) raw[i] = from_f<TL>(g[i]);
+            __stcs(reinterpret_cast<uint4*>(grow + first), *reinterpret_cast<uint4*>(raw));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (first + i >= 0 && first + i < cols) grow[first + i] = from_f<TL>(g[i]);
+    }
+}
+
+// Maximum and sum of exponentials of a part of a row. M starts at the lowest
+// finite value, so -inf entries add exp(-inf) = 0 and a row of nothing but the
+// lowest value is uniform; S == 0 means that nothing is left.
+struct Softmax {
+    float m = -FLT_MAX, s = 0.0f;
+    // Symmetric, so a butterfly of joins gives every lane the same bits.
+    __device__ __forceinline__ void join(float m2, float s2) {
+        const float top = fmaxf(m, m2);
+        // A part with nothing in it must not scale by exp(lowest - top).
+        s = (s == 0.0f ? 0.0f : s * expf(m - top)) + (s2 == 0.0f ? 0.0f : s2 * expf(m2 - top));
+        m = top;
+    }
+    __device__ __forceinline__ void join_lanes(int lanes) {
+        for (int o = lanes >> 1; o; o >>= 1) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+            join(m2, s2);
+        }
+    }
+};
+
+struct Row {
+    float m, inv_s, log_s, total_t;  // inv_s 0: the row is skipped
+    float c;                         // derivative of the row's loss by log p of the action
+    float loss;                      // without the target term
+    float log_p;
+    int64_t action;                  // -1: none
+};
+
+// What the row's scalar terms read; fetched before the statistics are known.
+struct RowInput {
+    int64_t action = -1;
+    float x = 0.0f, old = 0.0f, advantage = 0.0f, reference = 0.0f;
+    bool legal = false;
+};
+template <typename TL>
+__device__ __forceinline__ RowInput row_input(const gk_policy_loss_t& p, int64_t r, const TL* lrow,
+                                              const uint8_t* mrow) {
+    RowInput in;
+    if (p.actions != nullptr) {
+        in.action = p.actions[r];
+        in.old = p.old_log_probs[r];
+        in.advantage = p.advantages[r];
+        if (p.reference_log_probs != nullptr) in.reference = p.reference_log_probs[r];
+        in.legal = in.action >= 0 && in.action < p.cols && (mrow == nullptr || mrow[in.action] != 0);
+        if (in.legal) in.x = to_f(lrow[in.action]);
+    }
+    return in;
+}
+
+// The row's scalar terms from its statistics. WIDE: a long row's log p is in
+// the tens, where the ratio exp(log p - old) would feel the last fp32 bit of
+// log p, so the difference is formed in double (by one thread a row).
+template <bool WIDE>
+__device__ __forceinline__ Row row_terms(const gk_policy_loss_t& p, const RowInput& in, float m, float s,
+                                         float total_t) {
+    Row o;
+    o.m = m;
+    o.total_t = total_t;
+    o.c = o.loss = o.log_p = 0.0f;
+    o.log_s = logf(s);
+    o.action = -1;
+    bool skip = s == 0.0f;
+    if (p.actions != nullptr) {
+        skip = skip || in.action < 0;
+        if (!skip) {
+            if (!in.legal) {
+                // There is no log-probability to train on.
+                o.c = o.loss = o.log_p = nanf("");
+            } else {
+                o.action = in.action;
+                using W = typename std::conditional<WIDE, double, float>::type;
+                const W log_s = WIDE ? (W)log((double)s) : (W)o.log_s;
+                const W log_p = ((W)in.x - (W)m) - log_s;
+                o.log_p = (float)log_p;
+                const float adv = in.advantage;
+                const float q = expf((float)(log_p - (W)in.old));
+                const float free = q * adv, held = fminf(fmaxf(q, p.clip_low), p.clip_high) * adv;
+                // fminf drops a NaN; the comparisons keep it.
+                o.loss = free <= held ? -free : (held < free ? -held : nanf(""));
+                o.c = free <= held ? -free : (held < free ? 0.0f : nanf(""));
+                if (p.reference_log_probs != nullptr) {
+                    const float d = (float)((W)in.reference - log_p);
+                    const float e = expm1f(d);
+                    o.loss += p.kl_weight * (e - d);
+                    o.c -= p.kl_weight * e;
+                }
+            }
+        }
+    }
+    o.inv_s = skip ? 0.0f : 1.0f / s;
+    if (skip) o.total_t = 0.0f;
+    return o;
+}
+
+__device__ __forceinline__ float inverse_denominator(const gk_policy_loss_t& p) {
+    return 1.0f / (p.denominator_ptr != nullptr ? *p.denominator_ptr : p.denominator);
+}
+
+// Gradient of a group but for the action's own part: `kp` multiplies exp(x - M), `kt` the target.
+template <typename TL, typename TT, int V>
+__device__ __forceinline__ void gradient_group(const Group<TL, V>& h, const float (&t)[V], const Exp<TL>& e, float kp,
+                                               float kt, float (&g)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        g[i] = kp * e(h.x(i));
+        if constexpr (!std::is_same<TT, None>::value) g[i] -= kt * t[i];
+    }
+}
+
+__device__ __forceinline__ float target_term(float t, float x, float m, float log_s) {
+    return t > 0.0f ? t * (logf(t) - ((x - m) - log_s)) : (t == 0.0f ? 0.0f : nanf(""));
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    return v;
+}
+
+__device__ __forceinline__ void write_row(const gk_policy_loss_t& p, int64_t r, const Row& o) {
+    reinterpret_cast<float4*>(p.stats)[r] = make_float4(o.m, o.inv_s, o.c, o.total_t);
+    if (p.log_probs != nullptr) p.log_probs[r] = o.inv_s == 0.0f ? 0.0f : o.log_p;
+}
+
+// The sum of the blocks' sums in their order; one block.
+__device__ __forceinline__ void finish_loss(const gk_policy_loss_t& p, double sum) {
+    *p.loss = (float)(sum * (1.0 / (double)(p.denominator_ptr != nullptr ? *p.denominator_ptr : p.denominator)));
+}
+
+__global__ void __launch_bounds__(256) policy_loss_sum_kernel(gk_policy_loss_t p, int parts) {
+    __shared__ double sums[256];
+    double v = 0.0;
+    for (int i = threadIdx.x; i < parts; i += 256) v += p.partials[i];
+    sums[threadIdx.x] = v;
+    __syncthreads();
+    for (int o = 128; o; o >>= 1) {
+        if (threadIdx.x < o) sums[threadIdx.x] += sums[threadIdx.x + o];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) finish_loss(p, sums[0]);
+}
+
+// Rows of at most 32 * NPL entries: a warp holds its row in registers, so
+// logits, mask and target are read once and the gradient is written in the
+// same pass. Lane l holds entries l, l + 32, ...
+template <typename TL, typename TT, int NPL>
+__global__ void __launch_bounds__(kRowWarps * 32) policy_loss_rows_kernel(gk_policy_loss_t p) {
+    __shared__ double sums[kRowWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    double sum = 0.0;
+    const float inv_n = inverse_denominator(p);
+    for (int64_t r = (int64_t)blockIdx.x * kRowWarps + warp; r < p.rows; r += (int64_t)gridDim.x * kRowWarps) {
+        const TL* lrow = static_cast<const TL*>(p.logits) + r * p.logits_stride;
+        const uint8_t* mrow = p.mask == nullptr ? nullptr : p.mask + r * p.mask_stride;
+        const TT* trow = std::is_same<TT, None>::value ? nullptr
+                                                       : static_cast<const TT*>(p.target) + r * p.target_stride;
+        float x[NPL], t[NPL];
+        uint32_t legal = 0u;
+        float m = -FLT_MAX, total_t = 0.0f;
+        const RowInput in_row = row_input(p, r, lrow, mrow);
+#pragma unroll
+        for (int k = 0; k < NPL; ++k) {
+            const int j = lane + 32 * k;
+            const bool in = j < p.cols && (mrow == nullptr || mrow[j] != 0);
+            legal |= (in ? 1u : 0u) << k;
+            x[k] = in ? to_f(lrow[j]) : -INFINITY;
+            t[k] = 0.0f;
+            if constexpr (!std::is_same<TT, None>::value) t[k] = in ? to_f(trow[j]) : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < NPL; ++k) {
+            m = fmaxf(m, x[k]);
+            total_t += t[k];
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+        const Exp<TL> exp_m(m);
+        float e[NPL], s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NPL; ++k) {
+            e[k] = exp_m(x[k]);
+            s += e[k];
+        }
+        s = warp_sum(s) * exp_m.correct;
+        if constexpr (!std::is_same<TT, None>::value) total_t = warp_sum(total_t);
+        const Row o = row_terms<false>(p, in_row, m, s, total_t);
+        float loss = lane == 0 ? o.loss : 0.0f;
+        if constexpr (!std::is_same<TT, None>::value) {
+            float kl = 0.0f;
+#pragma unroll
+            for (int k = 0; k < NPL; ++k) kl += target_term(t[k], x[k], m, o.log_s);
+            kl = warp_sum(kl);
+            if (lane == 0 && o.inv_s != 0.0f) loss += p.target_weight * kl;
+        }
+        if (lane == 0) {
+            sum += (double)loss;
+            write_row(p, r, o);
+        }
+        if (p.grad != nullptr) {
+            TL* grow = static_cast<TL*>(p.grad) + r * p.cols;
+            const float kp = inv_n * (p.target_weight * o.total_t - o.c) * o.inv_s * exp_m.correct;
+            const float kt = inv_n * p.target_weight;
+#pragma unroll
+            for (int k = 0; k < NPL; ++k) {
+                const int j = lane + 32 * k;
+                if (j >= p.cols) continue;
+                float g = 0.0f;
+                if (((legal >> k) & 1u) && o.inv_s != 0.0f) {
+                    g = kp * e[k] - kt * t[k];
+                    if (j == o.action) g += inv_n * o.c;
+                }
+                grow[j] = from_f<TL>(g);
+            }
+        }
+    }
+    if (lane == 0) sums[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double v = 0.0;
+        for (int w = 0; w < kRowWarps; ++w) v += sums[w];
+        if (gridDim.x == 1)
+            finish_loss(p, v);
+        else
+            p.partials[blockIdx.x] = v;
+    }
+}
+
+// The part of a row that one CTA of a cluster takes: groups of V entries that
+// start on 16-byte boundaries of the logits. Groups [full, full_end) lie in the
+// row; a group before or after them is the row's ragged edge.
+template <typename TL, typename TT, int V>
+struct Part {
+    const TL* lrow;
+    const uint8_t* mrow;
+    const TT* trow;
+    int shift, begin, end, full, full_end;
+    __device__ __forceinline__ Part(const gk_policy_loss_t& p, int64_t r, int rank, int ranks) {
+        lrow = static_cast<const TL*>(p.logits) + r * p.logits_stride;
+        mrow = p.mask == nullptr ? nullptr : p.mask + r * p.mask_stride;
+        trow = std::is_same<TT, None>::value ? nullptr : static_cast<const TT*>(p.target) + r * p.target_stride;
+        const int cols = (int)p.cols;
+        shift = V == 1 ? 0 : (int)((r * p.logits_stride) % V);
+        const int groups = (cols + shift + V - 1) / V, each = (groups + ranks - 1) / ranks;
+        begin = min(groups, rank * each);
+        end = min(groups, begin + each);
+        full = max(begin, shift > 0 ? 1 : 0);
+        full_end = min(end, (cols + shift) / V);
+    }
+};
+
+// Each thread copies the groups that it will read itself, so no barrier stands
+// between the copy and its use.
+template <typename TL, typename TT, int V>
+__device__ __forceinline__ void stage_row(const Part<TL, TT, V>& part, uint4* buffer) {
+    for (int q = part.full + threadIdx.x; q < part.full_end; q += blockDim.x) {
+        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(buffer + (q - part.full));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(part.lrow + ((int64_t)q * V - part.shift))
+                     : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+// Longer rows: a cluster of CTAs takes a row, each CTA a part of it; the parts
+// meet through distributed shared memory. STAGED: a CTA's part of the logits
+// lies in shared memory, with two buffers the next row's part on its way while
+// this one is worked on, so the logits are read from HBM once and the copies
+// never stop. Otherwise (a part past the shared memory, or rows that are not
+// aligned) each pass reads the row itself, from L2 where it fits.
+template <typename TL, typename TT, int V, bool STAGED>
+__global__ void __launch_bounds__(kLongThreads, 3) policy_loss_long_kernel(gk_policy_loss_t p, int buffers,
+                                                                           int part_groups) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    constexpr bool kTarget = !std::is_same<TT, None>::value;
+    constexpr int kWarps = kLongThreads / 32;
+    extern __shared__ uint4 staged[];
+    __shared__ float wm[kWarps], ws[kWarps], wt[kWarps], wk[kWarps];
+    __shared__ float part_sums[3];  // this CTA's maximum, sum, target sum: read by the cluster
+    __shared__ float part_kl[2];    // this CTA's target term, by turns: read by rank 0
+    __shared__ Row shared_row;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    const int64_t clusters = gridDim.x / ranks, first_row = blockIdx.x / ranks;
+    const float inv_n = inverse_denominator(p);
+    const int cols = (int)p.cols;
+    double sum = 0.0;
+    int turn = 0;
+    auto meet = [&] {
+        if (ranks > 1)
+            cluster.sync();
+        else
+            __syncthreads();
+    };
+    if constexpr (STAGED) stage_row(Part<TL, TT, V>(p, first_row, rank, ranks), staged);
+    for (int64_t r = first_row; r < p.rows; r += clusters, turn ^= 1) {
+        const Part<TL, TT, V> part(p, r, rank, ranks);
+        RowInput in;
+        if (tid == 0) in = row_input(p, r, part.lrow, part.mrow);
+        const TL* from = part.lrow + ((int64_t)part.full * V - part.shift);
+        if constexpr (STAGED) {
+            if (buffers == 2 && r + clusters < p.rows) {
+                // The other buffer's row was finished before the last barrier.
+                stage_row(Part<TL, TT, V>(p, r + clusters, rank, ranks), staged + (turn ^ 1) * part_groups);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            } else {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+            }
+            from = reinterpret_cast<const TL*>(staged + (buffers == 2 ? turn * part_groups : 0));
+        }
+        // f(group, index of its first entry, whether it is an edge); thread 0
+        // also takes the row's first edge and thread 32 its last.
+        auto each_group = [&](auto&& f) {
+            const int count = part.full_end - part.full, base = part.full * V - part.shift;
+#pragma unroll 4
+            for (int k = tid; k < count; k += blockDim.x) {
+                Group<TL, V> h;
+                h.load(from + k * V, part.mrow == nullptr ? nullptr : part.mrow + base + k * V);
+                f(h, base + k * V, false);
+            }
+            if (V > 1) {
+                if (tid == 0 && part.begin < part.full && part.begin < part.end) {
+                    Group<TL, V> h;
+                    h.load_edge(part.lrow, part.mrow, part.begin * V - part.shift, cols);
+                    f(h, part.begin * V - part.shift, true);
+                }
+                if (tid == 32 && part.full_end < part.end && part.end - 1 >= part.full) {
+                    Group<TL, V> h;
+                    h.load_edge(part.lrow, part.mrow, (part.end - 1) * V - part.shift, cols);
+                    f(h, (part.end - 1) * V - part.shift, true);
+                }
+            }
+        };
+        Softmax acc;
+        float total_t = 0.0f;
+        each_group([&](const Group<TL, V>& h, int, bool) { acc.m = fmaxf(acc.m, h.top()); });
+#pragma unroll
+        for (int o = 16; o; o >>= 1) acc.m = fmaxf(acc.m, __shfl_xor_sync(kFull, acc.m, o));
+        {
+            const Exp<TL> e(acc.m);
+            each_group([&](const Group<TL, V>& h, int first, bool edge) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc.s += e(h.x(i));
+                if constexpr (kTarget) {
+                    float t[V];
+                    load_target<TT, V>(part.trow, h.legal, first, edge, t);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) total_t += t[i];
+                }
+            });
+            acc.s = warp_sum(acc.s) * e.correct;
+        }
+        if (kTarget) total_t = warp_sum(total_t);
+        if (lane == 0) wm[warp] = acc.m, ws[warp] = acc.s, wt[warp] = total_t;
+        __syncthreads();
+        if (warp == 0) {
+            acc.m = lane < warps ? wm[lane] : -FLT_MAX;
+            acc.s = lane < warps ? ws[lane] : 0.0f;
+            acc.join_lanes(kWarps);
+            if (kTarget) total_t = warp_sum(lane < warps ? wt[lane] : 0.0f);
+            if (ranks > 1) {
+                if (lane == 0) part_sums[0] = acc.m, part_sums[1] = acc.s, part_sums[2] = total_t;
+            } else if (lane == 0) {
+                shared_row = row_terms<true>(p, in, acc.m, acc.s, total_t);
+                write_row(p, r, shared_row);
+            }
+        }
+        if (ranks > 1) {
+            cluster.sync();
+            if (warp == 0) {
+                const float* other = cluster.map_shared_rank(part_sums, lane < ranks ? lane : 0);
+                acc.m = lane < ranks ? other[0] : -FLT_MAX;
+                acc.s = lane < ranks ? other[1] : 0.0f;
+                if (kTarget) total_t = warp_sum(lane < ranks ? other[2] : 0.0f);
+                acc.join_lanes(kMaxCluster);
+                if (lane == 0) {
+                    shared_row = row_terms<true>(p, in, acc.m, acc.s, total_t);
+                    if (rank == 0) write_row(p, r, shared_row);
+                }
+            }
+        }
+        __syncthreads();
+        const Row o = shared_row;
+        if (kTarget || p.grad != nullptr) {
+            TL* grow = static_cast<TL*>(p.grad) + r * p.cols;
+            const Exp<TL> e(o.m);
+            const float kp = inv_n * (p.target_weight * o.total_t - o.c) * o.inv_s * e.correct;
+            const float kt = inv_n * p.target_weight;
+            const bool live = o.inv_s != 0.0f;
+            float kl = 0.0f;
+            each_group([&](const Group<TL, V>& h, int first, bool edge) {
+                float t[V], g[V];
+                load_target<TT, V>(part.trow, h.legal, first, edge, t);
+                if (kTarget) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) kl += target_term(t[i], h.x(i), o.m, o.log_s);
+                }
+                if (p.grad != nullptr) {
+                    if (live) {
+                        gradient_group<TL, TT, V>(h, t, e, kp, kt, g);
+                        const int64_t at = o.action - first;
+                        if (at >= 0 && at < V) {  // one group of the row
+#pragma unroll
+                            for (int i = 0; i < V; ++i)
+                                if (at == i) g[i] += inv_n * o.c;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < V; ++i) g[i] = 0.0f;
+                    }
+                    store_group<TL, V>(grow, first, cols, edge, g);
+                }
+            });
+            if (kTarget) {
+                kl = warp_sum(kl);
+                if (lane == 0) wk[warp] = kl;
+                __syncthreads();
+                if (warp == 0) {
+                    kl = warp_sum(lane < warps ? wk[lane] : 0.0f);
+                    if (lane == 0) part_kl[turn] = kl;
+                }
+            }
+        }
+        if constexpr (STAGED) {
+            if (buffers == 1 && r + clusters < p.rows)  // each thread has read its own groups
+                stage_row(Part<TL, TT, V>(p, r + clusters, rank, ranks), staged);
+        }
+        meet();  // also keeps every CTA's part until all have read it
+        if (rank == 0 && warp == 0) {
+            float kl = 0.0f;
+            if (kTarget) kl = warp_sum(lane < ranks ? *cluster.map_shared_rank(part_kl + turn, lane < ranks ? lane : 0) : 0.0f);
+            sum += (double)(o.loss + (kTarget && o.inv_s != 0.0f ? p.target_weight * kl : 0.0f));
+        }
+    }
+    if (ranks > 1) cluster.sync();  // no CTA leaves while another reads its shared memory
+    if (rank == 0 && tid == 0) {
+        if (clusters == 1)
+            finish_loss(p, sum);
+        else
+            p.partials[first_row] = sum;
+    }
+}
+
+// The gradient from the saved row statistics, scaled by the upstream
+// gradient. A gradient that the forward pass wrote is for an upstream of one,
+// and is left as it is when that holds (`written`).
+template <typename TL, typename TT, int V>
+__global__ void __launch_bounds__(256) policy_loss_backward_kernel(gk_policy_loss_t p, const float* upstream,
+                                                                   int written) {
+    const float up = *upstream;
+    if (written && up == 1.0f) return;
+    constexpr int kGroups = 4;  // groups a lane takes of a row's chunk
+    const float scale = up * inverse_denominator(p);
+    const int lane = threadIdx.x & 31, cols = (int)p.cols;
+    const int64_t chunks = (p.cols + V - 1 + V * 32 * kGroups - 1) / (V * 32 * kGroups), items = p.rows * chunks;
+    const int64_t warps = (int64_t)gridDim.x * 8;
+    for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += warps) {
+        const int64_t r = it / chunks;
+        const int chunk = (int)(it - r * chunks);
+        const Part<TL, TT, V> part(p, r, 0, 1);
+        TL* grow = static_cast<TL*>(p.grad) + r * p.cols;
+        const float4 st = reinterpret_cast<const float4*>(p.stats)[r];  // maximum, 1 / sum, c, target sum
+        const int64_t action = p.actions == nullptr ? -1 : p.actions[r];
+        const Exp<TL> e(st.x);
+        const float kp = scale * (p.target_weight * st.w - st.z) * st.y * e.correct, kt = scale * p.target_weight;
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) {
+            const int q = (chunk * kGroups + k) * 32 + lane;
+            if (q >= part.end) break;
+            const int first = q * V - part.shift;
+            const bool edge = q < part.full || q >= part.full_end;
+            float t[V], g[V];
+            Group<TL, V> h;
+            if (edge)
+                h.load_edge(part.lrow, part.mrow, first, cols);
+            else
+                h.load(part.lrow + first, part.mrow == nullptr ? nullptr : part.mrow + first);
+            load_target<TT, V>(part.trow, h.legal, first, edge, t);
+            if (st.y != 0.0f) {
+                gradient_group<TL, TT, V>(h, t, e, kp, kt, g);
+                const int64_t at = action - first;
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (at == i) g[i] += scale * st.z;
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) g[i] = 0.0f;
+            }
+            store_group<TL, V>(grow, first, cols, edge, g);
+        }
+    }
+}
+
+bool valid(const gk_policy_loss_t* p) {
+    if (p == nullptr || p->rows < 0 || p->cols < 1 || p->cols > (1ll << 30)) return false;
+    if (p->logits_type < GK_FP32 || p->logits_type > GK_FP16) return false;
+    if (p->rows == 0) return p->loss != nullptr;
+    if (p->logits == nullptr || p->stats == nullptr || p->partials == nullptr || p->loss == nullptr) return false;
+    if (p->target != nullptr && p->target_type != GK_FP32 && p->target_type != p->logits_type) return false;
+    if (p->actions == nullptr) {
+        if (p->target == nullptr || p->reference_log_probs != nullptr) return false;
+    } else if (p->old_log_probs == nullptr || p->advantages == nullptr) {
+        return false;
+    }
+    return true;
+}
+
+bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// Whether every operand's 16-byte groups fall on the logits' own groups in
+// every row: aligned bases, and row lengths that leave the same remainder.
+bool vectorised(const gk_policy_loss_t& p, int v) {
+    auto same = [&](int64_t stride) { return (stride - p.logits_stride) % v == 0; };
+    if (!aligned16(p.logits)) return false;
+    if (p.mask != nullptr && !(aligned(p.mask, v) && same(p.mask_stride))) return false;
+    if (p.target != nullptr && !(aligned16(p.target) && same(p.target_stride))) return false;
+    if (p.grad != nullptr && !(aligned16(p.grad) && same(p.cols))) return false;
+    return p.logits_stride >= 0;
+}
+
+// How a long row is split and staged. A CTA's part is at most 32 KB where two
+// buffers of it are kept (three CTAs an SM), at most 64 KB with one; the
+// cluster grows until the part fits, and with fewer rows than SMs until the
+// grid fills them, but no part gets shorter than two vectors a thread. Parts
+// under 8 KB take half the threads, so that more rows are in flight.
+struct LongPlan {
+    int cluster, threads, buffers, part_groups;
+    size_t smem;
+};
+constexpr int64_t kPartBytes = 32 << 10;
+
+LongPlan long_plan(const gk_policy_loss_t& p, int v) {
+    const int64_t groups = (p.cols + 2 * (v - 1)) / v;  // with the shift of an odd row
+    int c = 1;
+    auto part = [&](int k) { return (groups + k - 1) / k; };
+    while (c < kMaxCluster && (part(c) * 16 > kPartBytes ||
+                               (p.rows * c * 2 <= 3 * kSmCount && part(2 * c) >= 2 * kLongThreads)))
+        c *= 2;
+    LongPlan plan{};
+    plan.cluster = c;
+    plan.part_groups = (int)part(c);
+    const int64_t bytes = part(c) * 16;
+    plan.threads = bytes < (8 << 10) ? kLongThreads / 2 : kLongThreads;
+    plan.buffers = v == 1 || bytes > 2 * kPartBytes ? 0 : (bytes > kPartBytes ? 1 : 2);
+    plan.smem = (size_t)plan.buffers * bytes;
+    return plan;
+}
+
+int row_blocks(int64_t rows) { return blocks_for(rows, kRowWarps, kSmCount * 8); }
+// Clusters of a long-row launch: as many as the SMs hold at once (by a CTA's
+// shared memory, at most eight of half the threads), so each keeps its next row in flight.
+int long_clusters(int64_t rows, const LongPlan& plan) {
+    const int64_t per_sm = plan.threads == kLongThreads ? 3 : 6;
+    const int64_t most = kSmCount * per_sm / plan.cluster;
+    return (int)(rows < most ? rows : most);
+}
+
+template <typename TL, typename TT, int V, bool STAGED>
+int launch_long(const gk_policy_loss_t& p, const LongPlan& plan, int clusters, cudaStream_t s) {
+    auto* kernel = policy_loss_long_kernel<TL, TT, V, STAGED>;
+    static bool done[64] = {};
+    if (!once_per_device(done, [&] {
+            return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kPartBytes) ==
+                   cudaSuccess;
+        }))
+        return launch_status();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(clusters * plan.cluster));
+    cfg.blockDim = dim3(plan.threads);
+    cfg.dynamicSmemBytes = STAGED ? plan.smem : 0;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = plan.cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, p, plan.buffers, plan.part_groups);
+}
+
+template <typename TL, typename TT>
+int forward(const gk_policy_loss_t& p, cudaStream_t s) {
+    int parts;
+    if (p.cols <= kShortRow) {
+        parts = row_blocks(p.rows);
+        if (p.cols <= 96)
+            policy_loss_rows_kernel<TL, TT, 3><<<parts, kRowWarps * 32, 0, s>>>(p);
+        else
+            policy_loss_rows_kernel<TL, TT, 8><<<parts, kRowWarps * 32, 0, s>>>(p);
+    } else {
+        constexpr int V = kVec<TL>;
+        const bool vec = vectorised(p, V);
+        const LongPlan plan = long_plan(p, vec ? V : 1);
+        parts = long_clusters(p.rows, plan);
+        const int e = !vec ? launch_long<TL, TT, 1, false>(p, plan, parts, s)
+                           : (plan.buffers > 0 ? launch_long<TL, TT, V, true>(p, plan, parts, s)
+                                               : launch_long<TL, TT, V, false>(p, plan, parts, s));
+        if (e != 0) return e;
+    }
+    if (parts > 1) policy_loss_sum_kernel<<<1, 256, 0, s>>>(p, parts);
+    return launch_status();
+}
+
+template <typename TL, typename TT>
+int backward(const gk_policy_loss_t& p, const float* upstream, int written, cudaStream_t s) {
+    const bool vec = p.cols > kShortRow && vectorised(p, kVec<TL>);
+    const int64_t per = (int64_t)(vec ? kVec<TL> : 1) * 32 * 4;
+    const int64_t chunks = (p.cols + (vec ? kVec<TL> : 1) - 1 + per - 1) / per;
+    const int grid = blocks_for(p.rows * chunks, 8, kSmCount * 32);
+    if (vec)
+        policy_loss_backward_kernel<TL, TT, kVec<TL>><<<grid, 256, 0, s>>>(p, upstream, written);
+    else
+        policy_loss_backward_kernel<TL, TT, 1><<<grid, 256, 0, s>>>(p, upstream, written);
+    return launch_status();
+}
+
+template <typename F>
+int by_type(const gk_policy_loss_t& p, F&& f) {
+    const bool same = p.target != nullptr && p.target_type == p.logits_type;
+    if (p.logits_type == GK_FP32)
+        return p.target == nullptr ? f((float*)0, (None*)0) : f((float*)0, (float*)0);
+    if (p.logits_type == GK_BF16)
+        return p.target == nullptr ? f((__nv_bfloat16*)0, (None*)0)
+                                   : (same ? f((__nv_bfloat16*)0, (__nv_bfloat16*)0) : f((__nv_bfloat16*)0, (float*)0));
+    return p.target == nullptr ? f((__half*)0, (None*)0)
+                               : (same ? f((__half*)0, (__half*)0) : f((__half*)0, (float*)0));
+}
+
+}  // namespace
+}  // namespace gk
+
+extern "C" {
+
+int gk_policy_loss_parts(int64_t rows, int64_t cols) {
+    if (rows < 1 || cols < 1) return 0;
+    if (cols <= gk::kShortRow) return gk::row_blocks(rows);
+    const int64_t most = gk::kSmCount * 6;  // clusters of any plan
+    return (int)(rows < most ? rows : most);
+}
+
+int gk_policy_loss_forward(const gk_policy_loss_t* p, void* stream) {
+    using namespace gk;
+    if (!valid(p)) return GK_EINVAL;
+    cudaStream_t s = as_stream(stream);
+    if (p->rows == 0) {
+        const cudaError_t e = cudaMemsetAsync(p->loss, 0, sizeof(float), s);
+        return (int)e;
+    }
+    return by_type(*p, [&](auto* l, auto* t) {
+        return forward<std::remove_pointer_t<decltype(l)>, std::remove_pointer_t<decltype(t)>>(*p, s);
+    });
+}
+
+int gk_policy_loss_backward(const gk_policy_loss_t* p, const float* upstream, int written, void* stream) {
+    using namespace gk;
+    if (!valid(p) || upstream == nullptr) return GK_EINVAL;
+    if (p->rows == 0) return 0;
+    if (p->grad == nullptr) return GK_EINVAL;
+    return by_type(*p, [&](auto* l, auto* t) {
+        return backward<std::remove_pointer_t<decltype(l)>, std::remove_pointer_t<decltype(t)>>(
+            *p, upstream, written, as_stream(stream));
+    });
+}
+
+}  // extern "C"

@@ -16,3 +16,4 @@ from .replay import DeviceReplayBuffer, validate_rows  # noqa: F401
 from .batched_puct import BatchedSearchResult, GpuBatchedPUCT, PUCTOptions  # noqa: F401
 from .evaluation import EvaluationResult, evaluate_models_gpu  # noqa: F401
 from .engine_api import BatchedPUCT, PUCTMoveStatistics, PUCTSearchResult, encode_puct_batch  # noqa: F401
+from .losses import PolicyLoss, policy_loss  # noqa: F401

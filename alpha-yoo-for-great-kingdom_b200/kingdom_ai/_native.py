@@ -9,6 +9,7 @@ library is missing or a call fails, an exception is raised.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -22,6 +23,7 @@ c_int = ctypes.c_int
 c_int64 = ctypes.c_int64
 c_uint64 = ctypes.c_uint64
 c_double = ctypes.c_double
+c_float = ctypes.c_float
 c_size_t = ctypes.c_size_t
 
 
@@ -50,7 +52,20 @@ class NetStruct(ctypes.Structure):
                 ("norm", c_int), ("norm_w", c_void_p), ("norm_b", c_void_p), ("head_norm", c_void_p)]
 
 
+class PolicyLossStruct(ctypes.Structure):
+    _fields_ = [("logits", c_void_p), ("mask", c_void_p), ("target", c_void_p), ("actions", c_void_p),
+                ("old_log_probs", c_void_p), ("advantages", c_void_p), ("reference_log_probs", c_void_p),
+                ("denominator_ptr", c_void_p), ("rows", c_int64), ("cols", c_int64), ("logits_stride", c_int64),
+                ("mask_stride", c_int64), ("target_stride", c_int64), ("clip_low", c_float), ("clip_high", c_float),
+                ("kl_weight", c_float), ("target_weight", c_float), ("denominator", c_float), ("logits_type", c_int),
+                ("target_type", c_int), ("loss", c_void_p), ("log_probs", c_void_p), ("stats", c_void_p),
+                ("partials", c_void_p), ("grad", c_void_p)]
+
+
 _SIGNATURES = {
+    "gk_policy_loss_parts": [c_int64, c_int64],
+    "gk_policy_loss_forward": [ctypes.POINTER(PolicyLossStruct), c_void_p],
+    "gk_policy_loss_backward": [ctypes.POINTER(PolicyLossStruct), c_void_p, c_int, c_void_p],
     "gk_initial_records": [c_void_p, c_int64, c_int, c_void_p],
     "gk_initial_bits": [c_void_p, c_int64, c_int, c_void_p],
     "gk_play_records": [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p],
@@ -131,6 +146,22 @@ def ptr(tensor: torch.Tensor | None):
 
 def stream_of(device: torch.device):
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def launch_stream(device: torch.device, tensors):
+    """The current stream of `device`; the tensors are marked as used on it, so
+    that memory allocated on another stream is not reused under the launch."""
+    stream = torch.cuda.current_stream(device)
+    for tensor in tensors:
+        tensor.record_stream(stream)
+    return c_void_p(stream.cuda_stream)
+
+
+def on_device(device: torch.device):
+    """A context in which `device` is current (nothing to do if it already is)."""
+    if torch.cuda.current_device() == device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def require_cuda(device) -> torch.device:

@@ -538,6 +538,55 @@ GK_API int gk_bpuct_grow(const void* src, int capacity, void* dst, int new_capac
 GK_API int gk_replay_validate(const float* features, const uint8_t* masks, const float* policy, const float* value,
                               const int8_t* to_play, int64_t n, uint32_t* violations, void* stream);
 
+/* ------------------------------------------------------- training step */
+
+/* Element types of the training-step operators. */
+#define GK_FP32 0
+#define GK_BF16 1
+#define GK_FP16 2
+
+/* The policy loss of one batch. Per row with legal entries L (mask NULL: all)
+ * and log p = log softmax of the logits over L:
+ *   -min(q A, clip(q, clip_low, clip_high) A), q = exp(log p[action] - old)   (actions given)
+ *   + kl_weight (e^d - d - 1), d = reference - log p[action]                  (reference given)
+ *   + target_weight sum_j t_j (log t_j - log p_j)                             (target given)
+ * A row with action < 0, or with nothing left by its mask (-inf logits count
+ * as masked out), adds nothing and gets a zero gradient. An action past the row or masked out makes the
+ * row, and so the loss, NaN. Masked logits and targets do not enter, whatever they hold. */
+typedef struct {
+    const void* logits;               /* [rows, cols] of logits_type */
+    const uint8_t* mask;              /* [rows, cols], nonzero = legal; or NULL */
+    const void* target;               /* [rows, cols] fp32 or logits_type; or NULL */
+    const int64_t* actions;           /* [rows]; or NULL (then target is given) */
+    const float* old_log_probs;       /* [rows]; with actions */
+    const float* advantages;          /* [rows]; with actions */
+    const float* reference_log_probs; /* [rows]; or NULL */
+    const float* denominator_ptr;     /* the sum's divisor on the device; or NULL: `denominator` */
+    int64_t rows, cols;
+    int64_t logits_stride, mask_stride, target_stride; /* elements between rows */
+    float clip_low, clip_high, kl_weight, target_weight, denominator;
+    int logits_type, target_type;
+    float* loss;                      /* [1] */
+    float* log_probs;                 /* [rows] log p[action], 0 for skipped rows; or NULL */
+    float* stats;                     /* [rows, 4] row statistics for the backward pass, 16-byte aligned */
+    double* partials;                 /* [gk_policy_loss_parts] */
+    void* grad;                       /* [rows, cols] of logits_type; NULL in the forward pass: no gradient */
+} gk_policy_loss_t;
+
+/* Doubles that gk_policy_loss_t.partials holds (workspace of the loss's sum). */
+GK_API int gk_policy_loss_parts(int64_t rows, int64_t cols);
+
+/* The loss, log-probabilities and row statistics; with p->grad also the
+ * gradient of the loss by the logits. Stands in for the loss of train_step
+ * (python/kingdom_ai/training.py:213-230). */
+GK_API int gk_policy_loss_forward(const gk_policy_loss_t* p, void* stream);
+
+/* p->grad = *upstream (device) times the gradient, from the statistics that
+ * the forward pass of the same p wrote; with `written` the forward pass wrote
+ * the gradient there already, and an upstream of one leaves it. No reference
+ * counterpart of its own: autograd of training.py:213-230. */
+GK_API int gk_policy_loss_backward(const gk_policy_loss_t* p, const float* upstream, int written, void* stream);
+
 /* CUDA-event timer for kernel launches inside gk_selfplay_ply: a host object
  * holding `pairs` start/stop event pairs (NULL on failure). No reference
  * counterpart: the reference times phases with perf_counter (loop.py:563-621). */
