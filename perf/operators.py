@@ -366,7 +366,7 @@ def run(state):
             return _own_loss(state)
         if state["op"] == "linear":
             return _own_linear(state)
-        return {"x": framework().pack_activation(state["x"]).unpack()}
+        return {"x": framework().pack_activation(state["x"]).unpack(torch.float32)}
     if state["op"] == "loss":
         return _plain_loss(state)
     if state["op"] == "linear":
