@@ -1,0 +1,330 @@
+// gk_gemm.cu - 16-bit matrix products on tcgen05 with a fused epilogue.
+//
+// Operands go from global to shared memory by TMA as 128-byte-swizzled panels
+// of 64 contiguous elements, whichever of the two dimensions is contiguous:
+//   k contiguous:      one panel of (tile rows) x 64 k, 128 bytes a row;
+//   m or n contiguous: a panel of 64 k rows for every 64 of m or n.
+// The matrix descriptors and the instruction descriptor carry the difference,
+// so the forward product (k, k), the input gradient (k, across) and the weight
+// gradient (across, across) run in the same kernels. TMA fills what lies
+// outside a tensor with zeros, so no size has to be a multiple of anything.
+//
+// Accumulation is fp32 in TMEM; bias, residual and activation are applied in
+// fp32 and each output is rounded once.
+#include "gk_gemm.cuh"
+
+#include <cooperative_groups.h>
+#include <cuda.h>
+
+#include "../../include/gk.h"
+#include "gk_act.cuh"
+#include "gk_launch.cuh"
+#include "gk_tc.cuh"
+
+namespace gk {
+namespace {
+
+namespace cg = cooperative_groups;
+using namespace tc;
+
+constexpr int kBK = 64;  // k elements of a stage: one 128-byte swizzled row
+
+struct Epilogue {
+    void* out;
+    const void* bias;
+    const void* residual;
+    void* pre;
+    int64_t out_ld, residual_ld, pre_ld;
+    int m, n;
+    int activation;
+    int bf16;
+    int aligned;  // every row of out, residual and pre starts on 16 bytes
+};
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+// Descriptor of a 128-byte-swizzled operand whose panels start on 1024 bytes.
+// k contiguous: rows in groups of 8, 1024 bytes apart. m or n contiguous: k in
+// groups of 8 rows, 1024 bytes apart, and panels of 64 m or n, 8192 apart.
+__device__ __forceinline__ uint64_t swizzled_desc(uint32_t addr, int across) {
+    uint64_t d = (uint64_t)((addr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)(across ? 8192 >> 4 : 1) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// Address step of 16 k elements, in 16-byte units.
+__device__ __forceinline__ uint32_t k_step(int across) { return across ? 16 * 128 / 16 : 32 / 16; }
+
+__host__ __device__ constexpr uint32_t idesc16(int m, int n, int bf16, int a_across, int b_across) {
+    return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)a_across << 15) |
+           ((uint32_t)b_across << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// Load an operand's ROWS x 64 stage: (mn, k) is its first element.
+template <int ROWS>
+__device__ __forceinline__ void load_stage(uint32_t dst, const CUtensorMap* map, int across, int mn, int k,
+                                           uint32_t bar) {
+    if (across) {
+#pragma unroll
+        for (int p = 0; p < ROWS / 64; ++p) tma_load(dst + p * 8192, map, mn + 64 * p, k, bar);
+    } else {
+        tma_load(dst, map, k, mn, bar);
+    }
+}
+
+// ------------------------------------------------------------------ split
+
+// Tiles of 128 x BN, one CTA each; with few tiles a cluster of CTAs shares a
+// tile along k. Every CTA of the cluster leaves its fp32 part in its shared
+// memory, and each then adds up, in rank order, and finishes a share of the
+// tile's rows: no workspace, no atomics, one launch.
+// Warp 0 loads, warp 1 issues the MMAs, warps 2-5 drain TMEM, all finish.
+constexpr int kSplitThreads = 192;
+template <int BN>
+struct Split {
+    static constexpr int kStages = 4;
+    static constexpr int kA = 128 * kBK * 2, kB = BN * kBK * 2, kStage = kA + kB;
+    static constexpr int kPitch = BN + 4;  // fp32 row pitch of the part: rows 16 bytes apart modulo the banks
+    static constexpr int kSmem = kStages * kStage + 1024;
+    static_assert(128 * kPitch * 4 <= kStages * kStage, "the part reuses the stages");
+};
+
+template <int BN>
+__global__ void __launch_bounds__(kSplitThreads) gemm_split_kernel(const __grid_constant__ CUtensorMap ta,
+                                                                   const __grid_constant__ CUtensorMap tb,
+                                                                   Epilogue ep, int tiles_n, int k_blocks,
+                                                                   int a_across, int b_across, uint32_t* status) {
+    using S = Split<BN>;
+    extern __shared__ uint8_t raw[];
+    __shared__ alignas(8) uint64_t full[S::kStages], empty[S::kStages], done;
+    __shared__ uint32_t tmem_slot;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t stages = smem_u32(base);
+    const int tile_m = blockIdx.x / tiles_n, m0 = tile_m * 128, n0 = (blockIdx.x - tile_m * tiles_n) * BN;
+    const int kb0 = (int)((int64_t)rank * k_blocks / ranks), kb1 = (int)((int64_t)(rank + 1) * k_blocks / ranks);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) mbar_init(smem_u32(&full[s]), 1), mbar_init(smem_u32(&empty[s]), 1);
+        mbar_init(smem_u32(&done), 1);
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(&tmem_slot), BN);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            bool ok = true;
+            int issued = kb0;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                const int i = kb - kb0, s = i % S::kStages, turn = i / S::kStages;
+                if (turn > 0 && !mbar_wait(smem_u32(&empty[s]), (turn - 1) & 1, status)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t bar = smem_u32(&full[s]), at = stages + s * S::kStage;
+                mbar_expect_tx(bar, S::kStage);
+                load_stage<128>(at, &ta, a_across, m0, kb * kBK, bar);
+                load_stage<BN>(at + S::kA, &tb, b_across, n0, kb * kBK, bar);
+                issued = kb + 1;
+            }
+            // After a wait that gave up: the copies in flight land before the block may end.
+            if (!ok)
+                for (int kb = max(kb0, issued - S::kStages); kb < issued; ++kb) {
+                    const int i = kb - kb0;
+                    mbar_wait(smem_u32(&full[i % S::kStages]), (i / S::kStages) & 1, status);
+                }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = idesc16(128, BN, ep.bf16, a_across, b_across);
+            const uint32_t step_a = k_step(a_across), step_b = k_step(b_across);
+            for (int kb = kb0; kb < kb1; ++kb) {
+                const int i = kb - kb0, s = i % S::kStages, turn = i / S::kStages;
+                if (!mbar_wait(smem_u32(&full[s]), turn & 1, status)) break;
+                tc_fence_after();
+                const uint64_t a = swizzled_desc(stages + s * S::kStage, a_across);
+                const uint64_t b = swizzled_desc(stages + s * S::kStage + S::kA, b_across);
+#pragma unroll
+                for (int j = 0; j < kBK / 16; ++j)
+                    mma_bf16(tmem, a + j * step_a, b + j * step_b, idesc, (i > 0 || j > 0) ? 1u : 0u);
+                mma_commit(smem_u32(&empty[s]));
+            }
+            mma_commit(smem_u32(&done));
+        }
+    }
+    __syncwarp();
+    // Everyone waits for the accumulator: the parts overwrite the stages.
+    mbar_wait(smem_u32(&done), 0, status);
+    tc_fence_after();
+    float* part = reinterpret_cast<float*>(base);
+    if (warp >= 2) {
+        const int quadrant = warp & 3, row = quadrant * 32 + lane;
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) {
+            float v[32];
+            tmem_ld32(tmem + ((uint32_t)(quadrant * 32) << 16) + c, v);
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<float4*>(part + row * S::kPitch + c + i) =
+                    make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
+    }
+    tc_fence_before();
+    if (ranks > 1)
+        cluster.sync();
+    else
+        __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, BN);
+    }
+    const int rows = 128 / ranks, first = rank * rows;
+    const bool bf16 = ep.bf16 != 0;
+    for (int i = threadIdx.x; i < rows * (BN / 4); i += kSplitThreads) {
+        const int r = first + i / (BN / 4), c = (i % (BN / 4)) * 4;
+        const int64_t m = m0 + r;
+        const int n = n0 + c;
+        if (m >= ep.m || n >= ep.n) continue;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < ranks; ++k) {
+            const float* other = ranks > 1 ? cluster.map_shared_rank(part, k) : part;
+            const float4 x = *reinterpret_cast<const float4*>(other + r * S::kPitch + c);
+            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+        }
+        const int count = min(4, ep.n - n);
+        const bool whole = ep.aligned && count == 4;
+        if (ep.bias != nullptr)
+            for (int j = 0; j < count; ++j) v[j] += load16(ep.bias, n + j, bf16);
+        if (ep.residual != nullptr) {
+            if (whole) {
+                const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(ep.residual) +
+                                                               m * ep.residual_ld + n);
+                float lo, hi;
+                unpack16(x.x, bf16, lo, hi);
+                v[0] += lo, v[1] += hi;
+                unpack16(x.y, bf16, lo, hi);
+                v[2] += lo, v[3] += hi;
+            } else {
+                for (int j = 0; j < count; ++j) v[j] += load16(ep.residual, m * ep.residual_ld + n + j, bf16);
+            }
+        }
+        if (ep.pre != nullptr) {
+            if (whole)
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(ep.pre) + m * ep.pre_ld + n) =
+                    make_uint2(pack16(v[0], v[1], bf16), pack16(v[2], v[3], bf16));
+            else
+                for (int j = 0; j < count; ++j) store16(ep.pre, m * ep.pre_ld + n + j, v[j], bf16);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = act_value(v[j], ep.activation);
+        if (whole)
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(ep.out) + m * ep.out_ld + n) =
+                make_uint2(pack16(v[0], v[1], bf16), pack16(v[2], v[3], bf16));
+        else
+            for (int j = 0; j < count; ++j) store16(ep.out, m * ep.out_ld + n + j, v[j], bf16);
+    }
+    if (ranks > 1) cluster.sync();  // no CTA leaves while another reads its part
+}
+
+// ------------------------------------------------------------------ host
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encoder() {
+    static EncodeFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+// Map of an operand of `mn` rows (or columns, if across) by k; a box is 64
+// contiguous elements by `rows` (k contiguous) or by 64 k (across).
+bool encode(CUtensorMap* map, const void* p, int64_t ld, int across, int64_t mn, int64_t k, int rows, int dtype) {
+    EncodeFn fn = encoder();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)(across ? mn : k), (cuuint64_t)(across ? k : mn)};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    const cuuint32_t box[2] = {kBK, (cuuint32_t)(across ? kBK : rows)};
+    const cuuint32_t steps[2] = {1, 1};
+    return fn(map, dtype == GK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+              const_cast<void*>(p), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+Epilogue epilogue_of(const GemmArgs& g) {
+    Epilogue e{g.out, g.bias, g.residual, g.pre, g.out_ld, g.residual_ld, g.pre_ld, (int)g.m, (int)g.n,
+               g.activation, g.dtype == GK_BF16, 0};
+    e.aligned = aligned16(g.out) && g.out_ld % 8 == 0 &&
+                (g.residual == nullptr || (aligned16(g.residual) && g.residual_ld % 8 == 0)) &&
+                (g.pre == nullptr || (aligned16(g.pre) && g.pre_ld % 8 == 0));
+    return e;
+}
+
+template <int BN>
+int launch_split(const GemmArgs& g, uint32_t* status, cudaStream_t stream) {
+    using S = Split<BN>;
+    auto* kernel = gemm_split_kernel<BN>;
+    static bool ready[64] = {};
+    if (!once_per_device(ready, [&] {
+            return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) == cudaSuccess;
+        }))
+        return launch_status();
+    CUtensorMap ta, tb;
+    if (!encode(&ta, g.a, g.a_ld, g.a_across, g.m, g.k, 128, g.dtype) ||
+        !encode(&tb, g.b, g.b_ld, g.b_across, g.n, g.k, BN, g.dtype))
+        return GK_EINVAL;
+    const int64_t tiles_m = (g.m + 127) / 128, tiles_n = (g.n + BN - 1) / BN, blocks = (g.k + kBK - 1) / kBK;
+    // Split k until the CTAs fill two to an SM, in parts of four stages or more.
+    int ranks = 1;
+    while (ranks < 8 && tiles_m * tiles_n * ranks * 2 <= 2 * kSmCount && blocks >= ranks * 2 * 4) ranks *= 2;
+    cudaLaunchConfig_t cfg = {};
+    if (tiles_m * tiles_n >= (1ll << 31)) return GK_EINVAL;
+    cfg.gridDim = dim3((unsigned)(tiles_n * tiles_m), 1, (unsigned)ranks);
+    cfg.blockDim = dim3(kSplitThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = ranks;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, ta, tb, epilogue_of(g), (int)tiles_n,
+                                   (int)blocks, g.a_across, g.b_across, status);
+}
+
+}  // namespace
+
+int gemm16(const GemmArgs& g, uint32_t* status, cudaStream_t stream) {
+    if (g.m < 1 || g.n < 1 || g.k < 1 || g.m >= (1ll << 31) || g.n >= (1ll << 31) || g.k >= (1ll << 31))
+        return GK_EINVAL;
+    if (!aligned16(g.a) || !aligned16(g.b) || g.a_ld % 8 != 0 || g.b_ld % 8 != 0) return GK_EINVAL;
+    return launch_split<64>(g, status, stream);
+}
+
+}  // namespace gk

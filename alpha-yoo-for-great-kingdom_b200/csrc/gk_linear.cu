@@ -1,0 +1,654 @@
+// gk_linear.cu - the linear operator y = act(x W^T + b + r) and its gradients.
+//
+//   dz = dy act'(z),  dr = dz,  db = sum_m dz,  dx = dz W,  dW = dz^T x
+//
+// 16-bit types run their three products on tcgen05 (gk_gemm.cu). fp32 runs on
+// the fp32 units: its callers train the network's heads in fp32, and one tf32
+// or bf16 product would lose the bits that they keep fp32 for. A product with
+// at most eight rows reads each weight once and is bound by that: it runs as
+// dot products on the cores whatever the type.
+#include <cooperative_groups.h>
+
+#include <type_traits>
+
+#include "../../include/gk.h"
+#include "gk_act.cuh"
+#include "gk_gemm.cuh"
+#include "gk_launch.cuh"
+
+namespace gk {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kFewRows = 8;
+
+template <typename T>
+constexpr int kVec = 16 / (int)sizeof(T);
+
+// ------------------------------------------------------------ few rows
+
+struct FewRows {
+    const void* x;
+    const void* w;
+    const void* bias;
+    const void* residual;
+    void* y;
+    void* pre;
+    int64_t x_stride, w_stride, residual_stride;
+    int m, n;
+    int64_t k;
+    int activation;
+    int k_parts;  // warps that share an output along k: 1, 2, 4 or 8
+};
+
+// A warp (or k_parts of them) takes R rows of W; its lanes run along k, 16
+// bytes of each row at a time where V > 1, and every value of W meets the M
+// rows of x (held by L1) in registers.
+template <typename T, int M, int R, int V>
+__global__ void __launch_bounds__(256) linear_few_kernel(FewRows p) {
+    __shared__ float parts[8][R * M];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int teams = 8 / p.k_parts, team = warp / p.k_parts, part = warp % p.k_parts;
+    const int64_t n0 = ((int64_t)blockIdx.x * teams + team) * R;
+    const T* x = static_cast<const T*>(p.x);
+    const T* w = static_cast<const T*>(p.w);
+    float acc[R][M];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int m = 0; m < M; ++m) acc[r][m] = 0.0f;
+    const T* wr[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) wr[r] = w + (n0 + r < p.n ? n0 + r : p.n - 1) * p.w_stride;
+    const int64_t step = (int64_t)32 * V * p.k_parts;
+#pragma unroll 2
+    for (int64_t k = ((int64_t)part * 32 + lane) * V; k < p.k; k += step) {
+        alignas(16) T wv[R][V];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if constexpr (V > 1)
+                *reinterpret_cast<uint4*>(wv[r]) = __ldcs(reinterpret_cast<const uint4*>(wr[r] + k));
+            else
+                wv[r][0] = wr[r][k];
+        }
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            if (m >= p.m) break;
+            alignas(16) T xv[V];
+            if constexpr (V > 1)
+                *reinterpret_cast<uint4*>(xv) = __ldg(reinterpret_cast<const uint4*>(x + m * p.x_stride + k));
+            else
+                xv[0] = x[m * p.x_stride + k];
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[r][m] = fmaf(as_float<T>(wv[r][i]), as_float<T>(xv[i]), acc[r][m]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            float v = acc[r][m];
+#pragma unroll
+            for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+            if (lane == 0) parts[warp][r * M + m] = v;
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < teams * R * M; i += 256) {
+        const int t = i / (R * M), r = (i / M) % R, m = i % M;
+        const int64_t n = ((int64_t)blockIdx.x * teams + t) * R + r;
+        if (n >= p.n || m >= p.m) continue;
+        float v = 0.0f;
+        for (int q = 0; q < p.k_parts; ++q) v += parts[t * p.k_parts + q][r * M + m];
+        if (p.bias != nullptr) v += as_float<T>(static_cast<const T*>(p.bias)[n]);
+        if (p.residual != nullptr) v += as_float<T>(static_cast<const T*>(p.residual)[m * p.residual_stride + n]);
+        if (p.pre != nullptr) static_cast<T*>(p.pre)[(int64_t)m * p.n + n] = rounded<T>(v);
+        static_cast<T*>(p.y)[(int64_t)m * p.n + n] = rounded<T>(act_value(v, p.activation));
+    }
+}
+
+template <typename T>
+bool rows_aligned(const void* p, int64_t stride) {
+    return aligned16(p) && stride % kVec<T> == 0;
+}
+
+template <typename T, int M>
+int few_rows(FewRows p, cudaStream_t s) {
+    const bool vec = p.k % kVec<T> == 0 && rows_aligned<T>(p.x, p.x_stride) && rows_aligned<T>(p.w, p.w_stride);
+    // Four rows of W a warp, for the loads in flight and the reuse of x; fewer
+    // outputs than that keeps busy are split along k over the block's warps.
+    const int64_t warps = (p.n + 3) / 4;
+    p.k_parts = 1;
+    while (p.k_parts < 8 && warps * p.k_parts < 16 * kSmCount && p.k >= (int64_t)p.k_parts * 2 * 32 * kVec<T>)
+        p.k_parts *= 2;
+    const int64_t per_block = 4 * (8 / p.k_parts);
+    const unsigned grid = (unsigned)((p.n + per_block - 1) / per_block);
+    if (vec)
+        linear_few_kernel<T, M, 4, kVec<T>><<<grid, 256, 0, s>>>(p);
+    else
+        linear_few_kernel<T, M, 4, 1><<<grid, 256, 0, s>>>(p);
+    return launch_status();
+}
+
+// ------------------------------------------------------------ fp32 products
+
+struct Gemm32 {
+    const float* a;
+    const float* b;
+    int64_t a_row, a_k, b_row, b_k;  // strides of A[m, k] and B[n, k]; one of each pair is 1
+    float* out;
+    const float* bias;
+    const float* residual;
+    float* pre;
+    int64_t out_ld, residual_ld, pre_ld;
+    int64_t m, n, k;
+    int activation;
+};
+
+// A tile of B x B outputs, 256 threads of (B/16)^2 outputs each, k in steps of
+// 16 through two shared-memory buffers with the next step in registers. With
+// few tiles a cluster of CTAs shares one along k and adds the parts up in rank
+// order through distributed shared memory.
+constexpr int kStep = 16;
+template <int B>
+constexpr int kGemm32Smem = (B * (B + 4) > 4 * kStep * (B + 4) ? B * (B + 4) : 4 * kStep * (B + 4)) * 4;
+
+// One operand's B x 16 step: thread t takes elements (row, k) along whichever is contiguous.
+template <int B>
+struct Loader32 {
+    static constexpr int kEach = B * kStep / 256;
+    float v[kEach];
+    __device__ __forceinline__ static void place(int t, int i, bool k_contiguous, int& row, int& k) {
+        const int e = t + i * 256;
+        if (k_contiguous)
+            k = e % kStep, row = e / kStep;
+        else
+            row = e % B, k = e / B;
+    }
+    __device__ __forceinline__ void fetch(const float* p, int64_t s_row, int64_t s_k, int64_t row0, int64_t rows,
+                                          int64_t k0, int64_t k_end, int t) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            int row, k;
+            place(t, i, s_k == 1, row, k);
+            const bool in = row0 + row < rows && k0 + k < k_end;
+            v[i] = in ? __ldg(p + (row0 + row) * s_row + (k0 + k) * s_k) : 0.0f;
+        }
+    }
+    __device__ __forceinline__ void store(float (*tile)[B + 4], bool k_contiguous, int t) const {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            int row, k;
+            place(t, i, k_contiguous, row, k);
+            tile[k][row] = v[i];
+        }
+    }
+};
+
+template <int B>
+__global__ void __launch_bounds__(256) gemm32_kernel(Gemm32 g, int tiles_n) {
+    extern __shared__ float smem[];
+    constexpr int E = B / 16, kPitch = B + 4;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    float(*as)[kPitch] = reinterpret_cast<float(*)[kPitch]>(smem);                      // [2 * kStep]
+    float(*bs)[kPitch] = reinterpret_cast<float(*)[kPitch]>(smem + 2 * kStep * kPitch);  // [2 * kStep]
+    const int t = threadIdx.x, tx = t % 16, ty = t / 16;
+    const int64_t tile_m = blockIdx.x / tiles_n, tile_n = blockIdx.x - tile_m * tiles_n;
+    const int64_t m0 = tile_m * B, n0 = tile_n * B;
+    const int64_t steps = (g.k + kStep - 1) / kStep;
+    const int64_t s0 = steps * rank / ranks, s1 = steps * (rank + 1) / ranks;
+    float acc[E][E];
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+        for (int j = 0; j < E; ++j) acc[i][j] = 0.0f;
+    Loader32<B> la, lb;
+    la.fetch(g.a, g.a_row, g.a_k, m0, g.m, s0 * kStep, g.k, t);
+    lb.fetch(g.b, g.b_row, g.b_k, n0, g.n, s0 * kStep, g.k, t);
+    for (int64_t s = s0; s < s1; ++s) {
+        const int buf = (int)((s - s0) & 1) * kStep;
+        la.store(as + buf, g.a_k == 1, t);
+        lb.store(bs + buf, g.b_k == 1, t);
+        __syncthreads();
+        if (s + 1 < s1) {
+            la.fetch(g.a, g.a_row, g.a_k, m0, g.m, (s + 1) * kStep, g.k, t);
+            lb.fetch(g.b, g.b_row, g.b_k, n0, g.n, (s + 1) * kStep, g.k, t);
+        }
+#pragma unroll
+        for (int k = 0; k < kStep; ++k) {
+            float a[E], b[E];
+#pragma unroll
+            for (int q = 0; q < E / 4; ++q) {
+                *reinterpret_cast<float4*>(a + 4 * q) = *reinterpret_cast<float4*>(&as[buf + k][64 * q + ty * 4]);
+                *reinterpret_cast<float4*>(b + 4 * q) = *reinterpret_cast<float4*>(&bs[buf + k][64 * q + tx * 4]);
+            }
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+#pragma unroll
+                for (int j = 0; j < E; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+        for (int q = 0; q < E / 4; ++q)
+            *reinterpret_cast<float4*>(smem + (64 * (i / 4) + ty * 4 + i % 4) * kPitch + 64 * q + tx * 4) =
+                make_float4(acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]);
+    if (ranks > 1)
+        cluster.sync();
+    else
+        __syncthreads();
+    const int rows = B / ranks, first = rank * rows;
+    for (int i = t; i < rows * B; i += 256) {
+        const int r = first + i / B, c = i % B;
+        const int64_t m = m0 + r, n = n0 + c;
+        if (m >= g.m || n >= g.n) continue;
+        float v = 0.0f;
+        for (int k = 0; k < ranks; ++k)
+            v += (ranks > 1 ? cluster.map_shared_rank(smem, k) : smem)[r * kPitch + c];
+        if (g.bias != nullptr) v += g.bias[n];
+        if (g.residual != nullptr) v += g.residual[m * g.residual_ld + n];
+        if (g.pre != nullptr) g.pre[m * g.pre_ld + n] = v;
+        g.out[m * g.out_ld + n] = act_value(v, g.activation);
+    }
+    if (ranks > 1) cluster.sync();  // no CTA leaves while another reads its part
+}
+
+template <int B>
+int launch_gemm32(const Gemm32& g, cudaStream_t s) {
+    auto* kernel = gemm32_kernel<B>;
+    static bool ready[64] = {};
+    if (!once_per_device(ready, [&] {
+            return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemm32Smem<B>) ==
+                   cudaSuccess;
+        }))
+        return launch_status();
+    const int64_t tiles_n = (g.n + B - 1) / B, tiles = (g.m + B - 1) / B * tiles_n;
+    if (tiles >= (1ll << 31)) return GK_EINVAL;
+    const int64_t steps = (g.k + kStep - 1) / kStep;
+    int ranks = 1;  // parts of four steps or more, until the CTAs fill two to an SM
+    while (ranks < 8 && tiles * ranks * 2 <= 2 * kSmCount && steps >= ranks * 2 * 4) ranks *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)tiles, 1, (unsigned)ranks);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = kGemm32Smem<B>;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = ranks;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, g, (int)tiles_n);
+}
+
+int gemm32(const Gemm32& g, cudaStream_t s) {
+    // The larger tile once its CTAs fill the SMs: half the shared-memory traffic a product.
+    const int64_t large = ((g.m + 127) / 128) * ((g.n + 127) / 128);
+    return large >= kSmCount ? launch_gemm32<128>(g, s) : launch_gemm32<64>(g, s);
+}
+
+// ------------------------------------------------------------ dz and db
+
+struct Slope {
+    const void* dy;
+    const void* kept;  // [m, n] contiguous, or nullptr without activation
+    void* dz;          // or nullptr: sums only
+    float* sums;       // [slabs, n] column sums of each slab of rows, or nullptr
+    int64_t dy_stride, dz_stride;
+    int64_t m, n, slab;  // rows of a slab
+    int activation;
+};
+
+// 32 lanes of V columns by 8 rows at a time down a slab of rows.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) linear_slope_kernel(Slope p) {
+    __shared__ float sums[8][32 * V];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * V, r0 = (int64_t)blockIdx.y * p.slab;
+    const int64_t r1 = r0 + p.slab < p.m ? r0 + p.slab : p.m;
+    float sum[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = 0.0f;
+    if (c < p.n) {
+#pragma unroll 4
+        for (int64_t r = r0 + warp; r < r1; r += 8) {
+            alignas(16) T dy[V], kept[V];
+            const T* dyp = static_cast<const T*>(p.dy) + r * p.dy_stride + c;
+            const T* keptp = static_cast<const T*>(p.kept) + r * p.n + c;
+            if constexpr (V > 1)
+                *reinterpret_cast<uint4*>(dy) = __ldg(reinterpret_cast<const uint4*>(dyp));
+            else
+                dy[0] = *dyp;
+            if (p.kept != nullptr) {
+                if constexpr (V > 1)
+                    *reinterpret_cast<uint4*>(kept) = __ldg(reinterpret_cast<const uint4*>(keptp));
+                else
+                    kept[0] = *keptp;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float z = as_float<T>(dy[i]) * act_slope(as_float<T>(kept[i]), p.activation);
+                    sum[i] += z;
+                    dy[i] = rounded<T>(z);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum[i] += as_float<T>(dy[i]);
+            }
+            if (p.dz != nullptr) {
+                T* dz = static_cast<T*>(p.dz) + r * p.dz_stride + c;
+                if constexpr (V > 1)
+                    *reinterpret_cast<uint4*>(dz) = *reinterpret_cast<uint4*>(dy);
+                else
+                    *dz = dy[0];
+            }
+        }
+    }
+    if (p.sums == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < V; ++i) sums[warp][lane * V + i] = sum[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * V; i += 256) {
+        const int64_t col = (int64_t)blockIdx.x * 32 * V + i;
+        if (col >= p.n) break;
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) v += sums[w][i];
+        p.sums[(int64_t)blockIdx.y * p.n + col] = v;
+    }
+}
+
+// db from the slabs' sums, in their order.
+template <typename T>
+__global__ void __launch_bounds__(256) linear_bias_kernel(const float* sums, int64_t n, int slabs, T* db) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= n) return;
+    float v = 0.0f;
+    for (int s = 0; s < slabs; ++s) v += sums[(int64_t)s * n + c];
+    db[c] = rounded<T>(v);
+}
+
+struct SlopePlan {
+    int vec, slabs;
+    int64_t slab, col_blocks;
+};
+template <typename T>
+SlopePlan slope_plan(int64_t m, int64_t n, bool vec) {
+    SlopePlan p{};
+    p.vec = vec ? kVec<T> : 1;
+    p.col_blocks = (n + 32 * p.vec - 1) / (32 * p.vec);
+    // Slabs of 32 rows or more, until there are eight blocks an SM.
+    int64_t slabs = (8 * kSmCount + p.col_blocks - 1) / p.col_blocks;
+    if (slabs > (m + 31) / 32) slabs = (m + 31) / 32;
+    if (slabs < 1) slabs = 1;
+    p.slab = (m + slabs - 1) / slabs;
+    p.slabs = (int)((m + p.slab - 1) / p.slab);
+    return p;
+}
+
+// Rows of a 16-bit matrix to rows that start on 16 bytes, as TMA needs them.
+__global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* from, int64_t stride, int64_t rows,
+                                                         int64_t cols, uint16_t* to, int64_t to_stride) {
+    // A thread makes one 16-byte chunk; its eight loads are in flight together.
+    const int64_t chunks = to_stride / 8, items = rows * chunks;
+    for (int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x; it < items; it += (int64_t)gridDim.x * 256) {
+        const int64_t r = it / chunks, c = (it - r * chunks) * 8;
+        alignas(16) uint16_t v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? __ldg(from + r * stride + c + i) : (uint16_t)0;
+        *reinterpret_cast<uint4*>(to + r * to_stride + c) = *reinterpret_cast<uint4*>(v);
+    }
+}
+
+// ------------------------------------------------------------ workspaces
+
+int64_t pad8(int64_t n) { return (n + 7) & ~(int64_t)7; }
+
+struct Arena {
+    uint8_t* base;
+    size_t used = 0;
+    explicit Arena(void* p) : base(static_cast<uint8_t*>(p)) {}
+    void* take(int64_t bytes) {
+        void* p = base == nullptr ? nullptr : base + used;
+        used += ((size_t)bytes + 255) & ~(size_t)255;
+        return p;
+    }
+};
+
+bool sizes_ok(int64_t m, int64_t n, int64_t k, int dtype, int activation) {
+    const int64_t most = (1ll << 31) - 1;
+    return m >= 0 && n >= 1 && k >= 1 && m <= most && n <= most && k <= most && dtype >= GK_FP32 &&
+           dtype <= GK_FP16 && activation >= GK_ACT_NONE && activation <= GK_ACT_SILU;
+}
+
+bool tma_rows(const void* p, int64_t stride, int64_t cols) {
+    return aligned16(p) && stride % 8 == 0 && stride >= cols;
+}
+
+// The matrix itself if TMA can read its rows, else an aligned copy in the arena.
+struct Operand {
+    const void* p;
+    int64_t ld;
+    bool copied;
+};
+Operand operand(Arena& arena, const void* p, int64_t stride, int64_t rows, int64_t cols) {
+    if (tma_rows(p, stride, cols)) return {p, stride, false};
+    return {arena.take(rows * pad8(cols) * 2), pad8(cols), true};
+}
+int copy_if_needed(const Operand& o, const void* p, int64_t stride, int64_t rows, int64_t cols, cudaStream_t s) {
+    if (!o.copied) return 0;
+    const int64_t items = rows * (o.ld / 8);
+    align_rows_kernel<<<blocks_for(items, 256, kSmCount * 32), 256, 0, s>>>(
+        static_cast<const uint16_t*>(p), stride, rows, cols, static_cast<uint16_t*>(const_cast<void*>(o.p)), o.ld);
+    return launch_status();
+}
+
+struct ForwardPlan {
+    Operand x, w;
+    size_t bytes;
+    bool few;
+};
+ForwardPlan forward_plan(const gk_linear_t& p, void* workspace) {
+    ForwardPlan f{};
+    Arena arena(workspace);
+    f.few = p.m <= kFewRows;
+    if (!f.few && p.dtype != GK_FP32) {
+        f.x = operand(arena, p.x, p.x_stride, p.m, p.k);
+        f.w = operand(arena, p.w, p.w_stride, p.n, p.k);
+    }
+    f.bytes = arena.used;
+    return f;
+}
+
+template <typename T>
+int few_rows_by_m(const FewRows& f, cudaStream_t s) {
+    if (f.m <= 1) return few_rows<T, 1>(f, s);
+    if (f.m <= 4) return few_rows<T, 4>(f, s);
+    return few_rows<T, 8>(f, s);
+}
+
+bool forward_ok(const gk_linear_t* p) {
+    if (p == nullptr || !sizes_ok(p->m, p->n, p->k, p->dtype, p->activation)) return false;
+    if (p->m == 0) return true;
+    return p->x != nullptr && p->w != nullptr && p->y != nullptr && p->x_stride >= 0 && p->w_stride >= 0 &&
+           (p->residual == nullptr || p->residual_stride >= 0);
+}
+
+struct BackwardPlan {
+    bool forms_dz;    // dz is another matrix than dy
+    Operand x, w, dz;
+    void* unpacked;   // x from its codes
+    int64_t unpacked_ld;
+    float* sums;
+    SlopePlan slope;
+    bool runs_slope;
+    size_t bytes;
+};
+
+template <typename T>
+BackwardPlan backward_plan(const gk_linear_grad_t& p, void* workspace) {
+    constexpr bool k16 = sizeof(T) == 2;
+    BackwardPlan b{};
+    Arena arena(workspace);
+    const bool products = p.dx != nullptr || p.dw != nullptr;
+    // Without an activation dz is dy, unless the product needs its rows aligned.
+    b.forms_dz = p.activation != GK_ACT_NONE || (k16 && products && !tma_rows(p.dy, p.dy_stride, p.n));
+    b.dz = {p.dy, p.dy_stride, false};
+    if (b.forms_dz) {
+        // The residual's gradient serves as dz where its rows are aligned.
+        if (p.dz != nullptr && (!k16 || p.n % 8 == 0))
+            b.dz = {p.dz, p.n, false};
+        else
+            b.dz = {arena.take(p.m * pad8(p.n) * (int64_t)sizeof(T)), pad8(p.n), false};
+    }
+    if (p.dw != nullptr && p.x_codes != nullptr) {
+        b.unpacked_ld = k16 ? pad8(p.k) : p.k;
+        b.unpacked = arena.take(p.m * b.unpacked_ld * (int64_t)sizeof(T));
+    }
+    if (k16) {
+        if (p.dw != nullptr && p.x_codes == nullptr) b.x = operand(arena, p.x, p.x_stride, p.m, p.k);
+        if (p.dx != nullptr) b.w = operand(arena, p.w, p.w_stride, p.n, p.k);
+    } else {
+        b.x = {p.x, p.x_stride, false};
+        b.w = {p.w, p.w_stride, false};
+    }
+    if (b.unpacked_ld > 0) b.x = {b.unpacked, b.unpacked_ld, false};
+    b.runs_slope = b.forms_dz || p.db != nullptr;
+    const bool vec = aligned16(p.dy) && p.dy_stride % kVec<T> == 0 && p.n % kVec<T> == 0 &&
+                     (p.kept == nullptr || aligned16(p.kept)) && (p.dz == nullptr || aligned16(p.dz));
+    b.slope = slope_plan<T>(p.m, p.n, vec);
+    if (p.db != nullptr) b.sums = static_cast<float*>(arena.take((int64_t)b.slope.slabs * p.n * 4));
+    b.bytes = arena.used;
+    return b;
+}
+
+bool backward_ok(const gk_linear_grad_t* p) {
+    if (p == nullptr || !sizes_ok(p->m, p->n, p->k, p->dtype, p->activation) || p->m < 1) return false;
+    if (p->dy == nullptr || p->dy_stride < 0) return false;
+    if (p->activation != GK_ACT_NONE && p->kept == nullptr) return false;
+    if (p->activation == GK_ACT_NONE && p->dz != nullptr) return false;
+    if (p->dx != nullptr && (p->w == nullptr || p->w_stride < 0)) return false;
+    if (p->dw != nullptr && p->x == nullptr && (p->x_codes == nullptr || p->x_scales == nullptr)) return false;
+    return true;
+}
+
+template <typename T>
+int backward(const gk_linear_grad_t& p, void* workspace, uint32_t* status, cudaStream_t s) {
+    constexpr bool k16 = sizeof(T) == 2;
+    const BackwardPlan b = backward_plan<T>(p, workspace);
+    int e = 0;
+    if (b.runs_slope) {
+        Slope a{p.dy, p.activation == GK_ACT_NONE ? nullptr : p.kept,
+                b.forms_dz ? const_cast<void*>(b.dz.p) : nullptr, b.sums, p.dy_stride, b.dz.ld, p.m, p.n,
+                b.slope.slab, p.activation};
+        const dim3 grid((unsigned)b.slope.col_blocks, (unsigned)b.slope.slabs);
+        if (b.slope.vec > 1)
+            linear_slope_kernel<T, kVec<T>><<<grid, 256, 0, s>>>(a);
+        else
+            linear_slope_kernel<T, 1><<<grid, 256, 0, s>>>(a);
+        if ((e = launch_status()) != 0) return e;
+        if (p.db != nullptr) {
+            linear_bias_kernel<T><<<(unsigned)((p.n + 255) / 256), 256, 0, s>>>(b.sums, p.n, b.slope.slabs,
+                                                                                 static_cast<T*>(p.db));
+            if ((e = launch_status()) != 0) return e;
+        }
+    }
+    if (p.dz != nullptr && b.dz.p != p.dz) {
+        // dz lies in aligned rows of the workspace; the residual's gradient has rows of n.
+        const cudaError_t c = cudaMemcpy2DAsync(p.dz, p.n * sizeof(T), b.dz.p, b.dz.ld * sizeof(T),
+                                                p.n * sizeof(T), p.m, cudaMemcpyDeviceToDevice, s);
+        if (c != cudaSuccess) return (int)c;
+    }
+    if (p.dw != nullptr && p.x_codes != nullptr) {
+        e = gk_unpack(p.x_codes, p.x_scales, p.m, p.k, b.unpacked, b.unpacked_ld, p.dtype, s);
+        if (e != 0) return e;
+    }
+    if constexpr (k16) {
+        if (p.dx != nullptr) {
+            if ((e = copy_if_needed(b.w, p.w, p.w_stride, p.n, p.k, s)) != 0) return e;
+            GemmArgs g{b.dz.p, b.w.p, b.dz.ld, b.w.ld, 0, 1, p.dx, p.k, nullptr, nullptr, 0, nullptr, 0,
+                       p.m, p.k, p.n, p.dtype, GK_ACT_NONE};
+            if ((e = gemm16(g, status, s)) != 0) return e;
+        }
+        if (p.dw != nullptr) {
+            if (p.x_codes == nullptr && (e = copy_if_needed(b.x, p.x, p.x_stride, p.m, p.k, s)) != 0) return e;
+            GemmArgs g{b.dz.p, b.x.p, b.dz.ld, b.x.ld, 1, 1, p.dw, p.k, nullptr, nullptr, 0, nullptr, 0,
+                       p.n, p.k, p.m, p.dtype, GK_ACT_NONE};
+            if ((e = gemm16(g, status, s)) != 0) return e;
+        }
+    } else {
+        const float* dz = static_cast<const float*>(b.dz.p);
+        if (p.dx != nullptr) {
+            Gemm32 g{dz, static_cast<const float*>(b.w.p), b.dz.ld, 1, 1, b.w.ld, static_cast<float*>(p.dx),
+                     nullptr, nullptr, nullptr, p.k, 0, 0, p.m, p.k, p.n, GK_ACT_NONE};
+            if ((e = gemm32(g, s)) != 0) return e;
+        }
+        if (p.dw != nullptr) {
+            Gemm32 g{dz, static_cast<const float*>(b.x.p), 1, b.dz.ld, 1, b.x.ld, static_cast<float*>(p.dw),
+                     nullptr, nullptr, nullptr, p.k, 0, 0, p.n, p.k, p.m, GK_ACT_NONE};
+            if ((e = gemm32(g, s)) != 0) return e;
+        }
+    }
+    return 0;
+}
+
+}  // namespace
+}  // namespace gk
+
+extern "C" {
+
+size_t gk_linear_workspace_bytes(const gk_linear_t* p) {
+    return gk::forward_ok(p) && p->m > 0 ? gk::forward_plan(*p, nullptr).bytes : 0;
+}
+
+int gk_linear_forward(const gk_linear_t* p, void* workspace, uint32_t* status, void* stream) {
+    using namespace gk;
+    if (!forward_ok(p) || status == nullptr) return GK_EINVAL;
+    if (p->m == 0) return 0;
+    const ForwardPlan f = forward_plan(*p, workspace);
+    if (f.bytes > 0 && workspace == nullptr) return GK_EINVAL;
+    cudaStream_t s = as_stream(stream);
+    if (f.few) {
+        FewRows r{p->x, p->w, p->bias, p->residual, p->y, p->pre, p->x_stride, p->w_stride, p->residual_stride,
+                  (int)p->m, (int)p->n, p->k, p->activation, 1};
+        if (p->dtype == GK_FP32) return few_rows_by_m<float>(r, s);
+        if (p->dtype == GK_BF16) return few_rows_by_m<__nv_bfloat16>(r, s);
+        return few_rows_by_m<__half>(r, s);
+    }
+    if (p->dtype == GK_FP32) {
+        Gemm32 g{static_cast<const float*>(p->x), static_cast<const float*>(p->w), p->x_stride, 1, p->w_stride, 1,
+                 static_cast<float*>(p->y), static_cast<const float*>(p->bias),
+                 static_cast<const float*>(p->residual), static_cast<float*>(p->pre), p->n, p->residual_stride, p->n,
+                 p->m, p->n, p->k, p->activation};
+        return gemm32(g, s);
+    }
+    int e = copy_if_needed(f.x, p->x, p->x_stride, p->m, p->k, s);
+    if (e == 0) e = copy_if_needed(f.w, p->w, p->w_stride, p->n, p->k, s);
+    if (e != 0) return e;
+    GemmArgs g{f.x.p, f.w.p, f.x.ld, f.w.ld, 0, 0, p->y, p->n, p->bias, p->residual, p->residual_stride, p->pre, p->n,
+               p->m, p->n, p->k, p->dtype, p->activation};
+    return gemm16(g, status, s);
+}
+
+size_t gk_linear_grad_workspace_bytes(const gk_linear_grad_t* p) {
+    using namespace gk;
+    if (!backward_ok(p)) return 0;
+    return p->dtype == GK_FP32 ? backward_plan<float>(*p, nullptr).bytes : backward_plan<__half>(*p, nullptr).bytes;
+}
+
+int gk_linear_backward(const gk_linear_grad_t* p, void* workspace, uint32_t* status, void* stream) {
+    using namespace gk;
+    if (!backward_ok(p) || status == nullptr) return GK_EINVAL;
+    if (workspace == nullptr && gk_linear_grad_workspace_bytes(p) > 0) return GK_EINVAL;
+    cudaStream_t s = as_stream(stream);
+    if (p->dtype == GK_FP32) return backward<float>(*p, workspace, status, s);
+    if (p->dtype == GK_BF16) return backward<__nv_bfloat16>(*p, workspace, status, s);
+    return backward<__half>(*p, workspace, status, s);
+}
+
+}  // extern "C"

@@ -1,0 +1,246 @@
+// gk_pack.cu - activations kept in 8 bits for the backward pass.
+//
+// A block of 32 values shares a power-of-two scale 2^s with
+// 448 2^(s-1) < max |x| <= 448 2^s, so a value x is held as e4m3(x 2^-s): three
+// fraction bits (relative step 2^-4) down to max |x| 2^-15, then evenly spaced
+// to 2^-18 of the maximum, below which it is held as zero. The scale being a
+// power of two, every held value is a bf16, fp16 and fp32 value: unpacking
+// rounds nothing. Memory traffic bounds both directions.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/gk.h"
+#include "gk_act.cuh"
+#include "gk_launch.cuh"
+
+namespace gk {
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kBlock = 32;
+
+template <typename T>
+constexpr int kLowest = -124;  // least scale exponent: the smallest step 2^(s-9) is a value of T
+template <>
+constexpr int kLowest<__half> = -15;
+template <typename T>
+constexpr float kLargest = 3.4028234663852886e38f;
+template <>
+constexpr float kLargest<__half> = 65504.0f;
+template <>
+constexpr float kLargest<__nv_bfloat16> = 3.3895313892515355e38f;
+
+// The scale exponent for a block whose largest finite magnitude is `top`.
+template <typename T>
+__device__ __forceinline__ int scale_exponent(float top) {
+    if (top == 0.0f) return max(0, kLowest<T>);
+    // top = f 2^e, 1 <= f < 2; 448 = 1.75 2^8. (A subnormal top counts as e = -127, which the least scale covers.)
+    const uint32_t bits = __float_as_uint(top);
+    const int e = (int)(bits >> 23) - 127;
+    return max(kLowest<T>, (bits & 0x7fffffu) > 0x600000u ? e - 7 : e - 8);
+}
+
+__device__ __forceinline__ float finite_magnitude(float x) {
+    const float a = fabsf(x);
+    return a <= 3.4028234663852886e38f ? a : 0.0f;  // also false for NaN
+}
+
+__device__ __forceinline__ uint32_t code_of(float x, float inverse) {
+    if (!(fabsf(x) <= 3.4028234663852886e38f)) return 0x7fu;
+    return __nv_cvt_float_to_fp8(x * inverse, __NV_SATFINITE, __NV_E4M3);
+}
+
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// The value of a code: the code's four exponent and three fraction bits under
+// a float's exponent, times 2^120 for the difference of the biases.
+__device__ __forceinline__ float value_of(uint32_t code) {
+    const uint32_t magnitude = code & 0x7fu;
+    if (magnitude == 0x7fu) return __uint_as_float(0x7fc00000u);
+    const float v = __uint_as_float(magnitude << 20) * 1.329227995784916e36f;
+    return __uint_as_float(__float_as_uint(v) | ((code & 0x80u) << 24));
+}
+
+template <typename T>
+__device__ __forceinline__ T held(uint32_t code, float scale) {
+    const float v = value_of(code) * scale;
+    const float most = kLargest<T>;
+    return rounded<T>(v > most ? most : (v < -most ? -most : v));
+}
+
+// A lane an element, a warp a block of 32.
+template <typename T>
+__global__ void __launch_bounds__(256) pack_rows_kernel(const T* x, int64_t stride, int64_t rows, int64_t cols,
+                                                        uint8_t* codes, uint8_t* scales) {
+    const int lane = threadIdx.x & 31;
+    const int64_t per_row = (cols + kBlock - 1) / kBlock, items = rows * per_row;
+    const int64_t warps = (int64_t)gridDim.x * 8;
+    for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += warps) {
+        const int64_t r = it / per_row, b = it - r * per_row, c = b * kBlock + lane;
+        const float v = c < cols ? as_float<T>(x[r * stride + c]) : 0.0f;
+        float top = finite_magnitude(v);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+        const int s = scale_exponent<T>(top);
+        if (c < cols) codes[r * cols + c] = (uint8_t)code_of(v, power_of_two(-s));
+        if (lane == 0) scales[it] = (uint8_t)(s + 127);
+    }
+}
+
+// Whole blocks of aligned rows: 16 bytes a thread, 32 * sizeof(T) / 16 threads
+// a block of 32, four vectors a thread in flight.
+template <typename T>
+__global__ void __launch_bounds__(256) pack_vectors_kernel(const T* x, int64_t vectors, uint8_t* codes,
+                                                           uint8_t* scales) {
+    constexpr int V = 16 / (int)sizeof(T), kTeam = kBlock / V, kUnroll = 4;
+    const int64_t start = (int64_t)blockIdx.x * (256 * kUnroll) + threadIdx.x;
+    uint4 raw[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const int64_t i = start + u * 256;
+        raw[u] = i < vectors ? __ldcs(reinterpret_cast<const uint4*>(x) + i) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const int64_t i = start + u * 256;
+        const T* v = reinterpret_cast<const T*>(&raw[u]);
+        float top = 0.0f;
+#pragma unroll
+        for (int k = 0; k < V; ++k) top = fmaxf(top, finite_magnitude(as_float<T>(v[k])));
+#pragma unroll
+        for (int o = kTeam / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+        const int s = scale_exponent<T>(top);
+        const float inverse = power_of_two(-s);
+        uint32_t word[V / 4];
+#pragma unroll
+        for (int k = 0; k < V / 4; ++k)
+            word[k] = code_of(as_float<T>(v[4 * k]), inverse) | code_of(as_float<T>(v[4 * k + 1]), inverse) << 8 |
+                      code_of(as_float<T>(v[4 * k + 2]), inverse) << 16 |
+                      code_of(as_float<T>(v[4 * k + 3]), inverse) << 24;
+        if (i < vectors) {
+            if constexpr (V == 4)
+                reinterpret_cast<uint32_t*>(codes)[i] = word[0];
+            else
+                reinterpret_cast<uint2*>(codes)[i] = make_uint2(word[0], word[1]);
+            if ((threadIdx.x & (kTeam - 1)) == 0) scales[i / kTeam] = (uint8_t)(s + 127);
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) unpack_rows_kernel(const uint8_t* codes, const uint8_t* scales, int64_t rows,
+                                                          int64_t cols, T* x, int64_t stride) {
+    const int lane = threadIdx.x & 31;
+    const int64_t per_row = (cols + kBlock - 1) / kBlock, items = rows * per_row;
+    const int64_t warps = (int64_t)gridDim.x * 8;
+    for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += warps) {
+        const int64_t r = it / per_row, c = (it - r * per_row) * kBlock + lane;
+        if (c < cols) x[r * stride + c] = held<T>(codes[r * cols + c], power_of_two((int)scales[it] - 127));
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) unpack_vectors_kernel(const uint8_t* codes, const uint8_t* scales,
+                                                             int64_t vectors, T* x) {
+    constexpr int V = 16 / (int)sizeof(T), kTeam = kBlock / V, kUnroll = 4;
+    const int64_t start = (int64_t)blockIdx.x * (256 * kUnroll) + threadIdx.x;
+    uint32_t word[kUnroll][V / 4];
+    float scale[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const int64_t i = start + u * 256;
+        if (i >= vectors) continue;
+        if constexpr (V == 4) {
+            word[u][0] = __ldcs(reinterpret_cast<const uint32_t*>(codes) + i);
+        } else {
+            const uint2 w = __ldcs(reinterpret_cast<const uint2*>(codes) + i);
+            word[u][0] = w.x, word[u][V / 4 - 1] = w.y;
+        }
+        scale[u] = power_of_two((int)scales[i / kTeam] - 127);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const int64_t i = start + u * 256;
+        if (i >= vectors) continue;
+        alignas(16) T out[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) out[k] = held<T>((word[u][k / 4] >> (8 * (k % 4))) & 0xffu, scale[u]);
+        reinterpret_cast<uint4*>(x)[i] = *reinterpret_cast<uint4*>(out);
+    }
+}
+
+bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
+
+// Rows that follow one another without a gap, in whole blocks: one run of vectors.
+bool one_run(int64_t rows, int64_t cols, int64_t stride) { return cols % kBlock == 0 && (rows == 1 || stride == cols); }
+
+template <typename T>
+int pack(const void* x, int64_t stride, int64_t rows, int64_t cols, uint8_t* codes, uint8_t* scales,
+         cudaStream_t s) {
+    if (one_run(rows, cols, stride) && aligned16(x) && aligned8(codes)) {
+        const int64_t vectors = rows * cols / (16 / (int64_t)sizeof(T));
+        pack_vectors_kernel<T><<<(unsigned)((vectors + 1023) / 1024), 256, 0, s>>>(static_cast<const T*>(x), vectors,
+                                                                                   codes, scales);
+    } else {
+        const int64_t items = rows * ((cols + kBlock - 1) / kBlock);
+        pack_rows_kernel<T><<<blocks_for(items, 8, kSmCount * 32), 256, 0, s>>>(static_cast<const T*>(x), stride,
+                                                                                rows, cols, codes, scales);
+    }
+    return launch_status();
+}
+
+template <typename T>
+int unpack(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* x, int64_t stride,
+           cudaStream_t s) {
+    if (one_run(rows, cols, stride) && aligned16(x) && aligned8(codes)) {
+        const int64_t vectors = rows * cols / (16 / (int64_t)sizeof(T));
+        unpack_vectors_kernel<T><<<(unsigned)((vectors + 1023) / 1024), 256, 0, s>>>(codes, scales, vectors,
+                                                                                     static_cast<T*>(x));
+    } else {
+        const int64_t items = rows * ((cols + kBlock - 1) / kBlock);
+        unpack_rows_kernel<T><<<blocks_for(items, 8, kSmCount * 32), 256, 0, s>>>(codes, scales, rows, cols,
+                                                                                  static_cast<T*>(x), stride);
+    }
+    return launch_status();
+}
+
+// Sizes whose element count, and grid, stay in range.
+bool valid(const void* x, int64_t stride, int64_t rows, int64_t cols, const void* codes, const void* scales) {
+    if (rows < 0 || cols < 0) return false;
+    if (rows == 0 || cols == 0) return true;
+    if (rows > (1ll << 40) / cols || (rows > 1 && stride < cols)) return false;
+    return x != nullptr && codes != nullptr && scales != nullptr;
+}
+
+}  // namespace
+}  // namespace gk
+
+extern "C" {
+
+int gk_pack(const void* x, int64_t stride, int dtype, int64_t rows, int64_t cols, uint8_t* codes, uint8_t* scales,
+            void* stream) {
+    using namespace gk;
+    if (!valid(x, stride, rows, cols, codes, scales) || dtype < GK_FP32 || dtype > GK_FP16) return GK_EINVAL;
+    if (rows == 0 || cols == 0) return 0;
+    cudaStream_t s = as_stream(stream);
+    if (dtype == GK_FP32) return pack<float>(x, stride, rows, cols, codes, scales, s);
+    if (dtype == GK_BF16) return pack<__nv_bfloat16>(x, stride, rows, cols, codes, scales, s);
+    return pack<__half>(x, stride, rows, cols, codes, scales, s);
+}
+
+int gk_unpack(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* x, int64_t stride,
+              int dtype, void* stream) {
+    using namespace gk;
+    if (!valid(x, stride, rows, cols, codes, scales) || dtype < GK_FP32 || dtype > GK_FP16) return GK_EINVAL;
+    if (rows == 0 || cols == 0) return 0;
+    cudaStream_t s = as_stream(stream);
+    if (dtype == GK_FP32) return unpack<float>(codes, scales, rows, cols, x, stride, s);
+    if (dtype == GK_BF16) return unpack<__nv_bfloat16>(codes, scales, rows, cols, x, stride, s);
+    return unpack<__half>(codes, scales, rows, cols, x, stride, s);
+}
+
+}  // extern "C"

@@ -27,6 +27,9 @@ c_float = ctypes.c_float
 c_size_t = ctypes.c_size_t
 
 
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # GK_FP32, GK_BF16, GK_FP16
+
+
 class PuctOptions(ctypes.Structure):
     _fields_ = [("c_puct", c_double), ("dirichlet_epsilon", c_double), ("fpu_enabled", c_int),
                 ("fpu_reduction", c_double)]
@@ -62,7 +65,24 @@ class PolicyLossStruct(ctypes.Structure):
                 ("partials", c_void_p), ("grad", c_void_p)]
 
 
+class LinearStruct(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("w", c_void_p), ("bias", c_void_p), ("residual", c_void_p), ("y", c_void_p),
+                ("pre", c_void_p), ("m", c_int64), ("n", c_int64), ("k", c_int64), ("x_stride", c_int64),
+                ("w_stride", c_int64), ("residual_stride", c_int64), ("dtype", c_int), ("activation", c_int)]
+
+
+class LinearGradStruct(ctypes.Structure):
+    _fields_ = [("dy", c_void_p), ("kept", c_void_p), ("x", c_void_p), ("x_codes", c_void_p), ("x_scales", c_void_p),
+                ("w", c_void_p), ("dx", c_void_p), ("dw", c_void_p), ("db", c_void_p), ("dz", c_void_p),
+                ("m", c_int64), ("n", c_int64), ("k", c_int64), ("dy_stride", c_int64), ("x_stride", c_int64),
+                ("w_stride", c_int64), ("dtype", c_int), ("activation", c_int)]
+
+
 _SIGNATURES = {
+    "gk_linear_forward": [ctypes.POINTER(LinearStruct), c_void_p, c_void_p, c_void_p],
+    "gk_linear_backward": [ctypes.POINTER(LinearGradStruct), c_void_p, c_void_p, c_void_p],
+    "gk_pack": [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
+    "gk_unpack": [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int, c_void_p],
     "gk_policy_loss_parts": [c_int64, c_int64],
     "gk_policy_loss_forward": [ctypes.POINTER(PolicyLossStruct), c_void_p],
     "gk_policy_loss_backward": [ctypes.POINTER(PolicyLossStruct), c_void_p, c_int, c_void_p],
@@ -97,6 +117,8 @@ _SIZE_FUNCTIONS = {
     "gk_puct_workspace_bytes": [c_int64, c_int],
     "gk_net_weight_bytes": [c_int, c_int],
     "gk_net_headfeat_bytes": [c_int64],
+    "gk_linear_workspace_bytes": [ctypes.POINTER(LinearStruct)],
+    "gk_linear_grad_workspace_bytes": [ctypes.POINTER(LinearGradStruct)],
 }
 
 _lock = threading.Lock()

@@ -16,10 +16,12 @@ from numbers import Real
 from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as native
+from .packing import keep_saved_tensors
 
-_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # GK_FP32, GK_BF16, GK_FP16
+_TYPES = native.TYPES
 _MOST_COLUMNS = 1 << 30
 
 
@@ -130,6 +132,7 @@ class _PolicyLossFunction(torch.autograd.Function):
         return loss, log_probs
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, upstream, _):
         logits = ctx.saved_tensors[0]  # raises if an input was modified in place
         grad, ctx.grad = ctx.grad, None
@@ -214,6 +217,7 @@ def policy_loss(logits, *, legal_mask=None, actions=None, old_log_probs=None, ad
     call = _Call(logits.detach(), legal_mask, actions, old_log_probs, advantages, reference_log_probs, target, clip,
                  kl_weight, target_weight, denominator)
     if torch.is_grad_enabled() and logits.requires_grad:
-        return PolicyLoss(*_PolicyLossFunction.apply(logits, call))
+        with keep_saved_tensors():
+            return PolicyLoss(*_PolicyLossFunction.apply(logits, call))
     with native.on_device(device):
         return PolicyLoss(*call.forward(False, logits)[:2])

@@ -587,6 +587,78 @@ GK_API int gk_policy_loss_forward(const gk_policy_loss_t* p, void* stream);
  * counterpart of its own: autograd of training.py:213-230. */
 GK_API int gk_policy_loss_backward(const gk_policy_loss_t* p, const float* upstream, int written, void* stream);
 
+/* Activations of gk_linear_*. */
+#define GK_ACT_NONE 0
+#define GK_ACT_RELU 1
+#define GK_ACT_TANH 2
+#define GK_ACT_GELU 3 /* z (1 + erf(z / sqrt 2)) / 2 */
+#define GK_ACT_SILU 4 /* z / (1 + e^-z) */
+
+/* y = act(x W^T + bias + residual): x [m, k], W [n, k], y [m, n], all of one
+ * type, rows contiguous. k and n at least 1, every size below 2^31. */
+typedef struct {
+    const void* x;
+    const void* w;
+    const void* bias;        /* [n] or NULL */
+    const void* residual;    /* [m, n] or NULL */
+    void* y;                 /* [m, n], contiguous */
+    void* pre;               /* [m, n], contiguous: the sum before the activation; or NULL */
+    int64_t m, n, k;
+    int64_t x_stride, w_stride, residual_stride; /* elements between rows */
+    int dtype;               /* GK_FP32, GK_BF16, GK_FP16 */
+    int activation;
+} gk_linear_t;
+
+/* Its gradients from dy. dz = dy act'(.) is formed from `kept`: y for relu and
+ * tanh, `pre` for gelu and silu, unused without an activation. dx, dw, db may
+ * be NULL. x is given as it is or packed by gk_pack (x_codes, x_scales: [m, k]
+ * with ceil(k / 32) scales a row). */
+typedef struct {
+    const void* dy;          /* [m, n] */
+    const void* kept;        /* [m, n], contiguous; or NULL */
+    const void* x;           /* [m, k]; or NULL */
+    const uint8_t* x_codes;
+    const uint8_t* x_scales;
+    const void* w;           /* [n, k] */
+    void* dx;                /* [m, k], contiguous */
+    void* dw;                /* [n, k], contiguous */
+    void* db;                /* [n] */
+    void* dz;                /* [m, n], contiguous: the residual's gradient; or NULL (always NULL without activation) */
+    int64_t m, n, k;
+    int64_t dy_stride, x_stride, w_stride;
+    int dtype;
+    int activation;
+} gk_linear_grad_t;
+
+/* Bytes of gk_linear_forward's workspace (0: none needed). */
+GK_API size_t gk_linear_workspace_bytes(const gk_linear_t* p);
+
+/* The linear operator of the network's fully connected heads
+ * (python/kingdom_ai/model.py:59-76, reference nn.Linear with its activation)
+ * in one product with a fused epilogue. `workspace` starts on 256 bytes. */
+GK_API int gk_linear_forward(const gk_linear_t* p, void* workspace, uint32_t* status, void* stream);
+
+/* Bytes of gk_linear_backward's workspace (0: none needed). */
+GK_API size_t gk_linear_grad_workspace_bytes(const gk_linear_grad_t* p);
+
+/* The gradients of gk_linear_forward. No reference counterpart of its own:
+ * autograd of nn.Linear under train_step (python/kingdom_ai/training.py:213-230). */
+GK_API int gk_linear_backward(const gk_linear_grad_t* p, void* workspace, uint32_t* status, void* stream);
+
+/* Activations kept in 8 bits: rows [rows, cols] of GK_FP32, GK_BF16 or GK_FP16
+ * become e4m3 codes [rows, cols] and one scale byte for every 32 columns of a
+ * row ([rows, ceil(cols / 32)], value 2^(byte - 127)). The scale is the
+ * smallest power of two that brings the block's largest magnitude to at most
+ * 448 (at least 2^-124; 2^-15 for fp16, so that every held value is a value of
+ * the type); infinities and NaN become NaN. No reference counterpart. */
+GK_API int gk_pack(const void* x, int64_t stride, int dtype, int64_t rows, int64_t cols, uint8_t* codes,
+                   uint8_t* scales, void* stream);
+
+/* The values that gk_pack's codes hold (saturated to the type's largest), rows
+ * `stride` elements apart. No reference counterpart. */
+GK_API int gk_unpack(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* x,
+                     int64_t stride, int dtype, void* stream);
+
 /* CUDA-event timer for kernel launches inside gk_selfplay_ply: a host object
  * holding `pairs` start/stop event pairs (NULL on failure). No reference
  * counterpart: the reference times phases with perf_counter (loop.py:563-621). */
