@@ -243,6 +243,272 @@ __global__ void __launch_bounds__(kSplitThreads) gemm_split_kernel(const __grid_
     if (ranks > 1) cluster.sync();  // no CTA leaves while another reads its part
 }
 
+// ------------------------------------------------------------------- pair
+
+// Tiles of 256 x BN on pairs of CTAs (cta_group::2): each CTA holds 128 rows of
+// A and half of B's rows, and the tensor cores of both read both halves, so an
+// SM stages half of what a tile of its own would need. Persistent: a pair walks
+// the tiles, and two accumulators in TMEM let the epilogue of one tile run
+// under the products of the next.
+// Warp 0 loads, warp 1 of the even CTA issues the MMAs, warp 2 owns TMEM, warps
+// 4-11 are the epilogue: two warps a quadrant of 32 rows, each with half the columns.
+constexpr int kPairThreads = 384;
+template <int BN>
+struct Pair {
+    static constexpr int kA = 128 * kBK * 2, kB = BN / 2 * kBK * 2, kStage = kA + kB;
+    static constexpr int kStages = BN == 256 ? 6 : 8;
+    static constexpr int kPatch = 32 * 33 * 4;  // a warp's 32 x 32 fp32 patch for rows that are not aligned
+    static constexpr int kSmem = kStages * kStage + 8 * kPatch + 1024;
+    static constexpr uint32_t kTmem = 2 * BN;
+};
+
+__device__ __forceinline__ uint32_t cluster_address(uint32_t local, uint32_t rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void arrive_at(uint32_t remote) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+}
+// A load whose bytes are counted by a barrier of the pair's even CTA.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+        "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+template <int ROWS>
+__device__ __forceinline__ void load_stage_pair(uint32_t dst, const CUtensorMap* map, int across, int mn, int k,
+                                                uint32_t bar) {
+    if (across) {
+#pragma unroll
+        for (int p = 0; p < ROWS / 64; ++p) tma_load_pair(dst + p * 8192, map, mn + 64 * p, k, bar);
+    } else {
+        tma_load_pair(dst, map, k, mn, bar);
+    }
+}
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Arrives on the barrier at this offset in both CTAs once the MMAs issued so far complete.
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+}
+
+// Tile `id` of a walk down groups of eight tile rows, so that the tiles in
+// flight at one time share their operands in L2.
+__device__ __forceinline__ void tile_at(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
+    constexpr int kGroup = 8;
+    const int per_group = kGroup * tiles_n, group = id / per_group, first = group * kGroup;
+    const int rows = min(kGroup, tiles_m - first), rest = id - group * per_group;
+    tm = first + rest % rows;
+    tn = rest / rows;
+}
+
+template <int ACT>
+__device__ __forceinline__ void activate(float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = act_value(v[i], ACT);
+}
+__device__ __forceinline__ void activate(float (&v)[32], int act) {
+    switch (act) {
+        case GK_ACT_RELU: activate<GK_ACT_RELU>(v); break;
+        case GK_ACT_TANH: activate<GK_ACT_TANH>(v); break;
+        case GK_ACT_GELU: activate<GK_ACT_GELU>(v); break;
+        case GK_ACT_SILU: activate<GK_ACT_SILU>(v); break;
+        default: break;
+    }
+}
+__device__ __forceinline__ void store_row32(void* p, int64_t at, const float (&v)[32], bool bf16) {
+    uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        to[i] = make_uint4(pack16(v[8 * i], v[8 * i + 1], bf16), pack16(v[8 * i + 2], v[8 * i + 3], bf16),
+                           pack16(v[8 * i + 4], v[8 * i + 5], bf16), pack16(v[8 * i + 6], v[8 * i + 7], bf16));
+}
+
+// 32 rows (a lane each) by 32 columns of sums: bias, residual, activation, stores.
+__device__ __forceinline__ void finish_patch(const Epilogue& ep, float (&v)[32], int row0, int lane, int n,
+                                             float* patch) {
+    const bool bf16 = ep.bf16 != 0;
+    const int row = row0 + lane;
+    if (ep.aligned && n + 32 <= ep.n) {
+        const bool in = row < ep.m;
+        if (ep.bias != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] += load16(ep.bias, n + i, bf16);
+        }
+        if (ep.residual != nullptr && in) {
+            const uint4* r = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(ep.residual) +
+                                                            row * ep.residual_ld + n);
+            uint4 x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = __ldg(r + i);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float lo, hi;
+                unpack16(reinterpret_cast<const uint32_t*>(x)[i], bf16, lo, hi);
+                v[2 * i] += lo, v[2 * i + 1] += hi;
+            }
+        }
+        if (ep.pre != nullptr && in) store_row32(ep.pre, row * ep.pre_ld + n, v, bf16);
+        activate(v, ep.activation);
+        if (in) store_row32(ep.out, row * ep.out_ld + n, v, bf16);
+        return;
+    }
+    // Rows that do not start on 16 bytes, or the last columns: a lane a column.
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) patch[lane * 33 + i] = v[i];
+    __syncwarp();
+    const int col = n + lane;
+    if (col >= ep.n) return;
+    const float bias = ep.bias != nullptr ? load16(ep.bias, col, bf16) : 0.0f;
+    const int rows = min(32, ep.m - row0);
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
+        const int64_t m = row0 + r;
+        float z = patch[r * 33 + lane] + bias;
+        if (ep.residual != nullptr) z += load16(ep.residual, m * ep.residual_ld + col, bf16);
+        if (ep.pre != nullptr) store16(ep.pre, m * ep.pre_ld + col, z, bf16);
+        store16(ep.out, m * ep.out_ld + col, act_value(z, ep.activation), bf16);
+    }
+}
+
+template <int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, Epilogue ep,
+                     int tiles_m, int tiles_n, int k_blocks, int a_across, int b_across, uint32_t* status) {
+    using P = Pair<BN>;
+    extern __shared__ uint8_t raw[];
+    __shared__ alignas(8) uint64_t full[P::kStages], empty[P::kStages], acc_full[2], acc_empty[2], drain;
+    __shared__ uint32_t tmem_slot;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = (int)cluster.block_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tiles = tiles_m * tiles_n;
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t stages = smem_u32(base);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < P::kStages; ++s) mbar_init(smem_u32(&full[s]), 1), mbar_init(smem_u32(&empty[s]), 1);
+        for (int a = 0; a < 2; ++a) mbar_init(smem_u32(&acc_full[a]), 1), mbar_init(smem_u32(&acc_empty[a]), 16);
+        mbar_init(smem_u32(&drain), 1);
+        fence_mbar_init();
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                     "r"(P::kTmem)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    cluster.sync();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int t = pair; t < tiles && ok; t += pairs) {
+                int tm, tn;
+                tile_at(t, tiles_m, tiles_n, tm, tn);
+                const int m0 = tm * 256 + rank * 128, n0 = tn * BN + rank * (BN / 2);
+                for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+                    const int s = it % P::kStages, turn = it / P::kStages;
+                    if (turn > 0 && !mbar_wait(smem_u32(&empty[s]), (turn - 1) & 1, status)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t at = stages + s * P::kStage, bar = cluster_address(smem_u32(&full[s]), 0);
+                    if (rank == 0) mbar_expect_tx(smem_u32(&full[s]), 2 * P::kStage);
+                    load_stage_pair<128>(at, &ta, a_across, m0, kb * kBK, bar);
+                    load_stage_pair<BN / 2>(at + P::kA, &tb, b_across, n0, kb * kBK, bar);
+                }
+            }
+            // After a wait that gave up: the pair's copies in flight land before the blocks may end.
+            if (!ok && rank == 0)
+                for (int i = max(0, it - P::kStages); i < it; ++i)
+                    mbar_wait(smem_u32(&full[i % P::kStages]), (i / P::kStages) & 1, status);
+        }
+    } else if (warp == 1 && rank == 0) {
+        if (lane == 0) {
+            const uint32_t idesc = idesc16(256, BN, ep.bf16, a_across, b_across);
+            const uint32_t step_a = k_step(a_across), step_b = k_step(b_across);
+            int it = 0, n = 0;
+            bool ok = true;
+            for (int t = pair; t < tiles && ok; t += pairs, ++n) {
+                const int a = n & 1, use = n >> 1;
+                if (use > 0 && !mbar_wait(smem_u32(&acc_empty[a]), (use - 1) & 1, status)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t acc = tmem + a * BN;
+                for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+                    const int s = it % P::kStages;
+                    if (!mbar_wait(smem_u32(&full[s]), (it / P::kStages) & 1, status)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t da = swizzled_desc(stages + s * P::kStage, a_across);
+                    const uint64_t db = swizzled_desc(stages + s * P::kStage + P::kA, b_across);
+#pragma unroll
+                    for (int j = 0; j < kBK / 16; ++j)
+                        mma_pair(acc, da + j * step_a, db + j * step_b, idesc, (kb > 0 || j > 0) ? 1u : 0u);
+                    mma_commit_pair(smem_u32(&empty[s]));
+                }
+                if (ok) mma_commit_pair(smem_u32(&acc_full[a]));
+            }
+            if (!ok) {  // the MMAs in flight end before TMEM is freed
+                mma_commit_pair(smem_u32(&drain));
+                mbar_wait(smem_u32(&drain), 0, status);
+            }
+        }
+    } else if (warp >= 4) {
+        const int quadrant = warp & 3, half = (warp - 4) >> 2;
+        float* patch = reinterpret_cast<float*>(base + P::kStages * P::kStage) + (warp - 4) * (P::kPatch / 4);
+        int n = 0;
+        for (int t = pair; t < tiles; t += pairs, ++n) {
+            const int a = n & 1, use = n >> 1;
+            int tm, tn;
+            tile_at(t, tiles_m, tiles_n, tm, tn);
+            // Every lane waits: the verdict is the warp's.
+            if (__any_sync(0xffffffffu, !mbar_wait(smem_u32(&acc_full[a]), use & 1, status))) break;
+            tc_fence_after();
+            const int row0 = tm * 256 + rank * 128 + quadrant * 32, n0 = tn * BN + half * (BN / 2);
+            const uint32_t from = tmem + ((uint32_t)(quadrant * 32) << 16) + a * BN + half * (BN / 2);
+#pragma unroll 1
+            for (int c = 0; c < BN / 2; c += 32) {
+                float v[32];
+                tmem_ld32(from + c, v);
+                if (c + 32 == BN / 2) {  // the last columns are in registers: the accumulator is free
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_at(cluster_address(smem_u32(&acc_empty[a]), 0));
+                }
+                if (row0 < ep.m && n0 + c < ep.n) finish_patch(ep, v, row0, lane, n0 + c, patch);
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    cluster.sync();  // both CTAs are done with the other's barriers, shared memory and TMEM
+    tc_fence_after();
+    if (warp == 2)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P::kTmem) : "memory");
+}
+
 // ------------------------------------------------------------------ host
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -318,12 +584,36 @@ int launch_split(const GemmArgs& g, uint32_t* status, cudaStream_t stream) {
                                    (int)blocks, g.a_across, g.b_across, status);
 }
 
+template <int BN>
+int launch_pair(const GemmArgs& g, uint32_t* status, cudaStream_t stream) {
+    using P = Pair<BN>;
+    auto* kernel = gemm_pair_kernel<BN>;
+    static bool ready[64] = {};
+    if (!once_per_device(ready, [&] {
+            return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kSmem) == cudaSuccess;
+        }))
+        return launch_status();
+    CUtensorMap ta, tb;
+    if (!encode(&ta, g.a, g.a_ld, g.a_across, g.m, g.k, 128, g.dtype) ||
+        !encode(&tb, g.b, g.b_ld, g.b_across, g.n, g.k, BN / 2, g.dtype))
+        return GK_EINVAL;
+    const int64_t tiles_m = (g.m + 255) / 256, tiles_n = (g.n + BN - 1) / BN;
+    if (tiles_m * tiles_n >= (1ll << 31) - kSmCount) return GK_EINVAL;
+    const int64_t pairs = tiles_m * tiles_n < kSmCount / 2 ? tiles_m * tiles_n : kSmCount / 2;
+    kernel<<<(unsigned)(2 * pairs), kPairThreads, P::kSmem, stream>>>(
+        ta, tb, epilogue_of(g), (int)tiles_m, (int)tiles_n, (int)((g.k + kBK - 1) / kBK), g.a_across, g.b_across,
+        status);
+    return launch_status();
+}
+
 }  // namespace
 
 int gemm16(const GemmArgs& g, uint32_t* status, cudaStream_t stream) {
     if (g.m < 1 || g.n < 1 || g.k < 1 || g.m >= (1ll << 31) || g.n >= (1ll << 31) || g.k >= (1ll << 31))
         return GK_EINVAL;
     if (!aligned16(g.a) || !aligned16(g.b) || g.a_ld % 8 != 0 || g.b_ld % 8 != 0) return GK_EINVAL;
+    const int64_t large = ((g.m + 255) / 256) * ((g.n + 255) / 256);
+    if (large >= kSmCount / 2) return launch_pair<256>(g, status, stream);
     return launch_split<64>(g, status, stream);
 }
 
