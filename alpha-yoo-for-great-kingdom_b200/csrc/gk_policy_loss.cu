@@ -65,25 +65,27 @@ __device__ __forceinline__ float ex2(float x) {
 
 // exp(x - m) for many x of one row. For 16-bit logits it is 2^(x s - m s),
 // one multiply-add and one 2^x; `correct` undoes the rounding of m s, which
-// all terms share. The difference of two values whose product with log2 e
-// would overflow is either 0 or below -1e35, so any small scale serves there.
+// all terms share. From 1e5 on 16-bit values are 32 (fp16) or 512 and more
+// (bf16) apart: exp is then 1 or nothing, which 2^(x - m) gives without overflow.
 template <typename T>
 struct Exp {
     float scale, offset, correct;
     __device__ __forceinline__ explicit Exp(float m) {
-        scale = fabsf(m) < 1e38f ? 1.4426950408889634f : 1e-30f;
+        scale = fabsf(m) < 1e5f ? 1.4426950408889634f : 1.0f;
         offset = m * scale;
         const float rest = fmaf(m, scale, -offset);
-        correct = fabsf(rest) < 1.0f ? ex2(-rest) : 1.0f;
+        correct = fabsf(rest) < 1.0f ? ex2(-rest) : 1.0f;  // not a number for an infinite m
     }
     __device__ __forceinline__ float operator()(float x) const { return ex2(fmaf(x, scale, -offset)); }
 };
+// fp32 logits: the difference first, which keeps the exponent's error at the
+// last bit of x - m.
 template <>
 struct Exp<float> {
     float m;
     static constexpr float correct = 1.0f;
     __device__ __forceinline__ explicit Exp(float top) : m(top) {}
-    __device__ __forceinline__ float operator()(float x) const { return expf(x - m); }
+    __device__ __forceinline__ float operator()(float x) const { return ex2((x - m) * 1.4426950408889634f); }
 };
 
 // Elements of one 16-byte vector of logits.
@@ -183,14 +185,27 @@ __device__ __forceinline__ void load_target(const TT* trow, uint32_t legal, int 
     }
 }
 
+template <typename T>
+__device__ __forceinline__ uint32_t pair_of(float lo, float hi) {
+    uint32_t v;
+    if constexpr (std::is_same<T, __half>::value)
+        *reinterpret_cast<__half2*>(&v) = __floats2half2_rn(lo, hi);
+    else
+        *reinterpret_cast<__nv_bfloat162*>(&v) = __floats2bfloat162_rn(lo, hi);
+    return v;
+}
 template <typename TL, int V>
 __device__ __forceinline__ void store_group(TL* grow, int first, int cols, bool edge, const float (&g)[V]) {
     if (V > 1 && !edge) {
         if constexpr (V > 1) {
-            alignas(16) TL raw[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) raw[i] = from_f<TL>(g[i]);
-            __stcs(reinterpret_cast<uint4*>(grow + first), *reinterpret_cast<uint4*>(raw));
+            uint4 w;
+            if constexpr (V == 4)
+                w = make_uint4(__float_as_uint(g[0]), __float_as_uint(g[1]), __float_as_uint(g[2]),
+                               __float_as_uint(g[3]));
+            else
+                w = make_uint4(pair_of<TL>(g[0], g[1]), pair_of<TL>(g[2], g[3]), pair_of<TL>(g[4], g[5]),
+                               pair_of<TL>(g[6], g[7]));
+            __stcs(reinterpret_cast<uint4*>(grow + first), w);
         }
     } else {
 #pragma unroll
@@ -270,7 +285,12 @@ __device__ __forceinline__ Row row_terms(const gk_policy_loss_t& p, const RowInp
             } else {
                 o.action = in.action;
                 using W = typename std::conditional<WIDE, double, float>::type;
-                const W log_s = WIDE ? (W)log((double)s) : (W)o.log_s;
+                W log_s = o.log_s;
+                if (WIDE && s < INFINITY) {
+                    // s = f 2^k with f in [0.75, 1.5): log f is small, so its last bit is too.
+                    const int k = (int)((__float_as_uint(s) + 0x400000u) >> 23) - 127;
+                    log_s = (W)k * (W)0.69314718055994531 + (W)logf(__uint_as_float(__float_as_uint(s) - (k << 23)));
+                }
                 const W log_p = ((W)in.x - (W)m) - log_s;
                 o.log_p = (float)log_p;
                 const float adv = in.advantage;
@@ -308,8 +328,9 @@ __device__ __forceinline__ void gradient_group(const Group<TL, V>& h, const floa
     }
 }
 
-__device__ __forceinline__ float target_term(float t, float x, float m, float log_s) {
-    return t > 0.0f ? t * (logf(t) - ((x - m) - log_s)) : (t == 0.0f ? 0.0f : nanf(""));
+// t (log t - d), with d the entry's log-probability or its distance to a maximum.
+__device__ __forceinline__ float target_term(float t, float d) {
+    return t > 0.0f ? t * (__logf(t) - d) : (t == 0.0f ? 0.0f : nanf(""));
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -389,7 +410,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) policy_loss_rows_kernel(gk_pol
         if constexpr (!std::is_same<TT, None>::value) {
             float kl = 0.0f;
 #pragma unroll
-            for (int k = 0; k < NPL; ++k) kl += target_term(t[k], x[k], m, o.log_s);
+            for (int k = 0; k < NPL; ++k) kl += target_term(t[k], (x[k] - m) - o.log_s);
             kl = warp_sum(kl);
             if (lane == 0 && o.inv_s != 0.0f) loss += p.target_weight * kl;
         }
@@ -449,189 +470,181 @@ struct Part {
     }
 };
 
-// Each thread copies the groups that it will read itself, so no barrier stands
-// between the copy and its use.
-template <typename TL, typename TT, int V>
-__device__ __forceinline__ void stage_row(const Part<TL, TT, V>& part, uint4* buffer) {
-    for (int q = part.full + threadIdx.x; q < part.full_end; q += blockDim.x) {
-        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(buffer + (q - part.full));
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(part.lrow + ((int64_t)q * V - part.shift))
-                     : "memory");
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+__device__ __forceinline__ void copy_async(uint4* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
+                 : "memory");
 }
 
 // Longer rows: a cluster of CTAs takes a row, each CTA a part of it; the parts
 // meet through distributed shared memory. STAGED: a CTA's part of the logits
-// lies in shared memory, with two buffers the next row's part on its way while
-// this one is worked on, so the logits are read from HBM once and the copies
-// never stop. Otherwise (a part past the shared memory, or rows that are not
-// aligned) each pass reads the row itself, from L2 where it fits.
+// lies in shared memory, so they are read from HBM once. Each thread copies the
+// groups that it reads itself, so no barrier stands between a copy and its use,
+// and a slot takes the next row's group as soon as this row's last pass has
+// read it: the loads of one row run under the stores of the row before.
+// Otherwise (a part past the shared memory, or rows that are not aligned) each
+// pass reads the row itself, from L2 where it fits.
 template <typename TL, typename TT, int V, bool STAGED>
-__global__ void __launch_bounds__(kLongThreads, 3) policy_loss_long_kernel(gk_policy_loss_t p, int buffers,
-                                                                           int part_groups) {
+__global__ void __launch_bounds__(kLongThreads, 3) policy_loss_long_kernel(gk_policy_loss_t p) {
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
     constexpr bool kTarget = !std::is_same<TT, None>::value;
     constexpr int kWarps = kLongThreads / 32;
     extern __shared__ uint4 staged[];
-    __shared__ float wm[kWarps], ws[kWarps], wt[kWarps], wk[kWarps];
-    __shared__ float part_sums[3];  // this CTA's maximum, sum, target sum: read by the cluster
-    __shared__ float part_kl[2];    // this CTA's target term, by turns: read by rank 0
-    __shared__ Row shared_row;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    // What each warp of the cluster found (maximum, sum, target sum, target
+    // term), by turns: written by every CTA, read after the cluster barrier.
+    // A slot is written again two rows later, a barrier after its last read.
+    __shared__ float4 found[2][kMaxCluster * kWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
     const int64_t clusters = gridDim.x / ranks, first_row = blockIdx.x / ranks;
     const float inv_n = inverse_denominator(p);
     const int cols = (int)p.cols;
     double sum = 0.0;
     int turn = 0;
-    auto meet = [&] {
-        if (ranks > 1)
-            cluster.sync();
-        else
-            __syncthreads();
-    };
-    if constexpr (STAGED) stage_row(Part<TL, TT, V>(p, first_row, rank, ranks), staged);
+    if constexpr (STAGED) {
+        const Part<TL, TT, V> part(p, first_row, rank, ranks);
+        const TL* from = part.lrow + ((int64_t)part.full * V - part.shift);
+        for (int k = tid; k < part.full_end - part.full; k += threads) copy_async(staged + k, from + k * V);
+    }
     for (int64_t r = first_row; r < p.rows; r += clusters, turn ^= 1) {
         const Part<TL, TT, V> part(p, r, rank, ranks);
-        RowInput in;
-        if (tid == 0) in = row_input(p, r, part.lrow, part.mrow);
-        const TL* from = part.lrow + ((int64_t)part.full * V - part.shift);
-        if constexpr (STAGED) {
-            if (buffers == 2 && r + clusters < p.rows) {
-                // The other buffer's row was finished before the last barrier.
-                stage_row(Part<TL, TT, V>(p, r + clusters, rank, ranks), staged + (turn ^ 1) * part_groups);
-                asm volatile("cp.async.wait_group 1;" ::: "memory");
-            } else {
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-            }
-            from = reinterpret_cast<const TL*>(staged + (buffers == 2 ? turn * part_groups : 0));
-        }
+        const RowInput in = row_input(p, r, part.lrow, part.mrow);
+        const int base = part.full * V - part.shift, count = part.full_end - part.full;
         // f(group, index of its first entry, whether it is an edge); thread 0
-        // also takes the row's first edge and thread 32 its last.
-        auto each_group = [&](auto&& f) {
-            const int count = part.full_end - part.full, base = part.full * V - part.shift;
-#pragma unroll 4
-            for (int k = tid; k < count; k += blockDim.x) {
-                Group<TL, V> h;
-                h.load(from + k * V, part.mrow == nullptr ? nullptr : part.mrow + base + k * V);
-                f(h, base + k * V, false);
-            }
+        // also takes the row's first edge and the last thread its last.
+        auto each_edge = [&](auto&& f) {
             if (V > 1) {
                 if (tid == 0 && part.begin < part.full && part.begin < part.end) {
                     Group<TL, V> h;
                     h.load_edge(part.lrow, part.mrow, part.begin * V - part.shift, cols);
                     f(h, part.begin * V - part.shift, true);
                 }
-                if (tid == 32 && part.full_end < part.end && part.end - 1 >= part.full) {
+                if (tid == threads - 1 && part.full_end < part.end && part.end - 1 >= part.full) {
                     Group<TL, V> h;
                     h.load_edge(part.lrow, part.mrow, (part.end - 1) * V - part.shift, cols);
                     f(h, (part.end - 1) * V - part.shift, true);
                 }
             }
         };
+        auto load = [&](Group<TL, V>& h, int k) {
+            const TL* from = STAGED ? reinterpret_cast<const TL*>(staged + k) : part.lrow + base + k * V;
+            h.load(from, part.mrow == nullptr ? nullptr : part.mrow + base + k * V);
+        };
+        auto each_group = [&](auto&& f) {
+#pragma unroll 4
+            for (int k = tid; k < count; k += threads) {
+                Group<TL, V> h;
+                load(h, k);
+                f(h, base + k * V, false);
+            }
+            each_edge(f);
+        };
+        if constexpr (STAGED) asm volatile("cp.async.wait_all;" ::: "memory");
         Softmax acc;
-        float total_t = 0.0f;
+        float total_t = 0.0f, kl = 0.0f;
         each_group([&](const Group<TL, V>& h, int, bool) { acc.m = fmaxf(acc.m, h.top()); });
 #pragma unroll
         for (int o = 16; o; o >>= 1) acc.m = fmaxf(acc.m, __shfl_xor_sync(kFull, acc.m, o));
         {
             const Exp<TL> e(acc.m);
+            float s2 = 0.0f;
             each_group([&](const Group<TL, V>& h, int first, bool edge) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) acc.s += e(h.x(i));
+                for (int i = 0; i < V; ++i) (i & 1 ? s2 : acc.s) += e(h.x(i));
                 if constexpr (kTarget) {
                     float t[V];
                     load_target<TT, V>(part.trow, h.legal, first, edge, t);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) total_t += t[i];
-                }
-            });
-            acc.s = warp_sum(acc.s) * e.correct;
-        }
-        if (kTarget) total_t = warp_sum(total_t);
-        if (lane == 0) wm[warp] = acc.m, ws[warp] = acc.s, wt[warp] = total_t;
-        __syncthreads();
-        if (warp == 0) {
-            acc.m = lane < warps ? wm[lane] : -FLT_MAX;
-            acc.s = lane < warps ? ws[lane] : 0.0f;
-            acc.join_lanes(kWarps);
-            if (kTarget) total_t = warp_sum(lane < warps ? wt[lane] : 0.0f);
-            if (ranks > 1) {
-                if (lane == 0) part_sums[0] = acc.m, part_sums[1] = acc.s, part_sums[2] = total_t;
-            } else if (lane == 0) {
-                shared_row = row_terms<true>(p, in, acc.m, acc.s, total_t);
-                write_row(p, r, shared_row);
-            }
-        }
-        if (ranks > 1) {
-            cluster.sync();
-            if (warp == 0) {
-                const float* other = cluster.map_shared_rank(part_sums, lane < ranks ? lane : 0);
-                acc.m = lane < ranks ? other[0] : -FLT_MAX;
-                acc.s = lane < ranks ? other[1] : 0.0f;
-                if (kTarget) total_t = warp_sum(lane < ranks ? other[2] : 0.0f);
-                acc.join_lanes(kMaxCluster);
-                if (lane == 0) {
-                    shared_row = row_terms<true>(p, in, acc.m, acc.s, total_t);
-                    if (rank == 0) write_row(p, r, shared_row);
-                }
-            }
-        }
-        __syncthreads();
-        const Row o = shared_row;
-        if (kTarget || p.grad != nullptr) {
-            TL* grow = static_cast<TL*>(p.grad) + r * p.cols;
-            const Exp<TL> e(o.m);
-            const float kp = inv_n * (p.target_weight * o.total_t - o.c) * o.inv_s * e.correct;
-            const float kt = inv_n * p.target_weight;
-            const bool live = o.inv_s != 0.0f;
-            float kl = 0.0f;
-            each_group([&](const Group<TL, V>& h, int first, bool edge) {
-                float t[V], g[V];
-                load_target<TT, V>(part.trow, h.legal, first, edge, t);
-                if (kTarget) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) kl += target_term(t[i], h.x(i), o.m, o.log_s);
-                }
-                if (p.grad != nullptr) {
-                    if (live) {
-                        gradient_group<TL, TT, V>(h, t, e, kp, kt, g);
-                        const int64_t at = o.action - first;
-                        if (at >= 0 && at < V) {  // one group of the row
-#pragma unroll
-                            for (int i = 0; i < V; ++i)
-                                if (at == i) g[i] += inv_n * o.c;
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < V; ++i) g[i] = 0.0f;
+                    for (int i = 0; i < V; ++i) {
+                        total_t += t[i];
+                        kl += target_term(t[i], h.x(i) - acc.m);
                     }
-                    store_group<TL, V>(grow, first, cols, edge, g);
                 }
             });
-            if (kTarget) {
-                kl = warp_sum(kl);
-                if (lane == 0) wk[warp] = kl;
-                __syncthreads();
-                if (warp == 0) {
-                    kl = warp_sum(lane < warps ? wk[lane] : 0.0f);
-                    if (lane == 0) part_kl[turn] = kl;
+            acc.s = warp_sum(acc.s + s2) * e.correct;
+        }
+        if (kTarget) {
+            total_t = warp_sum(total_t);
+            kl = warp_sum(kl);
+        }
+        const float4 mine = make_float4(acc.m, acc.s, total_t, kl);
+        if (ranks > 1) {
+            if (lane < ranks) cluster.map_shared_rank(found[turn], lane)[rank * warps + warp] = mine;
+            cluster.sync();
+        } else {
+            if (lane == 0) found[turn][warp] = mine;
+            __syncthreads();
+        }
+        // Every warp joins what all found and forms the row's terms for itself.
+        const int all = ranks * warps;
+        const float4 none = make_float4(-FLT_MAX, 0.0f, 0.0f, 0.0f);
+        const float4 f0 = lane < all ? found[turn][lane] : none, f1 = lane + 32 < all ? found[turn][lane + 32] : none;
+        acc.m = f0.x, acc.s = f0.y;
+        acc.join(f1.x, f1.y);
+        acc.join_lanes(32);
+        if (kTarget) {
+            total_t = warp_sum(f0.z + f1.z);
+            // A warp without mass has no distance to add (and no finite one, if all it saw was -inf).
+            kl = warp_sum((f0.z == 0.0f ? f0.w : f0.w + f0.z * (acc.m - f0.x)) +
+                          (f1.z == 0.0f ? f1.w : f1.w + f1.z * (acc.m - f1.x)));
+        }
+        const Row o = row_terms<true>(p, in, acc.m, acc.s, total_t);
+        if (rank == 0 && tid == 0) {
+            write_row(p, r, o);
+            sum += (double)(o.loss + (kTarget && o.inv_s != 0.0f ? p.target_weight * (kl + total_t * o.log_s) : 0.0f));
+        }
+        TL* grow = static_cast<TL*>(p.grad) + r * p.cols;
+        const Exp<TL> e(o.m);
+        const float kt = inv_n * p.target_weight;
+        const float kp = inv_n * (p.target_weight * o.total_t - o.c) * o.inv_s * e.correct;
+        auto finish = [&](const Group<TL, V>& h, int first, bool edge) {
+            float t[V], g[V];
+            load_target<TT, V>(part.trow, h.legal, first, edge, t);
+            gradient_group<TL, TT, V>(h, t, e, kp, kt, g);
+            store_group<TL, V>(grow, first, cols, edge, g);
+        };
+        // The next row of this CTA: its groups take the slots as the last pass empties them.
+        const bool more = STAGED && r + clusters < p.rows;
+        const Part<TL, TT, V> next(p, more ? r + clusters : r, rank, ranks);
+        const TL* next_from = next.lrow + ((int64_t)next.full * V - next.shift);
+        const int next_count = more ? next.full_end - next.full : 0;
+        if (o.inv_s != 0.0f && p.grad != nullptr) {
+            constexpr int U = 4;
+            for (int k0 = tid; k0 < count; k0 += U * threads) {
+                Group<TL, V> h[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (k0 + u * threads < count) load(h[u], k0 + u * threads);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (k0 + u * threads < count) finish(h[u], base + (k0 + u * threads) * V, false);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (k0 + u * threads < min(count, next_count))
+                        copy_async(staged + k0 + u * threads, next_from + (k0 + u * threads) * V);
+            }
+            // An odd row's part may be a group longer than the one before it.
+            if (count < next_count && tid == count % threads) copy_async(staged + count, next_from + count * V);
+            each_edge(finish);
+            if (o.action >= 0) {
+                // The action's own part: the thread that wrote its group writes it again.
+                const int q = ((int)o.action + part.shift) / V;
+                const bool head = q < part.full, tail = q >= part.full_end;
+                if (q >= part.begin && q < part.end &&
+                    tid == (head ? 0 : (tail ? threads - 1 : (q - part.full) % threads))) {
+                    float t = 0.0f;
+                    if constexpr (kTarget) t = to_f(part.trow[o.action]);
+                    grow[o.action] = from_f<TL>(kp * e(to_f(part.lrow[o.action])) - kt * t + inv_n * o.c);
                 }
             }
-        }
-        if constexpr (STAGED) {
-            if (buffers == 1 && r + clusters < p.rows)  // each thread has read its own groups
-                stage_row(Part<TL, TT, V>(p, r + clusters, rank, ranks), staged);
-        }
-        meet();  // also keeps every CTA's part until all have read it
-        if (rank == 0 && warp == 0) {
-            float kl = 0.0f;
-            if (kTarget) kl = warp_sum(lane < ranks ? *cluster.map_shared_rank(part_kl + turn, lane < ranks ? lane : 0) : 0.0f);
-            sum += (double)(o.loss + (kTarget && o.inv_s != 0.0f ? p.target_weight * kl : 0.0f));
+        } else {
+            for (int k = tid; k < next_count; k += threads) copy_async(staged + k, next_from + k * V);
+            if (p.grad != nullptr)
+                for (int j = max(0, part.begin * V - part.shift) + tid; j < min(cols, part.end * V - part.shift);
+                     j += threads)
+                    grow[j] = from_f<TL>(0.0f);
         }
     }
-    if (ranks > 1) cluster.sync();  // no CTA leaves while another reads its shared memory
+    if (ranks > 1) cluster.sync();  // no CTA leaves while another writes to its shared memory
     if (rank == 0 && tid == 0) {
         if (clusters == 1)
             finish_loss(p, sum);
@@ -717,16 +730,17 @@ bool vectorised(const gk_policy_loss_t& p, int v) {
     return p.logits_stride >= 0;
 }
 
-// How a long row is split and staged. A CTA's part is at most 32 KB where two
-// buffers of it are kept (three CTAs an SM), at most 64 KB with one; the
-// cluster grows until the part fits, and with fewer rows than SMs until the
-// grid fills them, but no part gets shorter than two vectors a thread. Parts
-// under 8 KB take half the threads, so that more rows are in flight.
+// How a long row is split and staged. A CTA's part is at most 72 KB, three to
+// an SM; the cluster grows until the part fits, and with fewer rows than the
+// SMs hold until the grid fills them, but no part gets shorter than two vectors
+// a thread. Short parts take fewer threads, four vectors each, so that more
+// rows are in flight.
 struct LongPlan {
-    int cluster, threads, buffers, part_groups;
+    int cluster, threads;
+    bool staged;
     size_t smem;
 };
-constexpr int64_t kPartBytes = 32 << 10;
+constexpr int64_t kPartBytes = 72 << 10;
 
 LongPlan long_plan(const gk_policy_loss_t& p, int v) {
     const int64_t groups = (p.cols + 2 * (v - 1)) / v;  // with the shift of an odd row
@@ -737,44 +751,61 @@ LongPlan long_plan(const gk_policy_loss_t& p, int v) {
         c *= 2;
     LongPlan plan{};
     plan.cluster = c;
-    plan.part_groups = (int)part(c);
-    const int64_t bytes = part(c) * 16;
-    plan.threads = bytes < (8 << 10) ? kLongThreads / 2 : kLongThreads;
-    plan.buffers = v == 1 || bytes > 2 * kPartBytes ? 0 : (bytes > kPartBytes ? 1 : 2);
-    plan.smem = (size_t)plan.buffers * bytes;
+    plan.threads = kLongThreads;
+    while (plan.threads > 32 && part(c) < plan.threads * 2) plan.threads /= 2;
+    plan.staged = v > 1 && part(c) * 16 <= kPartBytes;
+    plan.smem = plan.staged ? (size_t)part(c) * 16 : 0;
     return plan;
 }
 
 int row_blocks(int64_t rows) { return blocks_for(rows, kRowWarps, kSmCount * 8); }
-// Clusters of a long-row launch: as many as the SMs hold at once (by a CTA's
-// shared memory, at most eight of half the threads), so each keeps its next row in flight.
-int long_clusters(int64_t rows, const LongPlan& plan) {
-    const int64_t per_sm = plan.threads == kLongThreads ? 3 : 6;
-    const int64_t most = kSmCount * per_sm / plan.cluster;
-    return (int)(rows < most ? rows : most);
+
+// Most clusters of a long-row launch: CTAs of 3 * 256 threads an SM.
+int64_t most_clusters(const LongPlan& plan) {
+    const int64_t per_sm = 3 * kLongThreads / plan.threads;
+    return kSmCount * per_sm / plan.cluster;
 }
 
 template <typename TL, typename TT, int V, bool STAGED>
-int launch_long(const gk_policy_loss_t& p, const LongPlan& plan, int clusters, cudaStream_t s) {
+int launch_long(const gk_policy_loss_t& p, const LongPlan& plan, int* clusters, cudaStream_t s) {
     auto* kernel = policy_loss_long_kernel<TL, TT, V, STAGED>;
     static bool done[64] = {};
-    if (!once_per_device(done, [&] {
-            return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kPartBytes) ==
-                   cudaSuccess;
-        }))
-        return launch_status();
+    static int resident[64][4] = {};  // clusters of 1, 2, 4, 8 full-size CTAs that the device holds at once
+    int dev = 0;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(clusters * plan.cluster));
-    cfg.blockDim = dim3(plan.threads);
-    cfg.dynamicSmemBytes = STAGED ? plan.smem : 0;
-    cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = plan.cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, p, plan.buffers, plan.part_groups);
+    cfg.stream = s;
+    if (!once_per_device(done, [&] {
+            if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPartBytes) != cudaSuccess ||
+                cudaGetDevice(&dev) != cudaSuccess)
+                return false;
+            for (int i = 0; i < 4; ++i) {
+                attr[0].val.clusterDim.x = 1 << i;
+                cfg.gridDim = dim3(8);
+                cfg.blockDim = dim3(kLongThreads);
+                cfg.dynamicSmemBytes = STAGED ? kPartBytes : 0;
+                if (cudaOccupancyMaxActiveClusters(&resident[dev][i], kernel, &cfg) != cudaSuccess) return false;
+            }
+            return true;
+        }))
+        return launch_status();
+    if (cudaGetDevice(&dev) != cudaSuccess) return launch_status();
+    int64_t most = most_clusters(plan);
+    int log = 0;
+    while ((1 << log) < plan.cluster) ++log;
+    // GPCs of an odd number of SMs leave some out of a cluster: a grid that is
+    // resident at once has no second round for the rest.
+    if (plan.threads == kLongThreads && resident[dev][log] > 0 && resident[dev][log] < most) most = resident[dev][log];
+    *clusters = (int)(p.rows < most ? p.rows : most);
+    attr[0].val.clusterDim.x = plan.cluster;
+    cfg.gridDim = dim3((unsigned)(*clusters * plan.cluster));
+    cfg.blockDim = dim3(plan.threads);
+    cfg.dynamicSmemBytes = plan.smem;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 template <typename TL, typename TT>
@@ -790,10 +821,9 @@ int forward(const gk_policy_loss_t& p, cudaStream_t s) {
         constexpr int V = kVec<TL>;
         const bool vec = vectorised(p, V);
         const LongPlan plan = long_plan(p, vec ? V : 1);
-        parts = long_clusters(p.rows, plan);
-        const int e = !vec ? launch_long<TL, TT, 1, false>(p, plan, parts, s)
-                           : (plan.buffers > 0 ? launch_long<TL, TT, V, true>(p, plan, parts, s)
-                                               : launch_long<TL, TT, V, false>(p, plan, parts, s));
+        const int e = !vec ? launch_long<TL, TT, 1, false>(p, plan, &parts, s)
+                           : (plan.staged ? launch_long<TL, TT, V, true>(p, plan, &parts, s)
+                                          : launch_long<TL, TT, V, false>(p, plan, &parts, s));
         if (e != 0) return e;
     }
     if (parts > 1) policy_loss_sum_kernel<<<1, 256, 0, s>>>(p, parts);
@@ -833,7 +863,7 @@ extern "C" {
 int gk_policy_loss_parts(int64_t rows, int64_t cols) {
     if (rows < 1 || cols < 1) return 0;
     if (cols <= gk::kShortRow) return gk::row_blocks(rows);
-    const int64_t most = gk::kSmCount * 6;  // clusters of any plan
+    const int64_t most = gk::kSmCount * 3 * (gk::kLongThreads / 32);  // clusters of any plan
     return (int)(rows < most ? rows : most);
 }
 

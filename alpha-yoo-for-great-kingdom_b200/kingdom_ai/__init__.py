@@ -18,4 +18,4 @@ from .evaluation import EvaluationResult, evaluate_models_gpu  # noqa: F401
 from .engine_api import BatchedPUCT, PUCTMoveStatistics, PUCTSearchResult, encode_puct_batch  # noqa: F401
 from .losses import PolicyLoss, policy_loss  # noqa: F401
 from .packing import PackedActivation, pack_activation, packed_activations  # noqa: F401
-from .linear import check_linear, linear  # noqa: F401
+from .layers import check_linear, linear  # noqa: F401
