@@ -63,6 +63,8 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ float exp_of(float d) { return ex2(d * 1.4426950408889634f); }
+
 // exp(x - m) for many x of one row. For 16-bit logits it is 2^(x s - m s),
 // one multiply-add and one 2^x; `correct` undoes the rounding of m s, which
 // all terms share. From 1e5 on 16-bit values are 32 (fp16) or 512 and more
@@ -114,13 +116,24 @@ struct Raw<16> {
 // V consecutive entries of a row, masked ones as -inf, with a bit an entry for the legal ones.
 template <typename TL, int V>
 struct Group {
-    alignas(V > 1 ? 16 : alignof(TL)) TL raw[V];
+    static constexpr int kWords = V * (int)sizeof(TL) / 4;
+    uint32_t w[V > 1 ? kWords : 1];  // the entries as they lie in memory; V == 1: one entry, as fp32
     uint32_t legal;
-    __device__ __forceinline__ float x(int i) const { return to_f(raw[i]); }
+    __device__ __forceinline__ float x(int i) const {
+        if constexpr (V == 1 || sizeof(TL) == 4) {
+            return __uint_as_float(w[i]);
+        } else if constexpr (std::is_same<TL, __half>::value) {
+            const __half2 h = *reinterpret_cast<const __half2*>(&w[i / 2]);
+            return i & 1 ? __high2float(h) : __low2float(h);
+        } else {
+            // From the word: one shift or mask an entry.
+            return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        }
+    }
     __device__ __forceinline__ float top() const {
         if constexpr (V == 8) {  // 16-bit logits: in pairs, which keeps them packed
             using P = typename std::conditional<std::is_same<TL, __half>::value, __half2, __nv_bfloat162>::type;
-            const P* v = reinterpret_cast<const P*>(raw);
+            const P* v = reinterpret_cast<const P*>(w);
             const P m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
             return fmaxf(to_f(m.x), to_f(m.y));
         } else {
@@ -130,14 +143,25 @@ struct Group {
             return m;
         }
     }
+    __device__ __forceinline__ void hide(int i) {
+        if constexpr (V == 1 || sizeof(TL) == 4)
+            w[i] = 0xff800000u;
+        else if constexpr (std::is_same<TL, __half>::value)
+            w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | 0xfc000000u : (w[i / 2] & 0xffff0000u) | 0xfc00u;
+        else
+            w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | 0xff800000u : (w[i / 2] & 0xffff0000u) | 0xff80u;
+    }
     // All V entries lie in the row; `from` is 16-byte aligned if V > 1.
+    template <bool MASK>
     __device__ __forceinline__ void load(const TL* from, const uint8_t* mask) {
         legal = (1u << V) - 1u;
-        if constexpr (V > 1)
-            *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(from);
-        else
-            raw[0] = *from;
-        if (mask != nullptr) {
+        if constexpr (V > 1) {
+            const uint4 v = *reinterpret_cast<const uint4*>(from);
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        } else {
+            w[0] = __float_as_uint(to_f(*from));
+        }
+        if constexpr (MASK) {
             alignas(V) uint8_t m[V];
             using R = typename Raw<V>::type;
             *reinterpret_cast<R*>(m) = __ldg(reinterpret_cast<const R*>(mask));
@@ -145,7 +169,7 @@ struct Group {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 legal |= (m[i] != 0 ? 1u : 0u) << i;
-                if (m[i] == 0) raw[i] = from_f<TL>(-INFINITY);
+                if (m[i] == 0) hide(i);
             }
         }
     }
@@ -153,11 +177,18 @@ struct Group {
     __device__ __forceinline__ void load_edge(const TL* lrow, const uint8_t* mrow, int first, int cols) {
         legal = 0u;
 #pragma unroll
+        for (int i = 0; i < (V > 1 ? kWords : 1); ++i) w[i] = 0u;
+#pragma unroll
         for (int i = 0; i < V; ++i) {
             const int j = first + i;
             const bool in = j >= 0 && j < cols && (mrow == nullptr || mrow[j] != 0);
             legal |= (in ? 1u : 0u) << i;
-            raw[i] = in ? lrow[j] : from_f<TL>(-INFINITY);
+            if (!in)
+                hide(i);
+            else if constexpr (V == 1 || sizeof(TL) == 4)
+                w[i] = __float_as_uint(to_f(lrow[j]));
+            else
+                w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(lrow)[j] << (16 * (i & 1));
         }
     }
 };
@@ -223,7 +254,7 @@ struct Softmax {
     __device__ __forceinline__ void join(float m2, float s2) {
         const float top = fmaxf(m, m2);
         // A part with nothing in it must not scale by exp(lowest - top).
-        s = (s == 0.0f ? 0.0f : s * expf(m - top)) + (s2 == 0.0f ? 0.0f : s2 * expf(m2 - top));
+        s = (s == 0.0f ? 0.0f : s * exp_of(m - top)) + (s2 == 0.0f ? 0.0f : s2 * exp_of(m2 - top));
         m = top;
     }
     __device__ __forceinline__ void join_lanes(int lanes) {
@@ -456,13 +487,13 @@ struct Part {
     const uint8_t* mrow;
     const TT* trow;
     int shift, begin, end, full, full_end;
-    __device__ __forceinline__ Part(const gk_policy_loss_t& p, int64_t r, int rank, int ranks) {
+    __device__ __forceinline__ Part(const gk_policy_loss_t& p, int64_t r, int rank, int log_ranks) {
         lrow = static_cast<const TL*>(p.logits) + r * p.logits_stride;
         mrow = p.mask == nullptr ? nullptr : p.mask + r * p.mask_stride;
         trow = std::is_same<TT, None>::value ? nullptr : static_cast<const TT*>(p.target) + r * p.target_stride;
         const int cols = (int)p.cols;
-        shift = V == 1 ? 0 : (int)((r * p.logits_stride) % V);
-        const int groups = (cols + shift + V - 1) / V, each = (groups + ranks - 1) / ranks;
+        shift = (int)((uint32_t)r * (uint32_t)p.logits_stride % V);
+        const int groups = (cols + shift + V - 1) / V, each = (groups + (1 << log_ranks) - 1) >> log_ranks;
         begin = min(groups, rank * each);
         end = min(groups, begin + each);
         full = max(begin, shift > 0 ? 1 : 0);
@@ -483,71 +514,75 @@ __device__ __forceinline__ void copy_async(uint4* to, const void* from) {
 // read it: the loads of one row run under the stores of the row before.
 // Otherwise (a part past the shared memory, or rows that are not aligned) each
 // pass reads the row itself, from L2 where it fits.
-template <typename TL, typename TT, int V, bool STAGED>
-__global__ void __launch_bounds__(kLongThreads, 3) policy_loss_long_kernel(gk_policy_loss_t p) {
+template <typename TL, typename TT, int V, bool STAGED, int THREADS>
+__global__ void __launch_bounds__(THREADS, 3 * kLongThreads / THREADS) policy_loss_long_kernel(gk_policy_loss_t p,
+                                                                                             int log_ranks) {
     cg::cluster_group cluster = cg::this_cluster();
-    const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    const int ranks = 1 << log_ranks, rank = log_ranks == 0 ? 0 : (int)cluster.block_rank();
     constexpr bool kTarget = !std::is_same<TT, None>::value;
-    constexpr int kWarps = kLongThreads / 32;
+    constexpr int kWarps = THREADS / 32;
     extern __shared__ uint4 staged[];
     // What each warp of the cluster found (maximum, sum, target sum, target
     // term), by turns: written by every CTA, read after the cluster barrier.
     // A slot is written again two rows later, a barrier after its last read.
     __shared__ float4 found[2][kMaxCluster * kWarps];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
-    const int64_t clusters = gridDim.x / ranks, first_row = blockIdx.x / ranks;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t clusters = gridDim.x >> log_ranks;
     const float inv_n = inverse_denominator(p);
     const int cols = (int)p.cols;
     double sum = 0.0;
     int turn = 0;
+    int64_t r = blockIdx.x >> log_ranks;
+    Part<TL, TT, V> part(p, r, rank, log_ranks);
     if constexpr (STAGED) {
-        const Part<TL, TT, V> part(p, first_row, rank, ranks);
-        const TL* from = part.lrow + ((int64_t)part.full * V - part.shift);
-        for (int k = tid; k < part.full_end - part.full; k += threads) copy_async(staged + k, from + k * V);
+        const TL* from = part.lrow + (part.full * V - part.shift);
+        for (int k = tid; k < part.full_end - part.full; k += THREADS) copy_async(staged + k, from + k * V);
     }
-    for (int64_t r = first_row; r < p.rows; r += clusters, turn ^= 1) {
-        const Part<TL, TT, V> part(p, r, rank, ranks);
+    while (r < p.rows) {
         const RowInput in = row_input(p, r, part.lrow, part.mrow);
         const int base = part.full * V - part.shift, count = part.full_end - part.full;
-        // f(group, index of its first entry, whether it is an edge); thread 0
-        // also takes the row's first edge and the last thread its last.
-        auto each_edge = [&](auto&& f) {
-            if (V > 1) {
-                if (tid == 0 && part.begin < part.full && part.begin < part.end) {
-                    Group<TL, V> h;
-                    h.load_edge(part.lrow, part.mrow, part.begin * V - part.shift, cols);
-                    f(h, part.begin * V - part.shift, true);
-                }
-                if (tid == threads - 1 && part.full_end < part.end && part.end - 1 >= part.full) {
-                    Group<TL, V> h;
-                    h.load_edge(part.lrow, part.mrow, (part.end - 1) * V - part.shift, cols);
-                    f(h, (part.end - 1) * V - part.shift, true);
-                }
-            }
-        };
-        auto load = [&](Group<TL, V>& h, int k) {
-            const TL* from = STAGED ? reinterpret_cast<const TL*>(staged + k) : part.lrow + base + k * V;
-            h.load(from, part.mrow == nullptr ? nullptr : part.mrow + base + k * V);
-        };
-        auto each_group = [&](auto&& f) {
-#pragma unroll 4
-            for (int k = tid; k < count; k += threads) {
+        // The row's first group where it is an edge is thread 0's, its last the last thread's.
+        const bool head = V > 1 && tid == 0 && part.begin < part.full && part.begin < part.end;
+        const bool tail = V > 1 && tid == THREADS - 1 && part.full_end < part.end && part.end - 1 >= part.full;
+        const TL* from = STAGED ? reinterpret_cast<const TL*>(staged) : part.lrow + base;
+        const uint8_t* mask = part.mrow == nullptr ? nullptr : part.mrow + base;
+        // f(group, index of its first entry, whether it is an edge) for this thread's groups.
+        auto edges = [&](auto&& f) {
+            if (head || tail) {
+                const int first = (head ? part.begin : part.end - 1) * V - part.shift;
                 Group<TL, V> h;
-                load(h, k);
-                f(h, base + k * V, false);
+                h.load_edge(part.lrow, part.mrow, first, cols);
+                f(h, first, true);
             }
-            each_edge(f);
+        };
+        auto groups = [&](auto&& f) {
+            if (part.mrow == nullptr) {
+#pragma unroll 4
+                for (int k = tid; k < count; k += THREADS) {
+                    Group<TL, V> h;
+                    h.template load<false>(from + k * V, nullptr);
+                    f(h, base + k * V, false);
+                }
+            } else {
+#pragma unroll 4
+                for (int k = tid; k < count; k += THREADS) {
+                    Group<TL, V> h;
+                    h.template load<true>(from + k * V, mask + k * V);
+                    f(h, base + k * V, false);
+                }
+            }
+            edges(f);
         };
         if constexpr (STAGED) asm volatile("cp.async.wait_all;" ::: "memory");
         Softmax acc;
         float total_t = 0.0f, kl = 0.0f;
-        each_group([&](const Group<TL, V>& h, int, bool) { acc.m = fmaxf(acc.m, h.top()); });
+        groups([&](const Group<TL, V>& h, int, bool) { acc.m = fmaxf(acc.m, h.top()); });
 #pragma unroll
         for (int o = 16; o; o >>= 1) acc.m = fmaxf(acc.m, __shfl_xor_sync(kFull, acc.m, o));
         {
             const Exp<TL> e(acc.m);
             float s2 = 0.0f;
-            each_group([&](const Group<TL, V>& h, int first, bool edge) {
+            groups([&](const Group<TL, V>& h, int first, bool edge) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) (i & 1 ? s2 : acc.s) += e(h.x(i));
                 if constexpr (kTarget) {
@@ -568,16 +603,17 @@ __global__ void __launch_bounds__(kLongThreads, 3) policy_loss_long_kernel(gk_po
         }
         const float4 mine = make_float4(acc.m, acc.s, total_t, kl);
         if (ranks > 1) {
-            if (lane < ranks) cluster.map_shared_rank(found[turn], lane)[rank * warps + warp] = mine;
+            if (lane < ranks) cluster.map_shared_rank(found[turn], lane)[rank * kWarps + warp] = mine;
             cluster.sync();
         } else {
             if (lane == 0) found[turn][warp] = mine;
             __syncthreads();
         }
         // Every warp joins what all found and forms the row's terms for itself.
-        const int all = ranks * warps;
+        const int all = ranks * kWarps;
         const float4 none = make_float4(-FLT_MAX, 0.0f, 0.0f, 0.0f);
-        const float4 f0 = lane < all ? found[turn][lane] : none, f1 = lane + 32 < all ? found[turn][lane + 32] : none;
+        const float4 f0 = lane < all ? found[turn][lane] : none;
+        const float4 f1 = kWarps * kMaxCluster > 32 && lane + 32 < all ? found[turn][lane + 32] : none;
         acc.m = f0.x, acc.s = f0.y;
         acc.join(f1.x, f1.y);
         acc.join_lanes(32);
@@ -592,64 +628,82 @@ __global__ void __launch_bounds__(kLongThreads, 3) policy_loss_long_kernel(gk_po
             write_row(p, r, o);
             sum += (double)(o.loss + (kTarget && o.inv_s != 0.0f ? p.target_weight * (kl + total_t * o.log_s) : 0.0f));
         }
-        TL* grow = static_cast<TL*>(p.grad) + r * p.cols;
-        const Exp<TL> e(o.m);
-        const float kt = inv_n * p.target_weight;
-        const float kp = inv_n * (p.target_weight * o.total_t - o.c) * o.inv_s * e.correct;
-        auto finish = [&](const Group<TL, V>& h, int first, bool edge) {
-            float t[V], g[V];
-            load_target<TT, V>(part.trow, h.legal, first, edge, t);
-            gradient_group<TL, TT, V>(h, t, e, kp, kt, g);
-            store_group<TL, V>(grow, first, cols, edge, g);
-        };
         // The next row of this CTA: its groups take the slots as the last pass empties them.
-        const bool more = STAGED && r + clusters < p.rows;
-        const Part<TL, TT, V> next(p, more ? r + clusters : r, rank, ranks);
-        const TL* next_from = next.lrow + ((int64_t)next.full * V - next.shift);
-        const int next_count = more ? next.full_end - next.full : 0;
+        const int64_t next_r = r + clusters;
+        const Part<TL, TT, V> next(p, next_r < p.rows ? next_r : r, rank, log_ranks);
+        const TL* next_from = next.lrow + (next.full * V - next.shift);
+        const int next_count = STAGED && next_r < p.rows ? next.full_end - next.full : 0;
+        TL* grow = static_cast<TL*>(p.grad) + r * p.cols;
         if (o.inv_s != 0.0f && p.grad != nullptr) {
+            const Exp<TL> e(o.m);
+            const float kt = inv_n * p.target_weight;
+            const float kp = inv_n * (p.target_weight * o.total_t - o.c) * o.inv_s * e.correct;
+            auto finish = [&](const Group<TL, V>& h, int first, bool edge) {
+                float t[V], g[V];
+                load_target<TT, V>(part.trow, h.legal, first, edge, t);
+                gradient_group<TL, TT, V>(h, t, e, kp, kt, g);
+                store_group<TL, V>(grow, first, cols, edge, g);
+            };
             constexpr int U = 4;
-            for (int k0 = tid; k0 < count; k0 += U * threads) {
+            int k = tid;
+            const int whole = next_count > 0 ? min(count, next_count) : count;
+            for (; k + (U - 1) * THREADS < whole; k += U * THREADS) {
                 Group<TL, V> h[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (k0 + u * threads < count) load(h[u], k0 + u * threads);
+                for (int u = 0; u < U; ++u) {
+                    if (part.mrow == nullptr)
+                        h[u].template load<false>(from + (k + u * THREADS) * V, nullptr);
+                    else
+                        h[u].template load<true>(from + (k + u * THREADS) * V, mask + (k + u * THREADS) * V);
+                }
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (k0 + u * threads < count) finish(h[u], base + (k0 + u * threads) * V, false);
+                for (int u = 0; u < U; ++u) finish(h[u], base + (k + u * THREADS) * V, false);
+                if (next_count > 0) {
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (k0 + u * threads < min(count, next_count))
-                        copy_async(staged + k0 + u * threads, next_from + (k0 + u * threads) * V);
+                    for (int u = 0; u < U; ++u)
+                        copy_async(staged + k + u * THREADS, next_from + (k + u * THREADS) * V);
+                }
+            }
+            for (; k < count; k += THREADS) {
+                Group<TL, V> h;
+                if (part.mrow == nullptr)
+                    h.template load<false>(from + k * V, nullptr);
+                else
+                    h.template load<true>(from + k * V, mask + k * V);
+                finish(h, base + k * V, false);
+                if (k < next_count) copy_async(staged + k, next_from + k * V);
             }
             // An odd row's part may be a group longer than the one before it.
-            if (count < next_count && tid == count % threads) copy_async(staged + count, next_from + count * V);
-            each_edge(finish);
+            if (count < next_count && tid == count % THREADS) copy_async(staged + count, next_from + count * V);
+            edges(finish);
             if (o.action >= 0) {
                 // The action's own part: the thread that wrote its group writes it again.
                 const int q = ((int)o.action + part.shift) / V;
-                const bool head = q < part.full, tail = q >= part.full_end;
+                const bool first = q < part.full, last = q >= part.full_end;
                 if (q >= part.begin && q < part.end &&
-                    tid == (head ? 0 : (tail ? threads - 1 : (q - part.full) % threads))) {
+                    tid == (first ? 0 : (last ? THREADS - 1 : (q - part.full) % THREADS))) {
                     float t = 0.0f;
                     if constexpr (kTarget) t = to_f(part.trow[o.action]);
                     grow[o.action] = from_f<TL>(kp * e(to_f(part.lrow[o.action])) - kt * t + inv_n * o.c);
                 }
             }
         } else {
-            for (int k = tid; k < next_count; k += threads) copy_async(staged + k, next_from + k * V);
+            for (int k = tid; k < next_count; k += THREADS) copy_async(staged + k, next_from + k * V);
             if (p.grad != nullptr)
                 for (int j = max(0, part.begin * V - part.shift) + tid; j < min(cols, part.end * V - part.shift);
-                     j += threads)
+                     j += THREADS)
                     grow[j] = from_f<TL>(0.0f);
         }
+        part = next;
+        r = next_r;
+        turn ^= 1;
     }
     if (ranks > 1) cluster.sync();  // no CTA leaves while another writes to its shared memory
     if (rank == 0 && tid == 0) {
         if (clusters == 1)
             finish_loss(p, sum);
         else
-            p.partials[first_row] = sum;
+            p.partials[blockIdx.x >> log_ranks] = sum;
     }
 }
 
@@ -669,7 +723,7 @@ __global__ void __launch_bounds__(256) policy_loss_backward_kernel(gk_policy_los
     for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += warps) {
         const int64_t r = it / chunks;
         const int chunk = (int)(it - r * chunks);
-        const Part<TL, TT, V> part(p, r, 0, 1);
+        const Part<TL, TT, V> part(p, r, 0, 0);
         TL* grow = static_cast<TL*>(p.grad) + r * p.cols;
         const float4 st = reinterpret_cast<const float4*>(p.stats)[r];  // maximum, 1 / sum, c, target sum
         const int64_t action = p.actions == nullptr ? -1 : p.actions[r];
@@ -685,8 +739,10 @@ __global__ void __launch_bounds__(256) policy_loss_backward_kernel(gk_policy_los
             Group<TL, V> h;
             if (edge)
                 h.load_edge(part.lrow, part.mrow, first, cols);
+            else if (part.mrow == nullptr)
+                h.template load<false>(part.lrow + first, nullptr);
             else
-                h.load(part.lrow + first, part.mrow == nullptr ? nullptr : part.mrow + first);
+                h.template load<true>(part.lrow + first, part.mrow + first);
             load_target<TT, V>(part.trow, h.legal, first, edge, t);
             if (st.y != 0.0f) {
                 gradient_group<TL, TT, V>(h, t, e, kp, kt, g);
@@ -733,44 +789,37 @@ bool vectorised(const gk_policy_loss_t& p, int v) {
 // How a long row is split and staged. A CTA's part is at most 72 KB, three to
 // an SM; the cluster grows until the part fits, and with fewer rows than the
 // SMs hold until the grid fills them, but no part gets shorter than two vectors
-// a thread. Short parts take fewer threads, four vectors each, so that more
-// rows are in flight.
+// a thread. Parts of less take 64 threads, so that more rows are in flight.
 struct LongPlan {
-    int cluster, threads;
+    int log_cluster, threads;
     bool staged;
     size_t smem;
 };
 constexpr int64_t kPartBytes = 72 << 10;
+constexpr int kShortThreads = 64;
 
 LongPlan long_plan(const gk_policy_loss_t& p, int v) {
     const int64_t groups = (p.cols + 2 * (v - 1)) / v;  // with the shift of an odd row
-    int c = 1;
-    auto part = [&](int k) { return (groups + k - 1) / k; };
-    while (c < kMaxCluster && (part(c) * 16 > kPartBytes ||
-                               (p.rows * c * 2 <= 3 * kSmCount && part(2 * c) >= 2 * kLongThreads)))
-        c *= 2;
+    int log = 0;
+    auto part = [&](int k) { return (groups + (1 << k) - 1) >> k; };
+    while ((1 << log) < kMaxCluster && (part(log) * 16 > kPartBytes || ((p.rows << (log + 1)) <= 3 * kSmCount &&
+                                                                        part(log + 1) >= 2 * kLongThreads)))
+        ++log;
     LongPlan plan{};
-    plan.cluster = c;
-    plan.threads = kLongThreads;
-    while (plan.threads > 32 && part(c) < plan.threads * 2) plan.threads /= 2;
-    plan.staged = v > 1 && part(c) * 16 <= kPartBytes;
-    plan.smem = plan.staged ? (size_t)part(c) * 16 : 0;
+    plan.log_cluster = log;
+    plan.staged = v > 1 && part(log) * 16 <= kPartBytes;
+    plan.threads = plan.staged && part(log) < 2 * kLongThreads ? kShortThreads : kLongThreads;
+    plan.smem = plan.staged ? (size_t)part(log) * 16 : 0;
     return plan;
 }
 
 int row_blocks(int64_t rows) { return blocks_for(rows, kRowWarps, kSmCount * 8); }
 
-// Most clusters of a long-row launch: CTAs of 3 * 256 threads an SM.
-int64_t most_clusters(const LongPlan& plan) {
-    const int64_t per_sm = 3 * kLongThreads / plan.threads;
-    return kSmCount * per_sm / plan.cluster;
-}
-
-template <typename TL, typename TT, int V, bool STAGED>
+template <typename TL, typename TT, int V, bool STAGED, int THREADS>
 int launch_long(const gk_policy_loss_t& p, const LongPlan& plan, int* clusters, cudaStream_t s) {
-    auto* kernel = policy_loss_long_kernel<TL, TT, V, STAGED>;
+    auto* kernel = policy_loss_long_kernel<TL, TT, V, STAGED, THREADS>;
     static bool done[64] = {};
-    static int resident[64][4] = {};  // clusters of 1, 2, 4, 8 full-size CTAs that the device holds at once
+    static int resident[64][4] = {};  // clusters of 1, 2, 4, 8 CTAs that the device holds at once
     int dev = 0;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
@@ -778,6 +827,7 @@ int launch_long(const gk_policy_loss_t& p, const LongPlan& plan, int* clusters, 
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    cfg.blockDim = dim3(THREADS);
     cfg.stream = s;
     if (!once_per_device(done, [&] {
             if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPartBytes) != cudaSuccess ||
@@ -786,26 +836,21 @@ int launch_long(const gk_policy_loss_t& p, const LongPlan& plan, int* clusters, 
             for (int i = 0; i < 4; ++i) {
                 attr[0].val.clusterDim.x = 1 << i;
                 cfg.gridDim = dim3(8);
-                cfg.blockDim = dim3(kLongThreads);
-                cfg.dynamicSmemBytes = STAGED ? kPartBytes : 0;
+                cfg.dynamicSmemBytes = !STAGED ? 0 : (THREADS == kLongThreads ? kPartBytes : 2 * kLongThreads * 16);
                 if (cudaOccupancyMaxActiveClusters(&resident[dev][i], kernel, &cfg) != cudaSuccess) return false;
             }
             return true;
         }))
         return launch_status();
     if (cudaGetDevice(&dev) != cudaSuccess) return launch_status();
-    int64_t most = most_clusters(plan);
-    int log = 0;
-    while ((1 << log) < plan.cluster) ++log;
     // GPCs of an odd number of SMs leave some out of a cluster: a grid that is
     // resident at once has no second round for the rest.
-    if (plan.threads == kLongThreads && resident[dev][log] > 0 && resident[dev][log] < most) most = resident[dev][log];
+    const int64_t most = resident[dev][plan.log_cluster] > 0 ? resident[dev][plan.log_cluster] : 1;
     *clusters = (int)(p.rows < most ? p.rows : most);
-    attr[0].val.clusterDim.x = plan.cluster;
-    cfg.gridDim = dim3((unsigned)(*clusters * plan.cluster));
-    cfg.blockDim = dim3(plan.threads);
+    attr[0].val.clusterDim.x = 1 << plan.log_cluster;
+    cfg.gridDim = dim3((unsigned)(*clusters << plan.log_cluster));
     cfg.dynamicSmemBytes = plan.smem;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, p);
+    return (int)cudaLaunchKernelEx(&cfg, kernel, p, plan.log_cluster);
 }
 
 template <typename TL, typename TT>
@@ -821,9 +866,15 @@ int forward(const gk_policy_loss_t& p, cudaStream_t s) {
         constexpr int V = kVec<TL>;
         const bool vec = vectorised(p, V);
         const LongPlan plan = long_plan(p, vec ? V : 1);
-        const int e = !vec ? launch_long<TL, TT, 1, false>(p, plan, &parts, s)
-                           : (plan.staged ? launch_long<TL, TT, V, true>(p, plan, &parts, s)
-                                          : launch_long<TL, TT, V, false>(p, plan, &parts, s));
+        int e;
+        if (!vec)
+            e = launch_long<TL, TT, 1, false, kLongThreads>(p, plan, &parts, s);
+        else if (!plan.staged)
+            e = launch_long<TL, TT, V, false, kLongThreads>(p, plan, &parts, s);
+        else if (plan.threads == kLongThreads)
+            e = launch_long<TL, TT, V, true, kLongThreads>(p, plan, &parts, s);
+        else
+            e = launch_long<TL, TT, V, true, kShortThreads>(p, plan, &parts, s);
         if (e != 0) return e;
     }
     if (parts > 1) policy_loss_sum_kernel<<<1, 256, 0, s>>>(p, parts);
@@ -863,7 +914,7 @@ extern "C" {
 int gk_policy_loss_parts(int64_t rows, int64_t cols) {
     if (rows < 1 || cols < 1) return 0;
     if (cols <= gk::kShortRow) return gk::row_blocks(rows);
-    const int64_t most = gk::kSmCount * 3 * (gk::kLongThreads / 32);  // clusters of any plan
+    const int64_t most = gk::kSmCount * 32;  // clusters of any plan: the CTAs that the SMs hold at most
     return (int)(rows < most ? rows : most);
 }
 
