@@ -11,7 +11,10 @@ from .gpu_rules import (  # noqa: F401
     GPU_WINNER, GpuStateBatch,
 )
 from .gpu_puct import GpuPUCT, GpuPUCTOptions, GpuSearchResult, HashEvaluator  # noqa: F401
-from .training import Cell, EndReason, GameData, TrainingBatch, TrainingSample, collect_gpu_puct_games  # noqa: F401
+from .training import (  # noqa: F401
+    Cell, EndReason, GameData, PolicyValueLoss, TrainingBatch, TrainingSample, collect_gpu_puct_games,
+    policy_value_loss,
+)
 from .replay import DeviceReplayBuffer, validate_rows  # noqa: F401
 from .batched_puct import BatchedSearchResult, GpuBatchedPUCT, PUCTOptions  # noqa: F401
 from .evaluation import EvaluationResult, evaluate_models_gpu  # noqa: F401
@@ -19,3 +22,4 @@ from .engine_api import BatchedPUCT, PUCTMoveStatistics, PUCTSearchResult, encod
 from .losses import PolicyLoss, policy_loss  # noqa: F401
 from .packing import PackedActivation, pack_activation, packed_activations  # noqa: F401
 from .layers import check_linear, linear  # noqa: F401
+from .model import training_forward  # noqa: F401

@@ -19,6 +19,7 @@ bias, which is what the native network consumes.
 
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -195,6 +196,40 @@ class GroupNormPolicyValueNet(nn.Module):
     def forward(self, features: torch.Tensor):
         shared = self.trunk(features)
         return self.policy_head(shared), self.value_head(shared).squeeze(-1)
+
+
+def training_forward(model, features: torch.Tensor, *, checkpoint=None):
+    """``model(features)`` of a PolicyValueNet or GroupNormPolicyValueNet on
+    CUDA with its fully connected heads on ``linear``: (logits [N, 82], values
+    [N]), for a training step. ``checkpoint="e4m3"`` keeps the activations for
+    the backward pass in 8 bits: the trunk's through ``packed_activations``,
+    the heads' through ``linear``'s own. The heads run in the dtype that the
+    trunk hands them (bf16 under autocast)."""
+    from .layers import linear
+    from .packing import packed_activations
+
+    if not isinstance(model, (PolicyValueNet, GroupNormPolicyValueNet)):
+        raise TypeError("training_forward runs a PolicyValueNet or a GroupNormPolicyValueNet")
+    if checkpoint not in (None, "e4m3"):
+        raise ValueError('checkpoint must be None or "e4m3"')
+    with contextlib.nullcontext() if checkpoint is None else packed_activations():
+        if isinstance(model, PolicyValueNet):
+            x = torch.relu(model.stem_bn(model.stem(features)))
+            for block in model.blocks:
+                x = block(x)
+            p = torch.relu(model.policy_bn(model.policy_conv(x))).flatten(1)
+            v = torch.relu(model.value_bn(model.value_conv(x))).flatten(1)
+            policy, hidden, out = model.policy_fc, model.value_fc1, model.value_fc2
+        else:
+            x = model.trunk(features)
+            p, v = model.policy_head[:4](x), model.value_head[:4](x)
+            policy, hidden, out = model.policy_head[4], model.value_head[4], model.value_head[6]
+
+    def head(t, layer, activation):
+        return linear(t, layer.weight.to(t.dtype), layer.bias.to(t.dtype), activation=activation,
+                      checkpoint=checkpoint)
+
+    return head(p, policy, None), head(head(v, hidden, "relu"), out, "tanh").squeeze(1)
 
 
 def random_groupnorm_network(channels: int, blocks: int, seed: int) -> GroupNormPolicyValueNet:

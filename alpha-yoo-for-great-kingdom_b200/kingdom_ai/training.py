@@ -22,6 +22,7 @@ import copy
 import enum
 import math
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -77,6 +78,35 @@ class GameData:
     winner: Cell
     reason: EndReason
     action_history: tuple | None = None
+
+
+class PolicyValueLoss(NamedTuple):
+    loss: torch.Tensor    # policy + value_weight * value
+    policy: torch.Tensor  # mean KL of the search's visit shares to the policy over the legal actions
+    value: torch.Tensor   # mean squared error of the value
+
+
+def policy_value_loss(model, batch: TrainingBatch, *, value_weight=1.0, checkpoint=None) -> PolicyValueLoss:
+    """The loss of a training step on a sampled batch (python/kingdom_ai/
+    training.py:213-230, ``train_step``'s losses): the network's heads run on
+    ``linear``, the policy term on ``policy_loss`` over the batch's legal
+    actions, and ``checkpoint="e4m3"`` keeps the activations for the backward
+    pass in 8 bits (``training_forward``). The policy term is the cross entropy
+    to ``batch.policy`` less the target's own entropy, so its gradient is the
+    cross entropy's. The model and the batch are on one CUDA device."""
+    from .losses import policy_loss
+    from .model import training_forward
+
+    if not isinstance(batch, TrainingBatch):
+        raise TypeError("batch must be a TrainingBatch")
+    if isinstance(value_weight, bool) or not isinstance(value_weight, (int, float)):
+        raise TypeError("value_weight must be a real number")
+    if not math.isfinite(value_weight) or value_weight < 0:
+        raise ValueError("value_weight must be finite and non-negative")
+    logits, values = training_forward(model, batch.features, checkpoint=checkpoint)
+    policy = policy_loss(logits, legal_mask=batch.legal_mask, target=batch.policy).loss
+    value = (values.float() - batch.value).square().mean()
+    return PolicyValueLoss(policy + value_weight * value, policy.detach(), value.detach())
 
 
 def _check_schedule(temperature, temperature_moves, final_temperature):
