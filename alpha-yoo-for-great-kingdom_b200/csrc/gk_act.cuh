@@ -8,33 +8,79 @@
 
 namespace gk {
 
+// Activations of values that end in 16 bits are evaluated to about 2^-20 of
+// themselves (a 16-bit type keeps 2^-9 or 2^-12); those of fp32 with CUDA's
+// erff and expf. The quick gelu has one exponential for both of its parts:
+//   Phi(-a) = e^(-a^2/2) t Q(t) / 2,  t = 1 / (1 + 0.45 a / sqrt 2),  a >= 0,
+// with Q the degree-7 minimax fit of erfc(x) e^(x^2) / t over x in [0, 9.5]
+// (relative error 3e-7), so the far negative side keeps its relative accuracy.
+__device__ __forceinline__ float quick_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float quick_rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Phi(z); e = e^(-z^2/2).
+__device__ __forceinline__ float quick_cdf(float z, float& e) {
+    const float t = quick_rcp(fmaf(fabsf(z), 0.31819805153394639f, 1.0f));
+    e = quick_ex2(z * z * -0.72134752044448170f);
+    float q = 0.06631925f;
+    q = fmaf(q, t, -0.23788772f);
+    q = fmaf(q, t, 0.20455141f);
+    q = fmaf(q, t, 0.04441312f);
+    q = fmaf(q, t, 0.18637764f);
+    q = fmaf(q, t, 0.22879136f);
+    q = fmaf(q, t, 0.25351842f);
+    q = fmaf(q, t, 0.25391682f);
+    const float tail = 0.5f * e * t * q;
+    return z < 0.0f ? tail : 1.0f - tail;
+}
+
+template <bool QUICK>
 __device__ __forceinline__ float act_value(float z, int act) {
     switch (act) {
         case GK_ACT_RELU: return z > 0.0f ? z : (z != z ? z : 0.0f);
         case GK_ACT_TANH: return tanhf(z);
-        case GK_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-        case GK_ACT_SILU: return z / (1.0f + expf(-z));
+        case GK_ACT_GELU:
+            if (QUICK) {
+                float e;
+                return z * quick_cdf(z, e);
+            }
+            return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        case GK_ACT_SILU:
+            if (QUICK) return z * quick_rcp(1.0f + quick_ex2(z * -1.4426950408889634f));
+            return z / (1.0f + expf(-z));
         default: return z;
     }
 }
 
 // The derivative. relu and tanh take the output y, gelu and silu the sum z
 // before the activation: the value that the forward pass kept for them.
+template <bool QUICK>
 __device__ __forceinline__ float act_slope(float kept, int act) {
     switch (act) {
         case GK_ACT_RELU: return kept > 0.0f ? 1.0f : 0.0f;
         case GK_ACT_TANH: return 1.0f - kept * kept;
         case GK_ACT_GELU: {
-            // Far out z exp(-z^2/2) is 0, but inf * 0 is not.
+            if (kept != kept) return kept;
+            // Far out z e^(-z^2/2) is 0, but inf * 0 is not.
             const float z = fminf(fmaxf(kept, -32.0f), 32.0f);
-            return kept != kept ? kept
-                                : 0.5f * (1.0f + erff(z * 0.70710678118654752f)) +
-                                      z * expf(-0.5f * z * z) * 0.39894228040143268f;
+            if (QUICK) {
+                float e;
+                const float cdf = quick_cdf(z, e);
+                return fmaf(z * 0.39894228040143268f, e, cdf);
+            }
+            return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
         }
         case GK_ACT_SILU: {
-            const float s = 1.0f / (1.0f + expf(-kept));
-            // At -inf s is 0 and s * z is not a number; the limit is 0.
-            return s == 0.0f ? 0.0f : s * (1.0f + kept * (1.0f - s));
+            const float s = QUICK ? quick_rcp(1.0f + quick_ex2(kept * -1.4426950408889634f))
+                                  : 1.0f / (1.0f + expf(-kept));
+            // At -inf s is 0 and s * z is not a number; the limit is 0. At +inf z (1 - s) is not one; the limit is 1.
+            return s == 0.0f ? 0.0f : (s == 1.0f ? 1.0f : s * (1.0f + kept * (1.0f - s)));
         }
         default: return 1.0f;
     }

@@ -38,7 +38,7 @@ struct Epilogue {
     int m, n;
     int activation;
     int bf16;
-    int aligned;  // every row of out, residual and pre starts on 16 bytes
+    int aligned;  // every row of out, residual and pre, and the bias, start on 16 bytes
 };
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kSplitThreads) gemm_split_kernel(const __grid_
                 for (int j = 0; j < count; ++j) store16(ep.pre, m * ep.pre_ld + n + j, v[j], bf16);
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = act_value(v[j], ep.activation);
+        for (int j = 0; j < 4; ++j) v[j] = act_value<true>(v[j], ep.activation);
         if (whole)
             *reinterpret_cast<uint2*>(static_cast<uint16_t*>(ep.out) + m * ep.out_ld + n) =
                 make_uint2(pack16(v[0], v[1], bf16), pack16(v[2], v[3], bf16));
@@ -317,7 +317,7 @@ __device__ __forceinline__ void tile_at(int id, int tiles_m, int tiles_n, int& t
 template <int ACT>
 __device__ __forceinline__ void activate(float (&v)[32]) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = act_value(v[i], ACT);
+    for (int i = 0; i < 32; ++i) v[i] = act_value<true>(v[i], ACT);
 }
 __device__ __forceinline__ void activate(float (&v)[32], int act) {
     switch (act) {
@@ -344,8 +344,17 @@ __device__ __forceinline__ void finish_patch(const Epilogue& ep, float (&v)[32],
     if (ep.aligned && n + 32 <= ep.n) {
         const bool in = row < ep.m;
         if (ep.bias != nullptr) {
+            // Every lane reads the same 64 bytes.
+            const uint4* b = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(ep.bias) + n);
+            uint4 x[4];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += load16(ep.bias, n + i, bf16);
+            for (int i = 0; i < 4; ++i) x[i] = __ldg(b + i);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float lo, hi;
+                unpack16(reinterpret_cast<const uint32_t*>(x)[i], bf16, lo, hi);
+                v[2 * i] += lo, v[2 * i + 1] += hi;
+            }
         }
         if (ep.residual != nullptr && in) {
             const uint4* r = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(ep.residual) +
@@ -380,7 +389,7 @@ __device__ __forceinline__ void finish_patch(const Epilogue& ep, float (&v)[32],
         float z = patch[r * 33 + lane] + bias;
         if (ep.residual != nullptr) z += load16(ep.residual, m * ep.residual_ld + col, bf16);
         if (ep.pre != nullptr) store16(ep.pre, m * ep.pre_ld + col, z, bf16);
-        store16(ep.out, m * ep.out_ld + col, act_value(z, ep.activation), bf16);
+        store16(ep.out, m * ep.out_ld + col, act_value<true>(z, ep.activation), bf16);
     }
 }
 
@@ -545,7 +554,7 @@ bool encode(CUtensorMap* map, const void* p, int64_t ld, int across, int64_t mn,
 Epilogue epilogue_of(const GemmArgs& g) {
     Epilogue e{g.out, g.bias, g.residual, g.pre, g.out_ld, g.residual_ld, g.pre_ld, (int)g.m, (int)g.n,
                g.activation, g.dtype == GK_BF16, 0};
-    e.aligned = aligned16(g.out) && g.out_ld % 8 == 0 &&
+    e.aligned = aligned16(g.out) && (g.bias == nullptr || aligned16(g.bias)) && g.out_ld % 8 == 0 &&
                 (g.residual == nullptr || (aligned16(g.residual) && g.residual_ld % 8 == 0)) &&
                 (g.pre == nullptr || (aligned16(g.pre) && g.pre_ld % 8 == 0));
     return e;

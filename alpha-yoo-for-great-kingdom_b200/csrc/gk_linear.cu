@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(256) linear_few_kernel(FewRows p) {
         if (p.bias != nullptr) v += as_float<T>(static_cast<const T*>(p.bias)[n]);
         if (p.residual != nullptr) v += as_float<T>(static_cast<const T*>(p.residual)[m * p.residual_stride + n]);
         if (p.pre != nullptr) static_cast<T*>(p.pre)[(int64_t)m * p.n + n] = rounded<T>(v);
-        static_cast<T*>(p.y)[(int64_t)m * p.n + n] = rounded<T>(act_value(v, p.activation));
+        static_cast<T*>(p.y)[(int64_t)m * p.n + n] = rounded<T>(act_value<sizeof(T) == 2>(v, p.activation));
     }
 }
 
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(256) gemm32_kernel(Gemm32 g, int tiles_n) {
         if (g.bias != nullptr) v += g.bias[n];
         if (g.residual != nullptr) v += g.residual[m * g.residual_ld + n];
         if (g.pre != nullptr) g.pre[m * g.pre_ld + n] = v;
-        g.out[m * g.out_ld + n] = act_value(v, g.activation);
+        g.out[m * g.out_ld + n] = act_value<false>(v, g.activation);
     }
     if (ranks > 1) cluster.sync();  // no CTA leaves while another reads its part
 }
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(Slope p) {
                     kept[0] = *keptp;
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float z = as_float<T>(dy[i]) * act_slope(as_float<T>(kept[i]), p.activation);
+                    const float z = as_float<T>(dy[i]) * act_slope<sizeof(T) == 2>(as_float<T>(kept[i]), p.activation);
                     sum[i] += z;
                     dy[i] = rounded<T>(z);
                 }
@@ -363,14 +363,25 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(Slope p) {
     }
 }
 
-// db from the slabs' sums, in their order.
+// db from the slabs' sums: 32 columns a block, eight warps each add every
+// eighth slab, then in order.
 template <typename T>
 __global__ void __launch_bounds__(256) linear_bias_kernel(const float* sums, int64_t n, int slabs, T* db) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= n) return;
+    __shared__ float part[8][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
     float v = 0.0f;
-    for (int s = 0; s < slabs; ++s) v += sums[(int64_t)s * n + c];
-    db[c] = rounded<T>(v);
+    if (c < n) {
+#pragma unroll 4
+        for (int s = warp; s < slabs; s += 8) v += sums[(int64_t)s * n + c];
+    }
+    part[warp][lane] = v;
+    __syncthreads();
+    if (warp == 0 && c < n) {
+#pragma unroll
+        for (int w = 1; w < 8; ++w) v += part[w][lane];
+        db[c] = rounded<T>(v);
+    }
 }
 
 struct SlopePlan {
@@ -553,7 +564,7 @@ int backward(const gk_linear_grad_t& p, void* workspace, uint32_t* status, cudaS
             linear_slope_kernel<T, 1><<<grid, 256, 0, s>>>(a);
         if ((e = launch_status()) != 0) return e;
         if (p.db != nullptr) {
-            linear_bias_kernel<T><<<(unsigned)((p.n + 255) / 256), 256, 0, s>>>(b.sums, p.n, b.slope.slabs,
+            linear_bias_kernel<T><<<(unsigned)((p.n + 31) / 32), 256, 0, s>>>(b.sums, p.n, b.slope.slabs,
                                                                                  static_cast<T*>(p.db));
             if ((e = launch_status()) != 0) return e;
         }
