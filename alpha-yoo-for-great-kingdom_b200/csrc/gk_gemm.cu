@@ -257,7 +257,7 @@ template <int BN>
 struct Pair {
     static constexpr int kA = 128 * kBK * 2, kB = BN / 2 * kBK * 2, kStage = kA + kB;
     static constexpr int kStages = BN == 256 ? 6 : 8;
-    static constexpr int kPatch = 32 * 33 * 4;  // a warp's 32 x 32 fp32 patch for rows that are not aligned
+    static constexpr int kPatch = 4096;  // an epilogue warp's 32 rows x 64 outputs
     static constexpr int kSmem = kStages * kStage + 8 * kPatch + 1024;
     static constexpr uint32_t kTmem = 2 * BN;
 };
@@ -328,65 +328,86 @@ __device__ __forceinline__ void activate(float (&v)[32], int act) {
         default: break;
     }
 }
-__device__ __forceinline__ void store_row32(void* p, int64_t at, const float (&v)[32], bool bf16) {
-    uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at);
+
+// A patch is 32 rows of 128 bytes whose 16-byte chunks are swizzled by the row,
+// as TMA's 128-byte swizzle lays them: no bank conflict by rows or by columns.
+__device__ __forceinline__ uint4* patch_chunk(uint8_t* patch, int row, int chunk) {
+    return reinterpret_cast<uint4*>(patch + row * 128 + ((chunk ^ (row & 7)) << 4));
+}
+// This lane's row, columns [32 half, 32 half + 32).
+__device__ __forceinline__ void put_row(uint8_t* patch, int lane, int half, const float (&v)[32], bool bf16) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        to[i] = make_uint4(pack16(v[8 * i], v[8 * i + 1], bf16), pack16(v[8 * i + 2], v[8 * i + 3], bf16),
-                           pack16(v[8 * i + 4], v[8 * i + 5], bf16), pack16(v[8 * i + 6], v[8 * i + 7], bf16));
+        *patch_chunk(patch, lane, half * 4 + i) =
+            make_uint4(pack16(v[8 * i], v[8 * i + 1], bf16), pack16(v[8 * i + 2], v[8 * i + 3], bf16),
+                       pack16(v[8 * i + 4], v[8 * i + 5], bf16), pack16(v[8 * i + 6], v[8 * i + 7], bf16));
+}
+__device__ __forceinline__ void add_row(const uint8_t* patch, int lane, int half, float (&v)[32], bool bf16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint4 x = *patch_chunk(const_cast<uint8_t*>(patch), lane, half * 4 + i);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float lo, hi;
+            unpack16(w[j], bf16, lo, hi);
+            v[8 * i + 2 * j] += lo, v[8 * i + 2 * j + 1] += hi;
+        }
+    }
+}
+__device__ __forceinline__ void add_bias(const Epilogue& ep, int n, float (&v)[32], bool bf16) {
+    if (ep.aligned && n + 32 <= ep.n) {  // every lane reads the same 64 bytes
+        const uint4* b = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(ep.bias) + n);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 x = __ldg(b + i);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float lo, hi;
+                unpack16(w[j], bf16, lo, hi);
+                v[8 * i + 2 * j] += lo, v[8 * i + 2 * j + 1] += hi;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (n + i < ep.n) v[i] += load16(ep.bias, n + i, bf16);
+    }
+}
+// The warp's patch to rows [row0, row0 + 32), columns [n, n + 64) of an output; TMA clips what lies outside.
+__device__ __forceinline__ void store_patch(const CUtensorMap* map, uint8_t* patch, int n, int row0, int lane) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map),
+                     "r"(n), "r"(row0), "r"(smem_u32(patch))
+                     : "memory");
+        bulk_commit();
+    }
+}
+// The patch may be written again once the last store has read it.
+__device__ __forceinline__ void patch_free(int lane) {
+    if (lane == 0) bulk_wait_read<0>();
+    __syncwarp();
 }
 
-// 32 rows (a lane each) by 32 columns of sums: bias, residual, activation, stores.
-__device__ __forceinline__ void finish_patch(const Epilogue& ep, float (&v)[32], int row0, int lane, int n,
-                                             float* patch) {
+// Rows that do not start on 16 bytes: 32 rows by 32 columns of fp32 through the patch, a lane a column.
+__device__ __forceinline__ void finish_ragged(const Epilogue& ep, const float (&v)[32], int row0, int lane, int n,
+                                              uint8_t* patch) {
     const bool bf16 = ep.bf16 != 0;
-    const int row = row0 + lane;
-    if (ep.aligned && n + 32 <= ep.n) {
-        const bool in = row < ep.m;
-        if (ep.bias != nullptr) {
-            // Every lane reads the same 64 bytes.
-            const uint4* b = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(ep.bias) + n);
-            uint4 x[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = __ldg(b + i);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float lo, hi;
-                unpack16(reinterpret_cast<const uint32_t*>(x)[i], bf16, lo, hi);
-                v[2 * i] += lo, v[2 * i + 1] += hi;
-            }
-        }
-        if (ep.residual != nullptr && in) {
-            const uint4* r = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(ep.residual) +
-                                                            row * ep.residual_ld + n);
-            uint4 x[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = __ldg(r + i);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float lo, hi;
-                unpack16(reinterpret_cast<const uint32_t*>(x)[i], bf16, lo, hi);
-                v[2 * i] += lo, v[2 * i + 1] += hi;
-            }
-        }
-        if (ep.pre != nullptr && in) store_row32(ep.pre, row * ep.pre_ld + n, v, bf16);
-        activate(v, ep.activation);
-        if (in) store_row32(ep.out, row * ep.out_ld + n, v, bf16);
-        return;
-    }
-    // Rows that do not start on 16 bytes, or the last columns: a lane a column.
+    float* cell = reinterpret_cast<float*>(patch);  // column i of row r lies at i ^ r
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 32; ++i) patch[lane * 33 + i] = v[i];
+    for (int i = 0; i < 32; ++i) cell[lane * 32 + (i ^ lane)] = v[i];
     __syncwarp();
     const int col = n + lane;
     if (col >= ep.n) return;
-    const float bias = ep.bias != nullptr ? load16(ep.bias, col, bf16) : 0.0f;
     const int rows = min(32, ep.m - row0);
 #pragma unroll 4
     for (int r = 0; r < rows; ++r) {
         const int64_t m = row0 + r;
-        float z = patch[r * 33 + lane] + bias;
+        float z = cell[r * 32 + (lane ^ r)];
         if (ep.residual != nullptr) z += load16(ep.residual, m * ep.residual_ld + col, bf16);
         if (ep.pre != nullptr) store16(ep.pre, m * ep.pre_ld + col, z, bf16);
         store16(ep.out, m * ep.out_ld + col, act_value<true>(z, ep.activation), bf16);
@@ -395,7 +416,8 @@ __device__ __forceinline__ void finish_patch(const Epilogue& ep, float (&v)[32],
 
 template <int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
-    gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, Epilogue ep,
+    gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
+                     const __grid_constant__ CUtensorMap t_out, const __grid_constant__ CUtensorMap t_pre, Epilogue ep,
                      int tiles_m, int tiles_n, int k_blocks, int a_across, int b_across, uint32_t* status) {
     using P = Pair<BN>;
     extern __shared__ uint8_t raw[];
@@ -486,29 +508,75 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         }
     } else if (warp >= 4) {
         const int quadrant = warp & 3, half = (warp - 4) >> 2;
-        float* patch = reinterpret_cast<float*>(base + P::kStages * P::kStage) + (warp - 4) * (P::kPatch / 4);
+        uint8_t* patch = base + P::kStages * P::kStage + (warp - 4) * P::kPatch;
+        const bool bf16 = ep.bf16 != 0;
         int n = 0;
         for (int t = pair; t < tiles; t += pairs, ++n) {
             const int a = n & 1, use = n >> 1;
             int tm, tn;
             tile_at(t, tiles_m, tiles_n, tm, tn);
+            const int row0 = tm * 256 + rank * 128 + quadrant * 32, n0 = tn * BN + half * (BN / 2);
             // Every lane waits: the verdict is the warp's.
             if (__any_sync(0xffffffffu, !mbar_wait(smem_u32(&acc_full[a]), use & 1, status))) break;
             tc_fence_after();
-            const int row0 = tm * 256 + rank * 128 + quadrant * 32, n0 = tn * BN + half * (BN / 2);
             const uint32_t from = tmem + ((uint32_t)(quadrant * 32) << 16) + a * BN + half * (BN / 2);
 #pragma unroll 1
-            for (int c = 0; c < BN / 2; c += 32) {
-                float v[32];
-                tmem_ld32(from + c, v);
-                if (c + 32 == BN / 2) {  // the last columns are in registers: the accumulator is free
+            for (int c = 0; c < BN / 2; c += 64) {
+                const bool in = row0 < ep.m && n0 + c < ep.n;
+                uint4 held[8];
+                const bool residual = in && ep.aligned && ep.residual != nullptr;
+                if (residual) {  // eight lanes a row of 128 bytes, in flight while TMEM is read
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int row = row0 + i * 4 + (lane >> 3), col = n0 + c + (lane & 7) * 8;
+                        held[i] = row < ep.m && col < ep.n
+                                      ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(ep.residual) +
+                                                                            row * ep.residual_ld + col))
+                                      : make_uint4(0, 0, 0, 0);
+                    }
+                }
+                float v0[32], v1[32];
+                tmem_ld32x2(from + c, from + c + 32, v0, v1);
+                if (c + 64 == BN / 2) {  // the last columns are in registers: the accumulator is free
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) arrive_at(cluster_address(smem_u32(&acc_empty[a]), 0));
                 }
-                if (row0 < ep.m && n0 + c < ep.n) finish_patch(ep, v, row0, lane, n0 + c, patch);
+                if (!in) continue;
+                if (ep.bias != nullptr) {
+                    add_bias(ep, n0 + c, v0, bf16);
+                    add_bias(ep, n0 + c + 32, v1, bf16);
+                }
+                if (!ep.aligned) {
+                    finish_ragged(ep, v0, row0, lane, n0 + c, patch);
+                    if (n0 + c + 32 < ep.n) finish_ragged(ep, v1, row0, lane, n0 + c + 32, patch);
+                    continue;
+                }
+                patch_free(lane);
+                if (residual) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) *patch_chunk(patch, i * 4 + (lane >> 3), lane & 7) = held[i];
+                    __syncwarp();
+                    add_row(patch, lane, 0, v0, bf16);
+                    add_row(patch, lane, 1, v1, bf16);
+                }
+                if (ep.pre != nullptr) {  // each lane has read its row of the residual and writes the same row
+                    put_row(patch, lane, 0, v0, bf16);
+                    put_row(patch, lane, 1, v1, bf16);
+                    store_patch(&t_pre, patch, n0 + c, row0, lane);
+                    activate(v0, ep.activation);
+                    activate(v1, ep.activation);
+                    patch_free(lane);
+                } else {
+                    activate(v0, ep.activation);
+                    activate(v1, ep.activation);
+                }
+                put_row(patch, lane, 0, v0, bf16);
+                put_row(patch, lane, 1, v1, bf16);
+                store_patch(&t_out, patch, n0 + c, row0, lane);
             }
         }
+        if (lane == 0) bulk_wait<0>();  // the stores are done before the block ends
     }
     __syncwarp();
     tc_fence_before();
@@ -602,15 +670,20 @@ int launch_pair(const GemmArgs& g, uint32_t* status, cudaStream_t stream) {
             return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kSmem) == cudaSuccess;
         }))
         return launch_status();
-    CUtensorMap ta, tb;
+    const Epilogue ep = epilogue_of(g);
+    CUtensorMap ta, tb, t_out = {}, t_pre = {};
     if (!encode(&ta, g.a, g.a_ld, g.a_across, g.m, g.k, 128, g.dtype) ||
         !encode(&tb, g.b, g.b_ld, g.b_across, g.n, g.k, BN / 2, g.dtype))
+        return GK_EINVAL;
+    // The outputs as [m, n] with n contiguous, in boxes of 64 columns by 32 rows.
+    if (ep.aligned && (!encode(&t_out, g.out, g.out_ld, 0, g.m, g.n, 32, g.dtype) ||
+                       (g.pre != nullptr && !encode(&t_pre, g.pre, g.pre_ld, 0, g.m, g.n, 32, g.dtype))))
         return GK_EINVAL;
     const int64_t tiles_m = (g.m + 255) / 256, tiles_n = (g.n + BN - 1) / BN;
     if (tiles_m * tiles_n >= (1ll << 31) - kSmCount) return GK_EINVAL;
     const int64_t pairs = tiles_m * tiles_n < kSmCount / 2 ? tiles_m * tiles_n : kSmCount / 2;
     kernel<<<(unsigned)(2 * pairs), kPairThreads, P::kSmem, stream>>>(
-        ta, tb, epilogue_of(g), (int)tiles_m, (int)tiles_n, (int)((g.k + kBK - 1) / kBK), g.a_across, g.b_across,
+        ta, tb, t_out, t_pre, ep, (int)tiles_m, (int)tiles_n, (int)((g.k + kBK - 1) / kBK), g.a_across, g.b_across,
         status);
     return launch_status();
 }
