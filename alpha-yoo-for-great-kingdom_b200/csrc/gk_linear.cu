@@ -297,7 +297,7 @@ int gemm32(const Gemm32& g, cudaStream_t s) {
 
 struct Slope {
     const void* dy;
-    const void* kept;  // [m, n] contiguous, or nullptr without activation
+    const void* kept;  // [m, n] contiguous; unused without activation
     void* dz;          // or nullptr: sums only
     float* sums;       // [slabs, n] column sums of each slab of rows, or nullptr
     int64_t dy_stride, dz_stride;
@@ -305,47 +305,60 @@ struct Slope {
     int activation;
 };
 
-// 32 lanes of V columns by 8 rows at a time down a slab of rows.
-template <typename T, int V>
-__global__ void __launch_bounds__(256) linear_slope_kernel(Slope p) {
+// A warp goes down a slab of rows along 32 V columns; `across` of a block's
+// eight warps lie side by side (whole lines of a row next to one another), the
+// others take rows in turn.
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(256, 3) linear_slope_kernel(Slope p, int across) {
+    constexpr bool kSlope = ACT != GK_ACT_NONE;
     __shared__ float sums[8][32 * V];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * V, r0 = (int64_t)blockIdx.y * p.slab;
+    const int side = warp % across, down = warp / across, step = 8 / across;
+    const int64_t first = (int64_t)blockIdx.x * 32 * V * across;
+    const int64_t c = first + (side * 32 + lane) * V, r0 = (int64_t)blockIdx.y * p.slab;
     const int64_t r1 = r0 + p.slab < p.m ? r0 + p.slab : p.m;
     float sum[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.0f;
     if (c < p.n) {
-#pragma unroll 4
-        for (int64_t r = r0 + warp; r < r1; r += 8) {
-            alignas(16) T dy[V], kept[V];
-            const T* dyp = static_cast<const T*>(p.dy) + r * p.dy_stride + c;
-            const T* keptp = static_cast<const T*>(p.kept) + r * p.n + c;
-            if constexpr (V > 1)
-                *reinterpret_cast<uint4*>(dy) = __ldg(reinterpret_cast<const uint4*>(dyp));
-            else
-                dy[0] = *dyp;
-            if (p.kept != nullptr) {
-                if constexpr (V > 1)
-                    *reinterpret_cast<uint4*>(kept) = __ldg(reinterpret_cast<const uint4*>(keptp));
-                else
-                    kept[0] = *keptp;
+        const T* dyp = static_cast<const T*>(p.dy) + c;
+        const T* keptp = static_cast<const T*>(p.kept) + c;
+        T* dzp = static_cast<T*>(p.dz) + c;
+        constexpr int U = 4;  // rows in flight
+        for (int64_t r = r0 + down; r < r1; r += U * step) {
+            alignas(16) T dy[U][V], kept[U][V];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t row = r + u * step;
+                if (row >= r1) continue;
+                if constexpr (V > 1) {
+                    *reinterpret_cast<uint4*>(dy[u]) = __ldcs(reinterpret_cast<const uint4*>(dyp + row * p.dy_stride));
+                    if constexpr (kSlope)
+                        *reinterpret_cast<uint4*>(kept[u]) = __ldcs(reinterpret_cast<const uint4*>(keptp + row * p.n));
+                } else {
+                    dy[u][0] = dyp[row * p.dy_stride];
+                    if constexpr (kSlope) kept[u][0] = keptp[row * p.n];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t row = r + u * step;
+                if (row >= r1) continue;
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float z = as_float<T>(dy[i]) * act_slope<sizeof(T) == 2>(as_float<T>(kept[i]), p.activation);
+                    float z = as_float<T>(dy[u][i]);
+                    if constexpr (kSlope) {
+                        z *= act_slope<sizeof(T) == 2>(as_float<T>(kept[u][i]), ACT);
+                        dy[u][i] = rounded<T>(z);
+                    }
                     sum[i] += z;
-                    dy[i] = rounded<T>(z);
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) sum[i] += as_float<T>(dy[i]);
-            }
-            if (p.dz != nullptr) {
-                T* dz = static_cast<T*>(p.dz) + r * p.dz_stride + c;
-                if constexpr (V > 1)
-                    *reinterpret_cast<uint4*>(dz) = *reinterpret_cast<uint4*>(dy);
-                else
-                    *dz = dy[0];
+                if (p.dz != nullptr) {
+                    if constexpr (V > 1)
+                        *reinterpret_cast<uint4*>(dzp + row * p.dz_stride) = *reinterpret_cast<uint4*>(dy[u]);
+                    else
+                        dzp[row * p.dz_stride] = dy[u][0];
+                }
             }
         }
     }
@@ -353,12 +366,11 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(Slope p) {
 #pragma unroll
     for (int i = 0; i < V; ++i) sums[warp][lane * V + i] = sum[i];
     __syncthreads();
-    for (int i = threadIdx.x; i < 32 * V; i += 256) {
-        const int64_t col = (int64_t)blockIdx.x * 32 * V + i;
+    for (int i = threadIdx.x; i < 32 * V * across; i += 256) {
+        const int64_t col = first + i;
         if (col >= p.n) break;
         float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) v += sums[w][i];
+        for (int w = 0; w < step; ++w) v += sums[w * across + i / (32 * V)][i % (32 * V)];
         p.sums[(int64_t)blockIdx.y * p.n + col] = v;
     }
 }
@@ -385,21 +397,42 @@ __global__ void __launch_bounds__(256) linear_bias_kernel(const float* sums, int
 }
 
 struct SlopePlan {
-    int vec, slabs;
+    int vec, slabs, across;
     int64_t slab, col_blocks;
 };
 template <typename T>
 SlopePlan slope_plan(int64_t m, int64_t n, bool vec) {
     SlopePlan p{};
     p.vec = vec ? kVec<T> : 1;
-    p.col_blocks = (n + 32 * p.vec - 1) / (32 * p.vec);
-    // Slabs of 32 rows or more, until there are eight blocks an SM.
-    int64_t slabs = (8 * kSmCount + p.col_blocks - 1) / p.col_blocks;
-    if (slabs > (m + 31) / 32) slabs = (m + 31) / 32;
+    p.across = 1;
+    while (p.across < 8 && (int64_t)p.across * 32 * p.vec < n) p.across *= 2;
+    p.col_blocks = (n + 32 * p.vec * p.across - 1) / (32 * p.vec * p.across);
+    // One round of the three blocks that an SM holds, in slabs of 16 rows or more.
+    int64_t slabs = 3 * kSmCount / p.col_blocks;
+    if (slabs > (m + 15) / 16) slabs = (m + 15) / 16;
     if (slabs < 1) slabs = 1;
     p.slab = (m + slabs - 1) / slabs;
     p.slabs = (int)((m + p.slab - 1) / p.slab);
     return p;
+}
+
+template <typename T, int ACT>
+void launch_slope(const Slope& a, dim3 grid, const SlopePlan& plan, cudaStream_t s) {
+    if (plan.vec > 1)
+        linear_slope_kernel<T, kVec<T>, ACT><<<grid, 256, 0, s>>>(a, plan.across);
+    else
+        linear_slope_kernel<T, 1, ACT><<<grid, 256, 0, s>>>(a, plan.across);
+}
+template <typename T>
+int launch_slope(const Slope& a, dim3 grid, const SlopePlan& plan, cudaStream_t s) {
+    switch (a.activation) {
+        case GK_ACT_RELU: launch_slope<T, GK_ACT_RELU>(a, grid, plan, s); break;
+        case GK_ACT_TANH: launch_slope<T, GK_ACT_TANH>(a, grid, plan, s); break;
+        case GK_ACT_GELU: launch_slope<T, GK_ACT_GELU>(a, grid, plan, s); break;
+        case GK_ACT_SILU: launch_slope<T, GK_ACT_SILU>(a, grid, plan, s); break;
+        default: launch_slope<T, GK_ACT_NONE>(a, grid, plan, s); break;
+    }
+    return launch_status();
 }
 
 // Rows of a 16-bit matrix to rows that start on 16 bytes, as TMA needs them.
@@ -558,11 +591,7 @@ int backward(const gk_linear_grad_t& p, void* workspace, uint32_t* status, cudaS
                 b.forms_dz ? const_cast<void*>(b.dz.p) : nullptr, b.sums, p.dy_stride, b.dz.ld, p.m, p.n,
                 b.slope.slab, p.activation};
         const dim3 grid((unsigned)b.slope.col_blocks, (unsigned)b.slope.slabs);
-        if (b.slope.vec > 1)
-            linear_slope_kernel<T, kVec<T>><<<grid, 256, 0, s>>>(a);
-        else
-            linear_slope_kernel<T, 1><<<grid, 256, 0, s>>>(a);
-        if ((e = launch_status()) != 0) return e;
+        if ((e = launch_slope<T>(a, grid, b.slope, s)) != 0) return e;
         if (p.db != nullptr) {
             linear_bias_kernel<T><<<(unsigned)((p.n + 31) / 32), 256, 0, s>>>(b.sums, p.n, b.slope.slabs,
                                                                                  static_cast<T*>(p.db));
