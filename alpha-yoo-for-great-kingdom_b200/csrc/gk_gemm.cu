@@ -41,27 +41,94 @@ struct Epilogue {
     int aligned;  // every row of out, residual and pre, and the bias, start on 16 bytes
 };
 
+// Issue is warp-wide: every lane of a converged warp runs the loops, so that
+// addresses and descriptors stay on the uniform datapath, and elect.sync lets
+// one lane (always the same) issue. A single thread in a branch of its own took
+// about 750 cycles for a stage, half as long again as its MMAs.
+template <bool PAIR>  // PAIR: the bytes are counted by a barrier of the pair's even CTA
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    if (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred e;\n\t"
+            "elect.sync _|e, 0xffffffff;\n\t"
+            "@e cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+            "[%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred e;\n\t"
+            "elect.sync _|e, 0xffffffff;\n\t"
+            "@e cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+            "[%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+}
+__device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-            dst),
-        "l"(map), "r"(x), "r"(y), "r"(bar)
+        "{\n\t.reg .pred e;\n\t.reg .b64 st;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar),
+        "r"(bytes)
         : "memory");
 }
 
 // Descriptor of a 128-byte-swizzled operand whose panels start on 1024 bytes.
 // k contiguous: rows in groups of 8, 1024 bytes apart. m or n contiguous: k in
 // groups of 8 rows, 1024 bytes apart, and panels of 64 m or n, 8192 apart.
-__device__ __forceinline__ uint64_t swizzled_desc(uint32_t addr, int across) {
-    uint64_t d = (uint64_t)((addr & 0x3FFFFu) >> 4);
-    d |= (uint64_t)(across ? 8192 >> 4 : 1) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
+// The low word holds the address and the panel step, the high word is the same for all.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, int across) {
+    return ((addr & 0x3FFFFu) >> 4) | ((across ? 8192u >> 4 : 1u) << 16);
 }
 // Address step of 16 k elements, in 16-byte units.
 __device__ __forceinline__ uint32_t k_step(int across) { return across ? 16 * 128 / 16 : 32 / 16; }
+
+// The four MMAs of a stage (64 k) and the commit that frees the stage.
+template <bool PAIR>
+__device__ __forceinline__ void mma_stage(uint32_t acc, uint32_t a, uint32_t b, uint32_t step_a, uint32_t step_b,
+                                          uint32_t idesc, uint32_t accumulate, uint32_t bar) {
+#define GK_MMA_STAGE(GROUP, COMMIT)                                                          \
+    asm volatile(                                                                            \
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 ad, bd;\n\t.reg .b32 al, bl;\n\t"                  \
+        "setp.ne.b32 p, %6, 0;\n\t"                                                           \
+        "elect.sync _|e, 0xffffffff;\n\t"                                                     \
+        "mov.b64 ad, {%1, %8};\n\tmov.b64 bd, {%2, %8};\n\t"                                   \
+        "@e tcgen05.mma." GROUP ".kind::f16 [%0], ad, bd, %5, p;\n\t"                          \
+        "add.u32 al, %1, %3;\n\tadd.u32 bl, %2, %4;\n\t"                                       \
+        "mov.b64 ad, {al, %8};\n\tmov.b64 bd, {bl, %8};\n\t"                                   \
+        "@e tcgen05.mma." GROUP ".kind::f16 [%0], ad, bd, %5, 1;\n\t"                          \
+        "add.u32 al, al, %3;\n\tadd.u32 bl, bl, %4;\n\t"                                       \
+        "mov.b64 ad, {al, %8};\n\tmov.b64 bd, {bl, %8};\n\t"                                   \
+        "@e tcgen05.mma." GROUP ".kind::f16 [%0], ad, bd, %5, 1;\n\t"                          \
+        "add.u32 al, al, %3;\n\tadd.u32 bl, bl, %4;\n\t"                                       \
+        "mov.b64 ad, {al, %8};\n\tmov.b64 bd, {bl, %8};\n\t"                                   \
+        "@e tcgen05.mma." GROUP ".kind::f16 [%0], ad, bd, %5, 1;\n\t"                          \
+        "@e " COMMIT "\n\t}" ::"r"(acc),                                                       \
+        "r"(a), "r"(b), "r"(step_a), "r"(step_b), "r"(idesc), "r"(accumulate), "r"(bar), "r"(kDescHigh), \
+        "h"((uint16_t)3)                                                                      \
+        : "memory")
+    if (PAIR)
+        GK_MMA_STAGE("cta_group::2",
+                     "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%7], %9;");
+    else
+        GK_MMA_STAGE("cta_group::1", "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%7];");
+#undef GK_MMA_STAGE
+}
+// Arrives once the MMAs issued so far complete; PAIR: on the barrier at this offset in both CTAs.
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar) {
+    if (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred e;\n\t"
+            "elect.sync _|e, 0xffffffff;\n\t"
+            "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(
+                bar),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        mma_commit_warp(bar);
+}
 
 __host__ __device__ constexpr uint32_t idesc16(int m, int n, int bf16, int a_across, int b_across) {
     return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)a_across << 15) |
@@ -69,15 +136,19 @@ __host__ __device__ constexpr uint32_t idesc16(int m, int n, int bf16, int a_acr
 }
 
 // Load an operand's ROWS x 64 stage: (mn, k) is its first element.
-template <int ROWS>
+template <int ROWS, bool PAIR>
 __device__ __forceinline__ void load_stage(uint32_t dst, const CUtensorMap* map, int across, int mn, int k,
                                            uint32_t bar) {
     if (across) {
 #pragma unroll
-        for (int p = 0; p < ROWS / 64; ++p) tma_load(dst + p * 8192, map, mn + 64 * p, k, bar);
+        for (int p = 0; p < ROWS / 64; ++p) tma_load<PAIR>(dst + p * 8192, map, mn + 64 * p, k, bar);
     } else {
-        tma_load(dst, map, k, mn, bar);
+        tma_load<PAIR>(dst, map, k, mn, bar);
     }
+}
+// A wait of the whole warp with one verdict.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint32_t* status) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, status));
 }
 
 // ------------------------------------------------------------------ split
@@ -129,45 +200,34 @@ __global__ void __launch_bounds__(kSplitThreads) gemm_split_kernel(const __grid_
     const uint32_t tmem = tmem_slot;
 
     if (warp == 0) {
-        if (lane == 0) {
-            bool ok = true;
-            int issued = kb0;
-            for (int kb = kb0; kb < kb1; ++kb) {
-                const int i = kb - kb0, s = i % S::kStages, turn = i / S::kStages;
-                if (turn > 0 && !mbar_wait(smem_u32(&empty[s]), (turn - 1) & 1, status)) {
-                    ok = false;
-                    break;
-                }
-                const uint32_t bar = smem_u32(&full[s]), at = stages + s * S::kStage;
-                mbar_expect_tx(bar, S::kStage);
-                load_stage<128>(at, &ta, a_across, m0, kb * kBK, bar);
-                load_stage<BN>(at + S::kA, &tb, b_across, n0, kb * kBK, bar);
-                issued = kb + 1;
-            }
-            // After a wait that gave up: the copies in flight land before the block may end.
-            if (!ok)
-                for (int kb = max(kb0, issued - S::kStages); kb < issued; ++kb) {
-                    const int i = kb - kb0;
-                    mbar_wait(smem_u32(&full[i % S::kStages]), (i / S::kStages) & 1, status);
-                }
+        bool ok = true;
+        int s = 0, turn = 0;
+        for (int kb = kb0; kb < kb1 && ok; ++kb) {
+            ok = turn == 0 || warp_wait(smem_u32(&empty[s]), (turn - 1) & 1, status);
+            if (!ok) break;
+            const uint32_t bar = smem_u32(&full[s]), at = stages + s * S::kStage;
+            expect_tx(bar, S::kStage);
+            load_stage<128, false>(at, &ta, a_across, m0, kb * kBK, bar);
+            load_stage<BN, false>(at + S::kA, &tb, b_across, n0, kb * kBK, bar);
+            if (++s == S::kStages) s = 0, ++turn;
         }
+        // After a wait that gave up: the copies in flight land before the block may end.
+        if (!ok)
+            for (int i = max(0, turn * S::kStages + s - S::kStages); i < turn * S::kStages + s; ++i)
+                mbar_wait(smem_u32(&full[i % S::kStages]), (i / S::kStages) & 1, status);
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = idesc16(128, BN, ep.bf16, a_across, b_across);
-            const uint32_t step_a = k_step(a_across), step_b = k_step(b_across);
-            for (int kb = kb0; kb < kb1; ++kb) {
-                const int i = kb - kb0, s = i % S::kStages, turn = i / S::kStages;
-                if (!mbar_wait(smem_u32(&full[s]), turn & 1, status)) break;
-                tc_fence_after();
-                const uint64_t a = swizzled_desc(stages + s * S::kStage, a_across);
-                const uint64_t b = swizzled_desc(stages + s * S::kStage + S::kA, b_across);
-#pragma unroll
-                for (int j = 0; j < kBK / 16; ++j)
-                    mma_bf16(tmem, a + j * step_a, b + j * step_b, idesc, (i > 0 || j > 0) ? 1u : 0u);
-                mma_commit(smem_u32(&empty[s]));
-            }
-            mma_commit(smem_u32(&done));
+        const uint32_t idesc = idesc16(128, BN, ep.bf16, a_across, b_across);
+        const uint32_t step_a = k_step(a_across), step_b = k_step(b_across);
+        const uint32_t a0 = desc_low(stages, a_across), b0 = desc_low(stages + S::kA, b_across);
+        int s = 0, parity = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            if (!warp_wait(smem_u32(&full[s]), parity, status)) break;
+            tc_fence_after();
+            mma_stage<false>(tmem, a0 + s * (S::kStage >> 4), b0 + s * (S::kStage >> 4), step_a, step_b, idesc,
+                             kb > kb0 ? 1u : 0u, smem_u32(&empty[s]));
+            if (++s == S::kStages) s = 0, parity ^= 1;
         }
+        commit<false>(smem_u32(&done));
     }
     __syncwarp();
     // Everyone waits for the accumulator: the parts overwrite the stages.
@@ -270,37 +330,11 @@ __device__ __forceinline__ uint32_t cluster_address(uint32_t local, uint32_t ran
 __device__ __forceinline__ void arrive_at(uint32_t remote) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
 }
-// A load whose bytes are counted by a barrier of the pair's even CTA.
-__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+__device__ __forceinline__ void mma_commit_drain(uint32_t bar) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
-        "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(bar)
-        : "memory");
-}
-template <int ROWS>
-__device__ __forceinline__ void load_stage_pair(uint32_t dst, const CUtensorMap* map, int across, int mn, int k,
-                                                uint32_t bar) {
-    if (across) {
-#pragma unroll
-        for (int p = 0; p < ROWS / 64; ++p) tma_load_pair(dst + p * 8192, map, mn + 64 * p, k, bar);
-    } else {
-        tma_load_pair(dst, map, k, mn, bar);
-    }
-}
-__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// Arrives on the barrier at this offset in both CTAs once the MMAs issued so far complete.
-__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-        "h"((uint16_t)3)
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
         : "memory");
 }
 
@@ -447,64 +481,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const uint32_t tmem = tmem_slot;
 
     if (warp == 0) {
-        if (lane == 0) {
-            int it = 0;
-            bool ok = true;
-            for (int t = pair; t < tiles && ok; t += pairs) {
-                int tm, tn;
-                tile_at(t, tiles_m, tiles_n, tm, tn);
-                const int m0 = tm * 256 + rank * 128, n0 = tn * BN + rank * (BN / 2);
-                for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-                    const int s = it % P::kStages, turn = it / P::kStages;
-                    if (turn > 0 && !mbar_wait(smem_u32(&empty[s]), (turn - 1) & 1, status)) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t at = stages + s * P::kStage, bar = cluster_address(smem_u32(&full[s]), 0);
-                    if (rank == 0) mbar_expect_tx(smem_u32(&full[s]), 2 * P::kStage);
-                    load_stage_pair<128>(at, &ta, a_across, m0, kb * kBK, bar);
-                    load_stage_pair<BN / 2>(at + P::kA, &tb, b_across, n0, kb * kBK, bar);
-                }
+        int s = 0, turn = 0;
+        bool ok = true;
+        const uint32_t full0 = cluster_address(smem_u32(full), 0);
+        for (int t = pair; t < tiles && ok; t += pairs) {
+            int tm, tn;
+            tile_at(t, tiles_m, tiles_n, tm, tn);
+            const int m0 = tm * 256 + rank * 128, n0 = tn * BN + rank * (BN / 2);
+            for (int kb = 0; kb < k_blocks; ++kb) {
+                ok = turn == 0 || warp_wait(smem_u32(&empty[s]), (turn - 1) & 1, status);
+                if (!ok) break;
+                const uint32_t at = stages + s * P::kStage, bar = full0 + s * 8;
+                if (rank == 0) expect_tx(smem_u32(&full[s]), 2 * P::kStage);
+                load_stage<128, true>(at, &ta, a_across, m0, kb * kBK, bar);
+                load_stage<BN / 2, true>(at + P::kA, &tb, b_across, n0, kb * kBK, bar);
+                if (++s == P::kStages) s = 0, ++turn;
             }
-            // After a wait that gave up: the pair's copies in flight land before the blocks may end.
-            if (!ok && rank == 0)
-                for (int i = max(0, it - P::kStages); i < it; ++i)
-                    mbar_wait(smem_u32(&full[i % P::kStages]), (i / P::kStages) & 1, status);
         }
+        // After a wait that gave up: the pair's copies in flight land before the blocks may end.
+        if (!ok && rank == 0)
+            for (int i = max(0, turn * P::kStages + s - P::kStages); i < turn * P::kStages + s; ++i)
+                mbar_wait(smem_u32(&full[i % P::kStages]), (i / P::kStages) & 1, status);
     } else if (warp == 1 && rank == 0) {
-        if (lane == 0) {
-            const uint32_t idesc = idesc16(256, BN, ep.bf16, a_across, b_across);
-            const uint32_t step_a = k_step(a_across), step_b = k_step(b_across);
-            int it = 0, n = 0;
-            bool ok = true;
-            for (int t = pair; t < tiles && ok; t += pairs, ++n) {
-                const int a = n & 1, use = n >> 1;
-                if (use > 0 && !mbar_wait(smem_u32(&acc_empty[a]), (use - 1) & 1, status)) {
-                    ok = false;
-                    break;
-                }
+        const uint32_t idesc = idesc16(256, BN, ep.bf16, a_across, b_across);
+        const uint32_t step_a = k_step(a_across), step_b = k_step(b_across);
+        const uint32_t a0 = desc_low(stages, a_across), b0 = desc_low(stages + P::kA, b_across);
+        int s = 0, parity = 0, n = 0;
+        bool ok = true;
+        for (int t = pair; t < tiles && ok; t += pairs, ++n) {
+            const int a = n & 1, use = n >> 1;
+            ok = use == 0 || warp_wait(smem_u32(&acc_empty[a]), (use - 1) & 1, status);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t acc = tmem + a * BN;
+            for (int kb = 0; kb < k_blocks; ++kb) {
+                ok = warp_wait(smem_u32(&full[s]), parity, status);
+                if (!ok) break;
                 tc_fence_after();
-                const uint32_t acc = tmem + a * BN;
-                for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-                    const int s = it % P::kStages;
-                    if (!mbar_wait(smem_u32(&full[s]), (it / P::kStages) & 1, status)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint64_t da = swizzled_desc(stages + s * P::kStage, a_across);
-                    const uint64_t db = swizzled_desc(stages + s * P::kStage + P::kA, b_across);
-#pragma unroll
-                    for (int j = 0; j < kBK / 16; ++j)
-                        mma_pair(acc, da + j * step_a, db + j * step_b, idesc, (kb > 0 || j > 0) ? 1u : 0u);
-                    mma_commit_pair(smem_u32(&empty[s]));
-                }
-                if (ok) mma_commit_pair(smem_u32(&acc_full[a]));
+                mma_stage<true>(acc, a0 + s * (P::kStage >> 4), b0 + s * (P::kStage >> 4), step_a, step_b, idesc,
+                                kb > 0 ? 1u : 0u, smem_u32(&empty[s]));
+                if (++s == P::kStages) s = 0, parity ^= 1;
             }
-            if (!ok) {  // the MMAs in flight end before TMEM is freed
-                mma_commit_pair(smem_u32(&drain));
-                mbar_wait(smem_u32(&drain), 0, status);
-            }
+            if (ok) commit<true>(smem_u32(&acc_full[a]));
+        }
+        if (!ok) {  // the MMAs in flight end before TMEM is freed
+            mma_commit_drain(smem_u32(&drain));
+            mbar_wait(smem_u32(&drain), 0, status);
         }
     } else if (warp >= 4) {
         const int quadrant = warp & 3, half = (warp - 4) >> 2;
