@@ -42,34 +42,45 @@ struct Epilogue {
 };
 
 // Issue is warp-wide: every lane of a converged warp runs the loops, so that
-// addresses and descriptors stay on the uniform datapath, and elect.sync lets
-// one lane (always the same) issue. A single thread in a branch of its own took
-// about 750 cycles for a stage, half as long again as its MMAs.
+// addresses and descriptors stay on the uniform datapath, and a predicate from
+// one elect.sync lets one lane issue. A single thread in a branch of its own
+// took about 750 cycles for a stage, half as long again as its MMAs; an
+// elect.sync for each instruction about 480.
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, e;\n\t}"
+        : "=r"(r));
+    return r;
+}
 template <bool PAIR>  // PAIR: the bytes are counted by a barrier of the pair's even CTA
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+__device__ __forceinline__ void tma_load(uint32_t one, uint32_t dst, const CUtensorMap* map, int x, int y,
+                                         uint32_t bar) {
     if (PAIR)
         asm volatile(
             "{\n\t.reg .pred e;\n\t"
-            "elect.sync _|e, 0xffffffff;\n\t"
+            "setp.ne.b32 e, %5, 0;\n\t"
             "@e cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
             "[%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(dst),
-            "l"(map), "r"(x), "r"(y), "r"(bar)
+            "l"(map), "r"(x), "r"(y), "r"(bar), "r"(one)
             : "memory");
     else
         asm volatile(
             "{\n\t.reg .pred e;\n\t"
-            "elect.sync _|e, 0xffffffff;\n\t"
+            "setp.ne.b32 e, %5, 0;\n\t"
             "@e cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
             "[%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(dst),
-            "l"(map), "r"(x), "r"(y), "r"(bar)
+            "l"(map), "r"(x), "r"(y), "r"(bar), "r"(one)
             : "memory");
 }
-__device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
+__device__ __forceinline__ void expect_tx(uint32_t one, uint32_t bar, uint32_t bytes) {
     asm volatile(
         "{\n\t.reg .pred e;\n\t.reg .b64 st;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 e, %2, 0;\n\t"
         "@e mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar),
-        "r"(bytes)
+        "r"(bytes), "r"(one)
         : "memory");
 }
 
@@ -86,13 +97,13 @@ __device__ __forceinline__ uint32_t k_step(int across) { return across ? 16 * 12
 
 // The four MMAs of a stage (64 k) and the commit that frees the stage.
 template <bool PAIR>
-__device__ __forceinline__ void mma_stage(uint32_t acc, uint32_t a, uint32_t b, uint32_t step_a, uint32_t step_b,
+__device__ __forceinline__ void mma_stage(uint32_t one, uint32_t acc, uint32_t a, uint32_t b, uint32_t step_a, uint32_t step_b,
                                           uint32_t idesc, uint32_t accumulate, uint32_t bar) {
 #define GK_MMA_STAGE(GROUP, COMMIT)                                                          \
     asm volatile(                                                                            \
         "{\n\t.reg .pred p, e;\n\t.reg .b64 ad, bd;\n\t.reg .b32 al, bl;\n\t"                  \
         "setp.ne.b32 p, %6, 0;\n\t"                                                           \
-        "elect.sync _|e, 0xffffffff;\n\t"                                                     \
+        "setp.ne.b32 e, %10, 0;\n\t"                                                          \
         "mov.b64 ad, {%1, %8};\n\tmov.b64 bd, {%2, %8};\n\t"                                   \
         "@e tcgen05.mma." GROUP ".kind::f16 [%0], ad, bd, %5, p;\n\t"                          \
         "add.u32 al, %1, %3;\n\tadd.u32 bl, %2, %4;\n\t"                                       \
@@ -106,7 +117,7 @@ __device__ __forceinline__ void mma_stage(uint32_t acc, uint32_t a, uint32_t b, 
         "@e tcgen05.mma." GROUP ".kind::f16 [%0], ad, bd, %5, 1;\n\t"                          \
         "@e " COMMIT "\n\t}" ::"r"(acc),                                                       \
         "r"(a), "r"(b), "r"(step_a), "r"(step_b), "r"(idesc), "r"(accumulate), "r"(bar), "r"(kDescHigh), \
-        "h"((uint16_t)3)                                                                      \
+        "h"((uint16_t)3), "r"(one)                                                            \
         : "memory")
     if (PAIR)
         GK_MMA_STAGE("cta_group::2",
@@ -137,17 +148,32 @@ __host__ __device__ constexpr uint32_t idesc16(int m, int n, int bf16, int a_acr
 
 // Load an operand's ROWS x 64 stage: (mn, k) is its first element.
 template <int ROWS, bool PAIR>
-__device__ __forceinline__ void load_stage(uint32_t dst, const CUtensorMap* map, int across, int mn, int k,
+__device__ __forceinline__ void load_stage(uint32_t one, uint32_t dst, const CUtensorMap* map, int across, int mn, int k,
                                            uint32_t bar) {
     if (across) {
 #pragma unroll
-        for (int p = 0; p < ROWS / 64; ++p) tma_load<PAIR>(dst + p * 8192, map, mn + 64 * p, k, bar);
+        for (int p = 0; p < ROWS / 64; ++p) tma_load<PAIR>(one, dst + p * 8192, map, mn + 64 * p, k, bar);
     } else {
-        tma_load<PAIR>(dst, map, k, mn, bar);
+        tma_load<PAIR>(one, dst, map, k, mn, bar);
     }
 }
-// A wait of the whole warp with one verdict.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint32_t* status) {
+// Whether the phase is over, without waiting (try_wait may sleep for microseconds).
+__device__ __forceinline__ bool mbar_look(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+// A wait of the whole warp with one verdict. `ready`: an earlier look at the
+// barrier (a look takes some 150 cycles, so each is taken a stage ahead, under
+// the issue of the stage before).
+__device__ __forceinline__ bool warp_wait(bool ready, uint32_t bar, uint32_t parity, uint32_t* status) {
+    if (__all_sync(0xffffffffu, ready)) return true;
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, status));
 }
 
@@ -200,16 +226,19 @@ __global__ void __launch_bounds__(kSplitThreads) gemm_split_kernel(const __grid_
     const uint32_t tmem = tmem_slot;
 
     if (warp == 0) {
-        bool ok = true;
+        bool ok = true, ready = true;  // the first round finds every stage empty
         int s = 0, turn = 0;
+        const uint32_t one = elect_one();
         for (int kb = kb0; kb < kb1 && ok; ++kb) {
-            ok = turn == 0 || warp_wait(smem_u32(&empty[s]), (turn - 1) & 1, status);
+            ok = warp_wait(ready, smem_u32(&empty[s]), (turn - 1) & 1, status);
             if (!ok) break;
+            const int next = s + 1 == S::kStages ? 0 : s + 1, next_turn = next == 0 ? turn + 1 : turn;
+            ready = next_turn == 0 || mbar_look(smem_u32(&empty[next]), (next_turn - 1) & 1);
             const uint32_t bar = smem_u32(&full[s]), at = stages + s * S::kStage;
-            expect_tx(bar, S::kStage);
-            load_stage<128, false>(at, &ta, a_across, m0, kb * kBK, bar);
-            load_stage<BN, false>(at + S::kA, &tb, b_across, n0, kb * kBK, bar);
-            if (++s == S::kStages) s = 0, ++turn;
+            expect_tx(one, bar, S::kStage);
+            load_stage<128, false>(one, at, &ta, a_across, m0, kb * kBK, bar);
+            load_stage<BN, false>(one, at + S::kA, &tb, b_across, n0, kb * kBK, bar);
+            s = next, turn = next_turn;
         }
         // After a wait that gave up: the copies in flight land before the block may end.
         if (!ok)
@@ -220,12 +249,16 @@ __global__ void __launch_bounds__(kSplitThreads) gemm_split_kernel(const __grid_
         const uint32_t step_a = k_step(a_across), step_b = k_step(b_across);
         const uint32_t a0 = desc_low(stages, a_across), b0 = desc_low(stages + S::kA, b_across);
         int s = 0, parity = 0;
+        bool ready = false;
+        const uint32_t one = elect_one();
         for (int kb = kb0; kb < kb1; ++kb) {
-            if (!warp_wait(smem_u32(&full[s]), parity, status)) break;
+            if (!warp_wait(ready, smem_u32(&full[s]), parity, status)) break;
+            const int next = s + 1 == S::kStages ? 0 : s + 1, next_parity = next == 0 ? parity ^ 1 : parity;
+            ready = mbar_look(smem_u32(&full[next]), next_parity);
             tc_fence_after();
-            mma_stage<false>(tmem, a0 + s * (S::kStage >> 4), b0 + s * (S::kStage >> 4), step_a, step_b, idesc,
+            mma_stage<false>(one, tmem, a0 + s * (S::kStage >> 4), b0 + s * (S::kStage >> 4), step_a, step_b, idesc,
                              kb > kb0 ? 1u : 0u, smem_u32(&empty[s]));
-            if (++s == S::kStages) s = 0, parity ^= 1;
+            s = next, parity = next_parity;
         }
         commit<false>(smem_u32(&done));
     }
@@ -482,20 +515,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
     if (warp == 0) {
         int s = 0, turn = 0;
-        bool ok = true;
-        const uint32_t full0 = cluster_address(smem_u32(full), 0);
+        bool ok = true, ready = true;  // the first round finds every stage empty
+        const uint32_t full0 = cluster_address(smem_u32(full), 0), one = elect_one();
         for (int t = pair; t < tiles && ok; t += pairs) {
             int tm, tn;
             tile_at(t, tiles_m, tiles_n, tm, tn);
             const int m0 = tm * 256 + rank * 128, n0 = tn * BN + rank * (BN / 2);
             for (int kb = 0; kb < k_blocks; ++kb) {
-                ok = turn == 0 || warp_wait(smem_u32(&empty[s]), (turn - 1) & 1, status);
+                ok = warp_wait(ready, smem_u32(&empty[s]), (turn - 1) & 1, status);
                 if (!ok) break;
+                const int next = s + 1 == P::kStages ? 0 : s + 1, next_turn = next == 0 ? turn + 1 : turn;
+                ready = next_turn == 0 || mbar_look(smem_u32(&empty[next]), (next_turn - 1) & 1);
                 const uint32_t at = stages + s * P::kStage, bar = full0 + s * 8;
-                if (rank == 0) expect_tx(smem_u32(&full[s]), 2 * P::kStage);
-                load_stage<128, true>(at, &ta, a_across, m0, kb * kBK, bar);
-                load_stage<BN / 2, true>(at + P::kA, &tb, b_across, n0, kb * kBK, bar);
-                if (++s == P::kStages) s = 0, ++turn;
+                if (rank == 0) expect_tx(one, smem_u32(&full[s]), 2 * P::kStage);
+                load_stage<128, true>(one, at, &ta, a_across, m0, kb * kBK, bar);
+                load_stage<BN / 2, true>(one, at + P::kA, &tb, b_across, n0, kb * kBK, bar);
+                s = next, turn = next_turn;
             }
         }
         // After a wait that gave up: the pair's copies in flight land before the blocks may end.
@@ -507,20 +542,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const uint32_t step_a = k_step(a_across), step_b = k_step(b_across);
         const uint32_t a0 = desc_low(stages, a_across), b0 = desc_low(stages + P::kA, b_across);
         int s = 0, parity = 0, n = 0;
-        bool ok = true;
+        bool ok = true, ready = false;
+        const uint32_t one = elect_one();
         for (int t = pair; t < tiles && ok; t += pairs, ++n) {
             const int a = n & 1, use = n >> 1;
-            ok = use == 0 || warp_wait(smem_u32(&acc_empty[a]), (use - 1) & 1, status);
+            ok = warp_wait(use == 0, smem_u32(&acc_empty[a]), (use - 1) & 1, status);
             if (!ok) break;
             tc_fence_after();
             const uint32_t acc = tmem + a * BN;
             for (int kb = 0; kb < k_blocks; ++kb) {
-                ok = warp_wait(smem_u32(&full[s]), parity, status);
+                ok = warp_wait(ready, smem_u32(&full[s]), parity, status);
                 if (!ok) break;
+                const int next = s + 1 == P::kStages ? 0 : s + 1, next_parity = next == 0 ? parity ^ 1 : parity;
+                ready = mbar_look(smem_u32(&full[next]), next_parity);
                 tc_fence_after();
-                mma_stage<true>(acc, a0 + s * (P::kStage >> 4), b0 + s * (P::kStage >> 4), step_a, step_b, idesc,
+                mma_stage<true>(one, acc, a0 + s * (P::kStage >> 4), b0 + s * (P::kStage >> 4), step_a, step_b, idesc,
                                 kb > 0 ? 1u : 0u, smem_u32(&empty[s]));
-                if (++s == P::kStages) s = 0, parity ^= 1;
+                s = next, parity = next_parity;
             }
             if (ok) commit<true>(smem_u32(&acc_full[a]));
         }
