@@ -9,7 +9,6 @@ library is missing or a call fails, an exception is raised.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -17,17 +16,14 @@ from pathlib import Path
 import torch
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "libgk.so"
+TORCH_LIBRARY_PATH = Path(__file__).resolve().parent / "libgk_torch.so"
 
 c_void_p = ctypes.c_void_p
 c_int = ctypes.c_int
 c_int64 = ctypes.c_int64
 c_uint64 = ctypes.c_uint64
 c_double = ctypes.c_double
-c_float = ctypes.c_float
 c_size_t = ctypes.c_size_t
-
-
-TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # GK_FP32, GK_BF16, GK_FP16
 
 
 class PuctOptions(ctypes.Structure):
@@ -55,37 +51,7 @@ class NetStruct(ctypes.Structure):
                 ("norm", c_int), ("norm_w", c_void_p), ("norm_b", c_void_p), ("head_norm", c_void_p)]
 
 
-class PolicyLossStruct(ctypes.Structure):
-    _fields_ = [("logits", c_void_p), ("mask", c_void_p), ("target", c_void_p), ("actions", c_void_p),
-                ("old_log_probs", c_void_p), ("advantages", c_void_p), ("reference_log_probs", c_void_p),
-                ("denominator_ptr", c_void_p), ("rows", c_int64), ("cols", c_int64), ("logits_stride", c_int64),
-                ("mask_stride", c_int64), ("target_stride", c_int64), ("clip_low", c_float), ("clip_high", c_float),
-                ("kl_weight", c_float), ("target_weight", c_float), ("denominator", c_float), ("logits_type", c_int),
-                ("target_type", c_int), ("loss", c_void_p), ("log_probs", c_void_p), ("stats", c_void_p),
-                ("partials", c_void_p), ("grad", c_void_p)]
-
-
-class LinearStruct(ctypes.Structure):
-    _fields_ = [("x", c_void_p), ("w", c_void_p), ("bias", c_void_p), ("residual", c_void_p), ("y", c_void_p),
-                ("pre", c_void_p), ("m", c_int64), ("n", c_int64), ("k", c_int64), ("x_stride", c_int64),
-                ("w_stride", c_int64), ("residual_stride", c_int64), ("dtype", c_int), ("activation", c_int)]
-
-
-class LinearGradStruct(ctypes.Structure):
-    _fields_ = [("dy", c_void_p), ("kept", c_void_p), ("x", c_void_p), ("x_codes", c_void_p), ("x_scales", c_void_p),
-                ("w", c_void_p), ("dx", c_void_p), ("dw", c_void_p), ("db", c_void_p), ("dz", c_void_p),
-                ("m", c_int64), ("n", c_int64), ("k", c_int64), ("dy_stride", c_int64), ("x_stride", c_int64),
-                ("w_stride", c_int64), ("dtype", c_int), ("activation", c_int)]
-
-
 _SIGNATURES = {
-    "gk_linear_forward": [ctypes.POINTER(LinearStruct), c_void_p, c_void_p, c_void_p],
-    "gk_linear_backward": [ctypes.POINTER(LinearGradStruct), c_void_p, c_void_p, c_void_p],
-    "gk_pack": [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
-    "gk_unpack": [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int, c_void_p],
-    "gk_policy_loss_parts": [c_int64, c_int64],
-    "gk_policy_loss_forward": [ctypes.POINTER(PolicyLossStruct), c_void_p],
-    "gk_policy_loss_backward": [ctypes.POINTER(PolicyLossStruct), c_void_p, c_int, c_void_p],
     "gk_initial_records": [c_void_p, c_int64, c_int, c_void_p],
     "gk_initial_bits": [c_void_p, c_int64, c_int, c_void_p],
     "gk_play_records": [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p],
@@ -117,17 +83,18 @@ _SIZE_FUNCTIONS = {
     "gk_puct_workspace_bytes": [c_int64, c_int],
     "gk_net_weight_bytes": [c_int, c_int],
     "gk_net_headfeat_bytes": [c_int64],
-    "gk_linear_workspace_bytes": [ctypes.POINTER(LinearStruct)],
-    "gk_linear_grad_workspace_bytes": [ctypes.POINTER(LinearGradStruct)],
 }
 
 _lock = threading.Lock()
 _lib = None
+_operators = None
 
 
 def library():
     """Load libgk.so once; raise if it has not been built."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not LIBRARY_PATH.exists():
@@ -144,6 +111,21 @@ def library():
                 fn.restype = c_size_t
             _lib = lib
         return _lib
+
+
+def operators():
+    """The PyTorch operators of libgk_torch.so (csrc/gk_torch.cpp), loaded once."""
+    global _operators
+    if _operators is None:
+        library()
+        with _lock:
+            if _operators is None:
+                if not TORCH_LIBRARY_PATH.exists():
+                    raise RuntimeError(f"{TORCH_LIBRARY_PATH} is missing: build it with build_native.py "
+                                       "(the training-step operators have no fallback)")
+                torch.ops.load_library(str(TORCH_LIBRARY_PATH))
+                _operators = torch.ops.gk
+    return _operators
 
 
 def register(name: str, argtypes, restype=c_int):
@@ -168,22 +150,6 @@ def ptr(tensor: torch.Tensor | None):
 
 def stream_of(device: torch.device):
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
-
-def launch_stream(device: torch.device, tensors):
-    """The current stream of `device`; the tensors are marked as used on it, so
-    that memory allocated on another stream is not reused under the launch."""
-    stream = torch.cuda.current_stream(device)
-    for tensor in tensors:
-        tensor.record_stream(stream)
-    return c_void_p(stream.cuda_stream)
-
-
-def on_device(device: torch.device):
-    """A context in which `device` is current (nothing to do if it already is)."""
-    if torch.cuda.current_device() == device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
 
 
 def require_cuda(device) -> torch.device:

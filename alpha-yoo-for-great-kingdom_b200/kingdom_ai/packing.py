@@ -22,7 +22,7 @@ import torch
 
 from . import _native as native
 
-BLOCK = 32  # values that share a scale
+_PACKED_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 _active = threading.local()
 
 
@@ -30,11 +30,10 @@ class PackedActivation:
     """The 8-bit form of a tensor: ``codes`` (uint8, e4m3) and ``scales``
     (uint8, value 2^(byte - 127)), with the shape and dtype to unpack to."""
 
-    __slots__ = ("codes", "scales", "shape", "dtype", "rows", "cols")
+    __slots__ = ("codes", "scales", "shape", "dtype")
 
-    def __init__(self, codes, scales, shape, dtype, rows, cols):
+    def __init__(self, codes, scales, shape, dtype):
         self.codes, self.scales, self.shape, self.dtype = codes, scales, shape, dtype
-        self.rows, self.cols = rows, cols
 
     @property
     def nbytes(self) -> int:
@@ -43,28 +42,11 @@ class PackedActivation:
     def unpack(self, dtype=None) -> torch.Tensor:
         """The held values in the packed tensor's shape and its dtype (or in
         fp32, which holds them all), contiguous."""
-        if dtype not in (None, self.dtype, torch.float32):
+        if dtype is None:
+            dtype = self.dtype
+        elif dtype not in (self.dtype, torch.float32):
             raise ValueError(f"unpack gives {self.dtype} or torch.float32")
-        out = torch.empty(self.shape, dtype=dtype or self.dtype, device=self.codes.device)
-        if out.numel():
-            with native.on_device(out.device):
-                native.call("gk_unpack", native.ptr(self.codes), native.ptr(self.scales), self.rows, self.cols,
-                            native.ptr(out), self.cols, native.TYPES[out.dtype],
-                            native.launch_stream(out.device, (self.codes, self.scales)))
-        return out
-
-
-def pack_rows(x: torch.Tensor, rows: int, cols: int, stride: int, shape) -> PackedActivation:
-    """Pack [rows, cols] of x's memory, rows `stride` elements apart; a block never spans two rows."""
-    per_row = -(-cols // BLOCK)
-    # Codes and scales in one allocation; the codes start it, so they are aligned.
-    buffer = torch.empty(rows * (cols + per_row), dtype=torch.uint8, device=x.device)
-    codes, scales = buffer[:rows * cols], buffer[rows * cols:]
-    if rows and cols:
-        with native.on_device(x.device):
-            native.call("gk_pack", native.ptr(x), stride, native.TYPES[x.dtype], rows, cols, native.ptr(codes),
-                        native.ptr(scales), native.launch_stream(x.device, (x,)))
-    return PackedActivation(codes, scales, shape, x.dtype, rows, cols)
+        return native.operators().unpack.default(self.codes, self.scales, self.shape, dtype)
 
 
 def pack_activation(x: torch.Tensor) -> PackedActivation:
@@ -73,10 +55,8 @@ def pack_activation(x: torch.Tensor) -> PackedActivation:
     tensors are made contiguous first, and unpack as contiguous ones."""
     if not isinstance(x, torch.Tensor):
         raise TypeError("pack_activation packs a tensor")
-    if x.device.type != "cuda" or x.dtype not in native.TYPES:
-        raise ValueError("pack_activation packs CUDA tensors of float32, bfloat16 or float16")
-    x = x.detach().contiguous()
-    return pack_rows(x, 1, x.numel(), x.numel(), x.shape)
+    codes, scales = native.operators().pack.default(x)
+    return PackedActivation(codes, scales, x.shape, x.dtype)
 
 
 def _is_parameter(t: torch.Tensor) -> bool:
@@ -104,7 +84,7 @@ def packed_activations(min_elements: int = 1 << 16):
         raise ValueError("min_elements must be a positive integer")
 
     def pack(t):
-        if (t.device.type != "cuda" or t.dtype not in native.TYPES or t.numel() < min_elements
+        if (t.device.type != "cuda" or t.dtype not in _PACKED_TYPES or t.numel() < min_elements
                 or t.layout != torch.strided or _is_parameter(t)):
             return t
         return pack_activation(t)
@@ -121,10 +101,13 @@ def packed_activations(min_elements: int = 1 << 16):
             _active.depth = depth
 
 
+def packing_active() -> bool:
+    """Whether this thread is inside packed_activations."""
+    return getattr(_active, "depth", 0) > 0
+
+
 def keep_saved_tensors():
     """A context in which saved tensors are kept as they are inside packed_activations."""
-    if getattr(_active, "depth", 0) == 0:
-        return contextlib.nullcontext()
     return torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t)
 
 

@@ -44,15 +44,50 @@ def test_packed_activations_leaves_cpu_tensors_alone():
     assert torch.equal(x.grad, 1.5 * (x * 1.5).exp().detach())
 
 
+c_void_p, c_int64, c_int, c_float = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+
+
+class PolicyLossStruct(ctypes.Structure):
+    _fields_ = [("logits", c_void_p), ("mask", c_void_p), ("target", c_void_p), ("actions", c_void_p),
+                ("old_log_probs", c_void_p), ("advantages", c_void_p), ("reference_log_probs", c_void_p),
+                ("denominator_ptr", c_void_p), ("rows", c_int64), ("cols", c_int64), ("logits_stride", c_int64),
+                ("mask_stride", c_int64), ("target_stride", c_int64), ("clip_low", c_float), ("clip_high", c_float),
+                ("kl_weight", c_float), ("target_weight", c_float), ("denominator", c_float), ("logits_type", c_int),
+                ("target_type", c_int), ("loss", c_void_p), ("log_probs", c_void_p), ("stats", c_void_p),
+                ("partials", c_void_p), ("grad", c_void_p)]
+
+
+class LinearStruct(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("w", c_void_p), ("bias", c_void_p), ("residual", c_void_p), ("y", c_void_p),
+                ("pre", c_void_p), ("m", c_int64), ("n", c_int64), ("k", c_int64), ("x_stride", c_int64),
+                ("w_stride", c_int64), ("residual_stride", c_int64), ("dtype", c_int), ("activation", c_int)]
+
+
+class LinearGradStruct(ctypes.Structure):
+    _fields_ = [("dy", c_void_p), ("kept", c_void_p), ("x", c_void_p), ("x_codes", c_void_p), ("x_scales", c_void_p),
+                ("w", c_void_p), ("dx", c_void_p), ("dw", c_void_p), ("db", c_void_p), ("dz", c_void_p),
+                ("m", c_int64), ("n", c_int64), ("k", c_int64), ("dy_stride", c_int64), ("x_stride", c_int64),
+                ("w_stride", c_int64), ("dtype", c_int), ("activation", c_int)]
+
+
 def library():
     if not LIBRARY.exists():
         pytest.skip("libgk.so not built")
-    from kingdom_ai import _native
-    return _native.library()
+    lib = ctypes.CDLL(str(LIBRARY))
+    for name, result, arguments in (
+            ("gk_linear_forward", c_int, [c_void_p] * 4), ("gk_linear_backward", c_int, [c_void_p] * 4),
+            ("gk_linear_workspace_bytes", ctypes.c_size_t, [c_void_p]),
+            ("gk_policy_loss_parts", c_int, [c_int64, c_int64]),
+            ("gk_policy_loss_forward", c_int, [c_void_p] * 2),
+            ("gk_policy_loss_backward", c_int, [c_void_p, c_void_p, c_int, c_void_p]),
+            ("gk_pack", c_int, [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+            ("gk_unpack", c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int, c_void_p])):
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = result, arguments
+    return lib
 
 
 def linear_struct(**changes):
-    from kingdom_ai._native import LinearStruct
     p = LinearStruct()
     base = 1 << 20  # never read: the checks come first
     p.x, p.w, p.y = base, base, base
@@ -83,7 +118,6 @@ def test_linear_entry_refuses_missing_workspace_and_status():
 
 
 def test_linear_backward_entry_refuses():
-    from kingdom_ai._native import LinearGradStruct
     lib = library()
     status = ctypes.c_void_p(1 << 20)
 
@@ -103,7 +137,6 @@ def test_linear_backward_entry_refuses():
 
 
 def test_policy_loss_entry_refuses():
-    from kingdom_ai._native import PolicyLossStruct
     lib = library()
 
     def struct(**changes):
