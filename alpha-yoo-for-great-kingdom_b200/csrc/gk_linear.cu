@@ -138,7 +138,7 @@ int few_rows(FewRows p, cudaStream_t s) {
 struct Gemm32 {
     const float* a;
     const float* b;
-    int64_t a_row, a_k, b_row, b_k;  // strides of A[m, k] and B[n, k]; one of each pair is 1
+    int64_t a_ld, b_ld;  // elements between rows of A and B, or between their k where m or n is contiguous
     float* out;
     const float* bias;
     const float* residual;
@@ -148,103 +148,151 @@ struct Gemm32 {
     int activation;
 };
 
-// A tile of B x B outputs, 256 threads of (B/16)^2 outputs each, k in steps of
-// 16 through two shared-memory buffers with the next step in registers. With
-// few tiles a cluster of CTAs shares one along k and adds the parts up in rank
-// order through distributed shared memory.
+// A tile of B x B outputs, 8 x 8 to a thread, k in steps of 16 through two
+// shared-memory buffers with the next step's loads in registers. The products
+// are packed pairs (two fp32 multiply-adds an instruction, each rounded like
+// one of its own). With few tiles a cluster of CTAs shares one along k and adds
+// the parts up in rank order through distributed shared memory.
 constexpr int kStep = 16;
 template <int B>
-constexpr int kGemm32Smem = (B * (B + 4) > 4 * kStep * (B + 4) ? B * (B + 4) : 4 * kStep * (B + 4)) * 4;
+struct Tile32 {
+    static constexpr int kThreads = (B / 8) * (B / 8), kPitch = B + 4;
+    static constexpr int kSmem = (B * kPitch > 4 * kStep * kPitch ? B * kPitch : 4 * kStep * kPitch) * 4;
+    static constexpr int kQuads = B * kStep / 4 / kThreads;  // groups of four elements a thread loads of an operand
+};
 
-// One operand's B x 16 step: thread t takes elements (row, k) along whichever is contiguous.
-template <int B>
+// One operand's B x 16 step, four neighbours at a time along its contiguous
+// dimension: k (K) or the row. VEC: those four are one aligned 16-byte load.
+template <int B, bool K, bool VEC>
 struct Loader32 {
-    static constexpr int kEach = B * kStep / 256;
-    float v[kEach];
-    __device__ __forceinline__ static void place(int t, int i, bool k_contiguous, int& row, int& k) {
-        const int e = t + i * 256;
-        if (k_contiguous)
-            k = e % kStep, row = e / kStep;
+    using T = Tile32<B>;
+    float v[T::kQuads][4];
+    const float* at[T::kQuads];  // this thread's first element of each group, now
+    int64_t left[T::kQuads];     // K: rows left from it (1 or 0); else elements left of its four
+    int64_t step;
+    __device__ __forceinline__ static void place(int t, int i, int& row, int& k) {
+        const int q = t + i * T::kThreads;
+        if (K)
+            k = (q % (kStep / 4)) * 4, row = q / (kStep / 4);
         else
-            row = e % B, k = e / B;
+            row = (q % (B / 4)) * 4, k = q / (B / 4);
     }
-    __device__ __forceinline__ void fetch(const float* p, int64_t s_row, int64_t s_k, int64_t row0, int64_t rows,
-                                          int64_t k0, int64_t k_end, int t) {
+    __device__ __forceinline__ void start(const float* p, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int t) {
+        step = K ? kStep : kStep * ld;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
+        for (int i = 0; i < T::kQuads; ++i) {
             int row, k;
-            place(t, i, s_k == 1, row, k);
-            const bool in = row0 + row < rows && k0 + k < k_end;
-            v[i] = in ? __ldg(p + (row0 + row) * s_row + (k0 + k) * s_k) : 0.0f;
+            place(t, i, row, k);
+            left[i] = rows - (row0 + row);
+            at[i] = K ? p + (row0 + row) * ld + k0 + k : p + (k0 + k) * ld + row0 + row;
         }
     }
-    __device__ __forceinline__ void store(float (*tile)[B + 4], bool k_contiguous, int t) const {
+    // `k_left`: k elements left from the step's start.
+    __device__ __forceinline__ void fetch(int64_t k_left, int t) {
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
+        for (int i = 0; i < T::kQuads; ++i) {
             int row, k;
-            place(t, i, k_contiguous, row, k);
-            tile[k][row] = v[i];
+            place(t, i, row, k);
+            const int64_t count = K ? (left[i] > 0 ? k_left - k : 0) : (k < k_left ? left[i] : 0);
+            if (VEC && count >= 4) {
+                *reinterpret_cast<float4*>(v[i]) = __ldg(reinterpret_cast<const float4*>(at[i]));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[i][j] = j < count ? __ldg(at[i] + j) : 0.0f;
+            }
+            at[i] += step;
+        }
+    }
+    __device__ __forceinline__ void store(float (*tile)[T::kPitch], int t) const {
+#pragma unroll
+        for (int i = 0; i < T::kQuads; ++i) {
+            int row, k;
+            place(t, i, row, k);
+            if (K) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) tile[k + j][row] = v[i][j];
+            } else {
+                *reinterpret_cast<float4*>(&tile[k][row]) = *reinterpret_cast<const float4*>(v[i]);
+            }
         }
     }
 };
 
-template <int B>
-__global__ void __launch_bounds__(256) gemm32_kernel(Gemm32 g, int tiles_n) {
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void multiply_add(uint64_t& acc, uint64_t a, uint64_t b) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
+}
+
+template <int B, bool AK, bool BK, bool VEC>
+__global__ void __launch_bounds__(Tile32<B>::kThreads, B == 128 ? 2 : 6) gemm32_kernel(Gemm32 g, int tiles_n) {
     extern __shared__ float smem[];
-    constexpr int E = B / 16, kPitch = B + 4;
+    using T = Tile32<B>;
+    constexpr int kSide = B / 8, kPitch = T::kPitch;
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
     float(*as)[kPitch] = reinterpret_cast<float(*)[kPitch]>(smem);                      // [2 * kStep]
     float(*bs)[kPitch] = reinterpret_cast<float(*)[kPitch]>(smem + 2 * kStep * kPitch);  // [2 * kStep]
-    const int t = threadIdx.x, tx = t % 16, ty = t / 16;
+    const int t = threadIdx.x, tx = t % kSide, ty = t / kSide;
     const int64_t tile_m = blockIdx.x / tiles_n, tile_n = blockIdx.x - tile_m * tiles_n;
     const int64_t m0 = tile_m * B, n0 = tile_n * B;
     const int64_t steps = (g.k + kStep - 1) / kStep;
     const int64_t s0 = steps * rank / ranks, s1 = steps * (rank + 1) / ranks;
-    float acc[E][E];
+    uint64_t acc[8][4];
 #pragma unroll
-    for (int i = 0; i < E; ++i)
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < E; ++j) acc[i][j] = 0.0f;
-    Loader32<B> la, lb;
-    la.fetch(g.a, g.a_row, g.a_k, m0, g.m, s0 * kStep, g.k, t);
-    lb.fetch(g.b, g.b_row, g.b_k, n0, g.n, s0 * kStep, g.k, t);
+        for (int j = 0; j < 4; ++j) acc[i][j] = 0ull;
+    Loader32<B, AK, VEC> la;
+    Loader32<B, BK, VEC> lb;
+    la.start(g.a, g.a_ld, m0, g.m, s0 * kStep, t);
+    lb.start(g.b, g.b_ld, n0, g.n, s0 * kStep, t);
+    la.fetch(g.k - s0 * kStep, t);
+    lb.fetch(g.k - s0 * kStep, t);
     for (int64_t s = s0; s < s1; ++s) {
         const int buf = (int)((s - s0) & 1) * kStep;
-        la.store(as + buf, g.a_k == 1, t);
-        lb.store(bs + buf, g.b_k == 1, t);
+        la.store(as + buf, t);
+        lb.store(bs + buf, t);
         __syncthreads();
         if (s + 1 < s1) {
-            la.fetch(g.a, g.a_row, g.a_k, m0, g.m, (s + 1) * kStep, g.k, t);
-            lb.fetch(g.b, g.b_row, g.b_k, n0, g.n, (s + 1) * kStep, g.k, t);
+            la.fetch(g.k - (s + 1) * kStep, t);
+            lb.fetch(g.k - (s + 1) * kStep, t);
         }
 #pragma unroll
         for (int k = 0; k < kStep; ++k) {
-            float a[E], b[E];
+            float a[8];
+            uint64_t b[4];
 #pragma unroll
-            for (int q = 0; q < E / 4; ++q) {
-                *reinterpret_cast<float4*>(a + 4 * q) = *reinterpret_cast<float4*>(&as[buf + k][64 * q + ty * 4]);
-                *reinterpret_cast<float4*>(b + 4 * q) = *reinterpret_cast<float4*>(&bs[buf + k][64 * q + tx * 4]);
+            for (int q = 0; q < 2; ++q) {
+                *reinterpret_cast<float4*>(a + 4 * q) = *reinterpret_cast<float4*>(&as[buf + k][B / 2 * q + ty * 4]);
+                *reinterpret_cast<ulonglong2*>(b + 2 * q) =
+                    *reinterpret_cast<ulonglong2*>(&bs[buf + k][B / 2 * q + tx * 4]);
             }
 #pragma unroll
-            for (int i = 0; i < E; ++i)
+            for (int i = 0; i < 8; ++i) {
+                const uint64_t twice = pair_of(a[i], a[i]);
 #pragma unroll
-                for (int j = 0; j < E; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+                for (int j = 0; j < 4; ++j) multiply_add(acc[i][j], twice, b[j]);
+            }
         }
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < E; ++i)
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int q = 0; q < E / 4; ++q)
-            *reinterpret_cast<float4*>(smem + (64 * (i / 4) + ty * 4 + i % 4) * kPitch + 64 * q + tx * 4) =
-                make_float4(acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]);
+        for (int q = 0; q < 2; ++q)
+            *reinterpret_cast<ulonglong2*>(smem + (B / 2 * (i / 4) + ty * 4 + i % 4) * kPitch + B / 2 * q + tx * 4) =
+                make_ulonglong2(acc[i][2 * q], acc[i][2 * q + 1]);
     if (ranks > 1)
         cluster.sync();
     else
         __syncthreads();
     const int rows = B / ranks, first = rank * rows;
-    for (int i = t; i < rows * B; i += 256) {
+#pragma unroll 4
+    for (int i = t; i < rows * B; i += T::kThreads) {
         const int r = first + i / B, c = i % B;
         const int64_t m = m0 + r, n = n0 + c;
         if (m >= g.m || n >= g.n) continue;
@@ -259,24 +307,27 @@ __global__ void __launch_bounds__(256) gemm32_kernel(Gemm32 g, int tiles_n) {
     if (ranks > 1) cluster.sync();  // no CTA leaves while another reads its part
 }
 
-template <int B>
+template <int B, bool AK, bool BK, bool VEC>
 int launch_gemm32(const Gemm32& g, cudaStream_t s) {
-    auto* kernel = gemm32_kernel<B>;
+    using T = Tile32<B>;
+    auto* kernel = gemm32_kernel<B, AK, BK, VEC>;
     static bool ready[64] = {};
     if (!once_per_device(ready, [&] {
-            return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemm32Smem<B>) ==
-                   cudaSuccess;
+            return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem) == cudaSuccess &&
+                   cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
         }))
         return launch_status();
     const int64_t tiles_n = (g.n + B - 1) / B, tiles = (g.m + B - 1) / B * tiles_n;
     if (tiles >= (1ll << 31)) return GK_EINVAL;
     const int64_t steps = (g.k + kStep - 1) / kStep;
-    int ranks = 1;  // parts of four steps or more, until the CTAs fill two to an SM
-    while (ranks < 8 && tiles * ranks * 2 <= 2 * kSmCount && steps >= ranks * 2 * 4) ranks *= 2;
+    // Parts of four steps or more, until there are two (six of the small tile) CTAs an SM.
+    const int64_t most = (B == 128 ? 2 : 6) * kSmCount;
+    int ranks = 1;
+    while (ranks < 16 && tiles * ranks * 2 <= most && steps >= ranks * 2 * 4) ranks *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)tiles, 1, (unsigned)ranks);
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = kGemm32Smem<B>;
+    cfg.blockDim = dim3(T::kThreads);
+    cfg.dynamicSmemBytes = T::kSmem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -287,10 +338,13 @@ int launch_gemm32(const Gemm32& g, cudaStream_t s) {
     return (int)cudaLaunchKernelEx(&cfg, kernel, g, (int)tiles_n);
 }
 
+template <bool AK, bool BK>
 int gemm32(const Gemm32& g, cudaStream_t s) {
+    const bool vec = aligned16(g.a) && aligned16(g.b) && g.a_ld % 4 == 0 && g.b_ld % 4 == 0;
     // The larger tile once its CTAs fill the SMs: half the shared-memory traffic a product.
-    const int64_t large = ((g.m + 127) / 128) * ((g.n + 127) / 128);
-    return large >= kSmCount ? launch_gemm32<128>(g, s) : launch_gemm32<64>(g, s);
+    if (((g.m + 127) / 128) * ((g.n + 127) / 128) >= kSmCount)
+        return vec ? launch_gemm32<128, AK, BK, true>(g, s) : launch_gemm32<128, AK, BK, false>(g, s);
+    return vec ? launch_gemm32<64, AK, BK, true>(g, s) : launch_gemm32<64, AK, BK, false>(g, s);
 }
 
 // ------------------------------------------------------------ dz and db
@@ -624,14 +678,14 @@ int backward(const gk_linear_grad_t& p, void* workspace, uint32_t* status, cudaS
     } else {
         const float* dz = static_cast<const float*>(b.dz.p);
         if (p.dx != nullptr) {
-            Gemm32 g{dz, static_cast<const float*>(b.w.p), b.dz.ld, 1, 1, b.w.ld, static_cast<float*>(p.dx),
+            Gemm32 g{dz, static_cast<const float*>(b.w.p), b.dz.ld, b.w.ld, static_cast<float*>(p.dx),
                      nullptr, nullptr, nullptr, p.k, 0, 0, p.m, p.k, p.n, GK_ACT_NONE};
-            if ((e = gemm32(g, s)) != 0) return e;
+            if ((e = gemm32<true, false>(g, s)) != 0) return e;
         }
         if (p.dw != nullptr) {
-            Gemm32 g{dz, static_cast<const float*>(b.x.p), 1, b.dz.ld, 1, b.x.ld, static_cast<float*>(p.dw),
+            Gemm32 g{dz, static_cast<const float*>(b.x.p), b.dz.ld, b.x.ld, static_cast<float*>(p.dw),
                      nullptr, nullptr, nullptr, p.k, 0, 0, p.n, p.k, p.m, GK_ACT_NONE};
-            if ((e = gemm32(g, s)) != 0) return e;
+            if ((e = gemm32<false, false>(g, s)) != 0) return e;
         }
     }
     return 0;
@@ -661,11 +715,11 @@ int gk_linear_forward(const gk_linear_t* p, void* workspace, uint32_t* status, v
         return few_rows_by_m<__half>(r, s);
     }
     if (p->dtype == GK_FP32) {
-        Gemm32 g{static_cast<const float*>(p->x), static_cast<const float*>(p->w), p->x_stride, 1, p->w_stride, 1,
+        Gemm32 g{static_cast<const float*>(p->x), static_cast<const float*>(p->w), p->x_stride, p->w_stride,
                  static_cast<float*>(p->y), static_cast<const float*>(p->bias),
                  static_cast<const float*>(p->residual), static_cast<float*>(p->pre), p->n, p->residual_stride, p->n,
                  p->m, p->n, p->k, p->activation};
-        return gemm32(g, s);
+        return gemm32<true, true>(g, s);
     }
     int e = copy_if_needed(f.x, p->x, p->x_stride, p->m, p->k, s);
     if (e == 0) e = copy_if_needed(f.w, p->w, p->w_stride, p->n, p->k, s);

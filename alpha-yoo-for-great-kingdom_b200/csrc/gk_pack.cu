@@ -72,31 +72,55 @@ __device__ __forceinline__ T held(uint32_t code, float scale) {
     return rounded<T>(v > most ? most : (v < -most ? -most : v));
 }
 
-// A lane an element, a warp a block of 32.
+// The largest finite magnitude of a warp's lanes: as bits, which order like the magnitudes.
+__device__ __forceinline__ float warp_top(float v) {
+    return __uint_as_float(__reduce_max_sync(kFull, __float_as_uint(finite_magnitude(v))));
+}
+
+// A lane an element, a warp four blocks of 32 at a time along a chunk of a row.
+constexpr int64_t kChunk = 4096;  // columns a warp takes of a row
+template <typename T>
+__device__ __forceinline__ void pack_span(const T* x, int64_t count, uint8_t* codes, uint8_t* scales, int lane) {
+    for (int64_t c0 = 0; c0 < count; c0 += 4 * kBlock) {
+        float v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t c = c0 + u * kBlock + lane;
+            v[u] = c < count ? as_float<T>(x[c]) : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t c = c0 + u * kBlock + lane;
+            const int s = scale_exponent<T>(warp_top(v[u]));
+            if (c < count) codes[c] = (uint8_t)code_of(v[u], power_of_two(-s));
+            if (lane == 0 && c < count) scales[c / kBlock] = (uint8_t)(s + 127);
+        }
+    }
+}
 template <typename T>
 __global__ void __launch_bounds__(256) pack_rows_kernel(const T* x, int64_t stride, int64_t rows, int64_t cols,
                                                         uint8_t* codes, uint8_t* scales) {
     const int lane = threadIdx.x & 31;
-    const int64_t per_row = (cols + kBlock - 1) / kBlock, items = rows * per_row;
-    const int64_t warps = (int64_t)gridDim.x * 8;
+    const int64_t per_row = (cols + kBlock - 1) / kBlock, chunks = (cols + kChunk - 1) / kChunk;
+    const int64_t items = rows * chunks, warps = (int64_t)gridDim.x * 8;
     for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += warps) {
-        const int64_t r = it / per_row, b = it - r * per_row, c = b * kBlock + lane;
-        const float v = c < cols ? as_float<T>(x[r * stride + c]) : 0.0f;
-        float top = finite_magnitude(v);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
-        const int s = scale_exponent<T>(top);
-        if (c < cols) codes[r * cols + c] = (uint8_t)code_of(v, power_of_two(-s));
-        if (lane == 0) scales[it] = (uint8_t)(s + 127);
+        const int64_t r = it / chunks, c0 = (it - r * chunks) * kChunk;
+        pack_span(x + r * stride + c0, cols - c0 < kChunk ? cols - c0 : kChunk, codes + r * cols + c0,
+                  scales + r * per_row + c0 / kBlock, lane);
     }
 }
 
 // Whole blocks of aligned rows: 16 bytes a thread, 32 * sizeof(T) / 16 threads
 // a block of 32, four vectors a thread in flight.
 template <typename T>
-__global__ void __launch_bounds__(256) pack_vectors_kernel(const T* x, int64_t vectors, uint8_t* codes,
+__global__ void __launch_bounds__(256) pack_vectors_kernel(const T* x, int64_t vectors, int tail, uint8_t* codes,
                                                            uint8_t* scales) {
     constexpr int V = 16 / (int)sizeof(T), kTeam = kBlock / V, kUnroll = 4;
+    if (tail > 0 && blockIdx.x == gridDim.x - 1) {  // the last, shorter block of 32
+        if (threadIdx.x < 32)
+            pack_span(x + vectors * V, tail, codes + vectors * V, scales + vectors / kTeam, threadIdx.x);
+        return;
+    }
     const int64_t start = (int64_t)blockIdx.x * (256 * kUnroll) + threadIdx.x;
     uint4 raw[kUnroll];
 #pragma unroll
@@ -132,21 +156,45 @@ __global__ void __launch_bounds__(256) pack_vectors_kernel(const T* x, int64_t v
 }
 
 template <typename T>
+__device__ __forceinline__ void unpack_span(const uint8_t* codes, const uint8_t* scales, int64_t count, T* x,
+                                            int lane) {
+    for (int64_t c0 = 0; c0 < count; c0 += 4 * kBlock) {
+        uint32_t code[4], scale[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t c = c0 + u * kBlock + lane;
+            code[u] = c < count ? codes[c] : 0u;
+            scale[u] = c < count ? scales[c / kBlock] : 0u;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t c = c0 + u * kBlock + lane;
+            if (c < count) x[c] = held<T>(code[u], power_of_two((int)scale[u] - 127));
+        }
+    }
+}
+template <typename T>
 __global__ void __launch_bounds__(256) unpack_rows_kernel(const uint8_t* codes, const uint8_t* scales, int64_t rows,
                                                           int64_t cols, T* x, int64_t stride) {
     const int lane = threadIdx.x & 31;
-    const int64_t per_row = (cols + kBlock - 1) / kBlock, items = rows * per_row;
-    const int64_t warps = (int64_t)gridDim.x * 8;
+    const int64_t per_row = (cols + kBlock - 1) / kBlock, chunks = (cols + kChunk - 1) / kChunk;
+    const int64_t items = rows * chunks, warps = (int64_t)gridDim.x * 8;
     for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += warps) {
-        const int64_t r = it / per_row, c = (it - r * per_row) * kBlock + lane;
-        if (c < cols) x[r * stride + c] = held<T>(codes[r * cols + c], power_of_two((int)scales[it] - 127));
+        const int64_t r = it / chunks, c0 = (it - r * chunks) * kChunk;
+        unpack_span(codes + r * cols + c0, scales + r * per_row + c0 / kBlock,
+                    cols - c0 < kChunk ? cols - c0 : kChunk, x + r * stride + c0, lane);
     }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) unpack_vectors_kernel(const uint8_t* codes, const uint8_t* scales,
-                                                             int64_t vectors, T* x) {
+                                                             int64_t vectors, int tail, T* x) {
     constexpr int V = 16 / (int)sizeof(T), kTeam = kBlock / V, kUnroll = 4;
+    if (tail > 0 && blockIdx.x == gridDim.x - 1) {  // the last, shorter block of 32
+        if (threadIdx.x < 32)
+            unpack_span(codes + vectors * V, scales + vectors / kTeam, tail, x + vectors * V, threadIdx.x);
+        return;
+    }
     const int64_t start = (int64_t)blockIdx.x * (256 * kUnroll) + threadIdx.x;
     uint32_t word[kUnroll][V / 4];
     float scale[kUnroll];
@@ -175,18 +223,22 @@ __global__ void __launch_bounds__(256) unpack_vectors_kernel(const uint8_t* code
 
 bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 
-// Rows that follow one another without a gap, in whole blocks: one run of vectors.
-bool one_run(int64_t rows, int64_t cols, int64_t stride) { return cols % kBlock == 0 && (rows == 1 || stride == cols); }
+// Rows in whole blocks that follow one another without a gap, or one row: one
+// run of vectors, and the row's last block if it is shorter.
+bool one_run(int64_t rows, int64_t cols, int64_t stride) {
+    return rows == 1 || (cols % kBlock == 0 && stride == cols);
+}
 
 template <typename T>
 int pack(const void* x, int64_t stride, int64_t rows, int64_t cols, uint8_t* codes, uint8_t* scales,
          cudaStream_t s) {
     if (one_run(rows, cols, stride) && aligned16(x) && aligned8(codes)) {
-        const int64_t vectors = rows * cols / (16 / (int64_t)sizeof(T));
-        pack_vectors_kernel<T><<<(unsigned)((vectors + 1023) / 1024), 256, 0, s>>>(static_cast<const T*>(x), vectors,
-                                                                                   codes, scales);
+        const int tail = (int)(rows * cols % kBlock);
+        const int64_t vectors = (rows * cols - tail) / (16 / (int64_t)sizeof(T));
+        const unsigned grid = (unsigned)((vectors + 1023) / 1024) + (tail > 0 ? 1u : 0u);
+        pack_vectors_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(x), vectors, tail, codes, scales);
     } else {
-        const int64_t items = rows * ((cols + kBlock - 1) / kBlock);
+        const int64_t items = rows * ((cols + kChunk - 1) / kChunk);
         pack_rows_kernel<T><<<blocks_for(items, 8, kSmCount * 32), 256, 0, s>>>(static_cast<const T*>(x), stride,
                                                                                 rows, cols, codes, scales);
     }
@@ -197,11 +249,12 @@ template <typename T>
 int unpack(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* x, int64_t stride,
            cudaStream_t s) {
     if (one_run(rows, cols, stride) && aligned16(x) && aligned8(codes)) {
-        const int64_t vectors = rows * cols / (16 / (int64_t)sizeof(T));
-        unpack_vectors_kernel<T><<<(unsigned)((vectors + 1023) / 1024), 256, 0, s>>>(codes, scales, vectors,
-                                                                                     static_cast<T*>(x));
+        const int tail = (int)(rows * cols % kBlock);
+        const int64_t vectors = (rows * cols - tail) / (16 / (int64_t)sizeof(T));
+        const unsigned grid = (unsigned)((vectors + 1023) / 1024) + (tail > 0 ? 1u : 0u);
+        unpack_vectors_kernel<T><<<grid, 256, 0, s>>>(codes, scales, vectors, tail, static_cast<T*>(x));
     } else {
-        const int64_t items = rows * ((cols + kBlock - 1) / kBlock);
+        const int64_t items = rows * ((cols + kChunk - 1) / kChunk);
         unpack_rows_kernel<T><<<blocks_for(items, 8, kSmCount * 32), 256, 0, s>>>(codes, scales, rows, cols,
                                                                                   static_cast<T*>(x), stride);
     }
