@@ -16,6 +16,8 @@
 #include <cooperative_groups.h>
 #include <cuda.h>
 
+#include <cmath>
+
 #include "../../include/gk.h"
 #include "gk_act.cuh"
 #include "gk_launch.cuh"
@@ -179,27 +181,75 @@ __device__ __forceinline__ bool warp_wait(bool ready, uint32_t bar, uint32_t par
 
 // ------------------------------------------------------------------ split
 
-// Tiles of 128 x BN, one CTA each; with few tiles a cluster of CTAs shares a
+// Tiles of 128 x 64, one CTA each; with few tiles a cluster of CTAs shares a
 // tile along k. Every CTA of the cluster leaves its fp32 part in its shared
 // memory, and each then adds up, in rank order, and finishes a share of the
 // tile's rows: no workspace, no atomics, one launch.
 // Warp 0 loads, warp 1 issues the MMAs, warps 2-5 drain TMEM, all finish.
 constexpr int kSplitThreads = 192;
-template <int BN>
 struct Split {
+    static constexpr int kBN = 64;
     static constexpr int kStages = 4;
-    static constexpr int kA = 128 * kBK * 2, kB = BN * kBK * 2, kStage = kA + kB;
-    static constexpr int kPitch = BN + 4;  // fp32 row pitch of the part: rows 16 bytes apart modulo the banks
+    static constexpr int kA = 128 * kBK * 2, kB = kBN * kBK * 2, kStage = kA + kB;
+    static constexpr int kPitch = kBN + 4;  // fp32 row pitch of the part: rows 16 bytes apart modulo the banks
     static constexpr int kSmem = kStages * kStage + 1024;
     static_assert(128 * kPitch * 4 <= kStages * kStage, "the part reuses the stages");
 };
 
-template <int BN>
+// Bias, residual, activation and stores of four neighbours of a row.
+__device__ __forceinline__ void finish4(const Epilogue& ep, int64_t m, int n, float (&v)[4], bool bf16) {
+    const int count = min(4, ep.n - n);
+    const bool whole = ep.aligned && count == 4;
+    if (ep.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < count) v[j] += load16(ep.bias, n + j, bf16);
+    }
+    if (ep.residual != nullptr) {
+        if (whole) {
+            const uint2 x =
+                *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(ep.residual) + m * ep.residual_ld + n);
+            float lo, hi;
+            unpack16(x.x, bf16, lo, hi);
+            v[0] += lo, v[1] += hi;
+            unpack16(x.y, bf16, lo, hi);
+            v[2] += lo, v[3] += hi;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < count) v[j] += load16(ep.residual, m * ep.residual_ld + n + j, bf16);
+        }
+    }
+    if (ep.pre != nullptr) {
+        if (whole) {
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(ep.pre) + m * ep.pre_ld + n) =
+                make_uint2(pack16(v[0], v[1], bf16), pack16(v[2], v[3], bf16));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < count) store16(ep.pre, m * ep.pre_ld + n + j, v[j], bf16);
+        }
+    }
+    if (ep.activation != GK_ACT_NONE) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = act_value<true>(v[j], ep.activation);
+    }
+    if (whole) {
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(ep.out) + m * ep.out_ld + n) =
+            make_uint2(pack16(v[0], v[1], bf16), pack16(v[2], v[3], bf16));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < count) store16(ep.out, m * ep.out_ld + n + j, v[j], bf16);
+    }
+}
+
 __global__ void __launch_bounds__(kSplitThreads) gemm_split_kernel(const __grid_constant__ CUtensorMap ta,
                                                                    const __grid_constant__ CUtensorMap tb,
                                                                    Epilogue ep, int tiles_n, int k_blocks,
                                                                    int a_across, int b_across, uint32_t* status) {
-    using S = Split<BN>;
+    using S = Split;
+    constexpr int BN = S::kBN;
     extern __shared__ uint8_t raw[];
     __shared__ alignas(8) uint64_t full[S::kStages], empty[S::kStages], done;
     __shared__ uint32_t tmem_slot;
@@ -290,50 +340,28 @@ __global__ void __launch_bounds__(kSplitThreads) gemm_split_kernel(const __grid_
     }
     const int rows = 128 / ranks, first = rank * rows;
     const bool bf16 = ep.bf16 != 0;
+    if (ranks == 1) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < 128 * (BN / 4); i += kSplitThreads) {
+            const int r = i / (BN / 4), c = (i % (BN / 4)) * 4;
+            if (m0 + r >= ep.m || n0 + c >= ep.n) continue;
+            const float4 x = *reinterpret_cast<const float4*>(part + r * S::kPitch + c);
+            float v[4] = {x.x, x.y, x.z, x.w};
+            finish4(ep, m0 + r, n0 + c, v, bf16);
+        }
+        return;
+    }
     for (int i = threadIdx.x; i < rows * (BN / 4); i += kSplitThreads) {
         const int r = first + i / (BN / 4), c = (i % (BN / 4)) * 4;
-        const int64_t m = m0 + r;
-        const int n = n0 + c;
-        if (m >= ep.m || n >= ep.n) continue;
+        if (m0 + r >= ep.m || n0 + c >= ep.n) continue;
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int k = 0; k < ranks; ++k) {
-            const float* other = ranks > 1 ? cluster.map_shared_rank(part, k) : part;
-            const float4 x = *reinterpret_cast<const float4*>(other + r * S::kPitch + c);
+            const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(part, k) + r * S::kPitch + c);
             v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
         }
-        const int count = min(4, ep.n - n);
-        const bool whole = ep.aligned && count == 4;
-        if (ep.bias != nullptr)
-            for (int j = 0; j < count; ++j) v[j] += load16(ep.bias, n + j, bf16);
-        if (ep.residual != nullptr) {
-            if (whole) {
-                const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(ep.residual) +
-                                                               m * ep.residual_ld + n);
-                float lo, hi;
-                unpack16(x.x, bf16, lo, hi);
-                v[0] += lo, v[1] += hi;
-                unpack16(x.y, bf16, lo, hi);
-                v[2] += lo, v[3] += hi;
-            } else {
-                for (int j = 0; j < count; ++j) v[j] += load16(ep.residual, m * ep.residual_ld + n + j, bf16);
-            }
-        }
-        if (ep.pre != nullptr) {
-            if (whole)
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(ep.pre) + m * ep.pre_ld + n) =
-                    make_uint2(pack16(v[0], v[1], bf16), pack16(v[2], v[3], bf16));
-            else
-                for (int j = 0; j < count; ++j) store16(ep.pre, m * ep.pre_ld + n + j, v[j], bf16);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = act_value<true>(v[j], ep.activation);
-        if (whole)
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(ep.out) + m * ep.out_ld + n) =
-                make_uint2(pack16(v[0], v[1], bf16), pack16(v[2], v[3], bf16));
-        else
-            for (int j = 0; j < count; ++j) store16(ep.out, m * ep.out_ld + n + j, v[j], bf16);
+        finish4(ep, m0 + r, n0 + c, v, bf16);
     }
-    if (ranks > 1) cluster.sync();  // no CTA leaves while another reads its part
+    cluster.sync();  // no CTA leaves while another reads its part
 }
 
 // ------------------------------------------------------------------- pair
@@ -688,10 +716,17 @@ Epilogue epilogue_of(const GemmArgs& g) {
     return e;
 }
 
-template <int BN>
+// CTAs that share a tile along k: until they fill two to an SM, in parts of four stages or more.
+int split_ranks(int64_t tiles, int64_t stages) {
+    int ranks = 1;
+    while (ranks < 8 && tiles * ranks * 2 <= 2 * kSmCount && stages >= ranks * 2 * 4) ranks *= 2;
+    return ranks;
+}
+
 int launch_split(const GemmArgs& g, uint32_t* status, cudaStream_t stream) {
-    using S = Split<BN>;
-    auto* kernel = gemm_split_kernel<BN>;
+    using S = Split;
+    constexpr int BN = S::kBN;
+    auto* kernel = gemm_split_kernel;
     static bool ready[64] = {};
     if (!once_per_device(ready, [&] {
             return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) == cudaSuccess;
@@ -702,9 +737,7 @@ int launch_split(const GemmArgs& g, uint32_t* status, cudaStream_t stream) {
         !encode(&tb, g.b, g.b_ld, g.b_across, g.n, g.k, BN, g.dtype))
         return GK_EINVAL;
     const int64_t tiles_m = (g.m + 127) / 128, tiles_n = (g.n + BN - 1) / BN, blocks = (g.k + kBK - 1) / kBK;
-    // Split k until the CTAs fill two to an SM, in parts of four stages or more.
-    int ranks = 1;
-    while (ranks < 8 && tiles_m * tiles_n * ranks * 2 <= 2 * kSmCount && blocks >= ranks * 2 * 4) ranks *= 2;
+    const int ranks = split_ranks(tiles_m * tiles_n, blocks);
     cudaLaunchConfig_t cfg = {};
     if (tiles_m * tiles_n >= (1ll << 31)) return GK_EINVAL;
     cfg.gridDim = dim3((unsigned)(tiles_n * tiles_m), 1, (unsigned)ranks);
@@ -754,9 +787,24 @@ int gemm16(const GemmArgs& g, uint32_t* status, cudaStream_t stream) {
     if (g.m < 1 || g.n < 1 || g.k < 1 || g.m >= (1ll << 31) || g.n >= (1ll << 31) || g.k >= (1ll << 31))
         return GK_EINVAL;
     if (!aligned16(g.a) || !aligned16(g.b) || g.a_ld % 8 != 0 || g.b_ld % 8 != 0) return GK_EINVAL;
-    const int64_t large = ((g.m + 255) / 256) * ((g.n + 255) / 256);
-    if (large >= kSmCount / 2) return launch_pair<256>(g, status, stream);
-    return launch_split<64>(g, status, stream);
+    // The form is taken by an estimate of its time in microseconds: a start, and
+    // for every round of the tiles that run at once the stages of k that one CTA
+    // (or pair) walks, or the epilogue where k is short. Measured
+    // (split 128 x 64 | pairs 256 x 128 | pairs 256 x 256; m x k x n):
+    // 16 x 4096 x 4096 10.8 | 20.5 | 23.9, 256 x 256 x 256 6.9 | 6.4 | 8.0,
+    // 256 x 4096 x 4096 17.0 | 21.5 | 25.3, 1024 x 256 x 4096 14.3 | 8.9 | 8.6,
+    // 1024 x 1024 x 1024 10.5 | 9.7 | 11.7, 2048^3 29.5 | 22.7 | 17.8,
+    // 4096^3 161 | 123 | 95, 16384 x 1024 x 256 21.2 | 14.8 | 12.5.
+    const double stages = (double)((g.k + kBK - 1) / kBK);
+    auto rounds = [](int64_t work, int64_t at_once) { return (double)((work + at_once - 1) / at_once); };
+    const int64_t tiles_m = (g.m + 255) / 256, split_tiles = ((g.m + 127) / 128) * ((g.n + 63) / 64);
+    const int ranks = split_ranks(split_tiles, (g.k + kBK - 1) / kBK);
+    const double split = rounds(split_tiles * ranks, 2 * kSmCount) * (6.3 + stages / ranks * 0.28) -
+                         (g.m <= 64 ? 1.3 : 0.0);
+    const double narrow = 5.3 + rounds(tiles_m * ((g.n + 127) / 128), kSmCount / 2) * fmax(stages * 0.233, 1.3);
+    const double wide = 5.6 + rounds(tiles_m * ((g.n + 255) / 256), kSmCount / 2) * fmax(stages * 0.28, 2.0);
+    if (split <= narrow && split <= wide) return launch_split(g, status, stream);
+    return narrow <= wide ? launch_pair<128>(g, status, stream) : launch_pair<256>(g, status, stream);
 }
 
 }  // namespace gk

@@ -146,29 +146,30 @@ struct Gemm32 {
     int64_t out_ld, residual_ld, pre_ld;
     int64_t m, n, k;
     int activation;
+    int wide;  // rows of out and pre start on 16 bytes
 };
 
-// A tile of B x B outputs, 8 x 8 to a thread, k in steps of 16 through two
+// A tile of B x B outputs, P x P to a thread, k in steps of 16 through two
 // shared-memory buffers with the next step's loads in registers. The products
 // are packed pairs (two fp32 multiply-adds an instruction, each rounded like
 // one of its own). With few tiles a cluster of CTAs shares one along k and adds
 // the parts up in rank order through distributed shared memory.
 constexpr int kStep = 16;
-template <int B>
+template <int B, int P>
 struct Tile32 {
-    static constexpr int kThreads = (B / 8) * (B / 8), kPitch = B + 4;
+    static constexpr int kThreads = (B / P) * (B / P), kPitch = B + 4;
     static constexpr int kSmem = (B * kPitch > 4 * kStep * kPitch ? B * kPitch : 4 * kStep * kPitch) * 4;
     static constexpr int kQuads = B * kStep / 4 / kThreads;  // groups of four elements a thread loads of an operand
 };
 
 // One operand's B x 16 step, four neighbours at a time along its contiguous
 // dimension: k (K) or the row. VEC: those four are one aligned 16-byte load.
-template <int B, bool K, bool VEC>
+template <int B, int P, bool K, bool VEC>
 struct Loader32 {
-    using T = Tile32<B>;
+    using T = Tile32<B, P>;
     float v[T::kQuads][4];
     const float* at[T::kQuads];  // this thread's first element of each group, now
-    int64_t left[T::kQuads];     // K: rows left from it (1 or 0); else elements left of its four
+    int left;                    // rows of the tile
     int64_t step;
     __device__ __forceinline__ static void place(int t, int i, int& row, int& k) {
         const int q = t + i * T::kThreads;
@@ -179,27 +180,37 @@ struct Loader32 {
     }
     __device__ __forceinline__ void start(const float* p, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int t) {
         step = K ? kStep : kStep * ld;
+        left = rows - row0 < B ? (int)(rows - row0) : B;
 #pragma unroll
         for (int i = 0; i < T::kQuads; ++i) {
             int row, k;
             place(t, i, row, k);
-            left[i] = rows - (row0 + row);
             at[i] = K ? p + (row0 + row) * ld + k0 + k : p + (k0 + k) * ld + row0 + row;
         }
     }
     // `k_left`: k elements left from the step's start.
     __device__ __forceinline__ void fetch(int64_t k_left, int t) {
+        if (left == B && k_left >= kStep) {
+#pragma unroll
+            for (int i = 0; i < T::kQuads; ++i) {
+                if (VEC) {
+                    *reinterpret_cast<float4*>(v[i]) = __ldg(reinterpret_cast<const float4*>(at[i]));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[i][j] = __ldg(at[i] + j);
+                }
+                at[i] += step;
+            }
+            return;
+        }
+        const int k_end = k_left < kStep ? (int)k_left : kStep;
 #pragma unroll
         for (int i = 0; i < T::kQuads; ++i) {
             int row, k;
             place(t, i, row, k);
-            const int64_t count = K ? (left[i] > 0 ? k_left - k : 0) : (k < k_left ? left[i] : 0);
-            if (VEC && count >= 4) {
-                *reinterpret_cast<float4*>(v[i]) = __ldg(reinterpret_cast<const float4*>(at[i]));
-            } else {
+            const int count = K ? (row < left ? k_end - k : 0) : (k < k_end ? left - row : 0);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[i][j] = j < count ? __ldg(at[i] + j) : 0.0f;
-            }
+            for (int j = 0; j < 4; ++j) v[i][j] = j < count ? __ldg(at[i] + j) : 0.0f;
             at[i] += step;
         }
     }
@@ -227,11 +238,42 @@ __device__ __forceinline__ void multiply_add(uint64_t& acc, uint64_t a, uint64_t
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
 }
 
-template <int B, bool AK, bool BK, bool VEC>
-__global__ void __launch_bounds__(Tile32<B>::kThreads, B == 128 ? 2 : 6) gemm32_kernel(Gemm32 g, int tiles_n) {
+// Bias, residual, activation and stores of four neighbours of a row.
+__device__ __forceinline__ void finish4(const Gemm32& g, int64_t m, int64_t n, float (&v)[4]) {
+    const bool whole = g.wide && n + 4 <= g.n;
+    const int count = g.n - n < 4 ? (int)(g.n - n) : 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (j < count) {
+            if (g.bias != nullptr) v[j] += __ldg(g.bias + n + j);
+            if (g.residual != nullptr) v[j] += __ldg(g.residual + m * g.residual_ld + n + j);
+        }
+    }
+    float* pre = g.pre == nullptr ? nullptr : g.pre + m * g.pre_ld + n;
+    float* out = g.out + m * g.out_ld + n;
+    if (whole) {
+        if (pre != nullptr) *reinterpret_cast<float4*>(pre) = make_float4(v[0], v[1], v[2], v[3]);
+        if (g.activation != GK_ACT_NONE) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = act_value<false>(v[j], g.activation);
+        }
+        *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j >= count) break;
+            if (pre != nullptr) pre[j] = v[j];
+            out[j] = g.activation == GK_ACT_NONE ? v[j] : act_value<false>(v[j], g.activation);
+        }
+    }
+}
+
+template <int B, int P, bool AK, bool BK, bool VEC>
+__global__ void __launch_bounds__(Tile32<B, P>::kThreads, P == 8 ? 512 / Tile32<B, P>::kThreads : 1)
+    gemm32_kernel(Gemm32 g, int tiles_n) {
     extern __shared__ float smem[];
-    using T = Tile32<B>;
-    constexpr int kSide = B / 8, kPitch = T::kPitch;
+    using T = Tile32<B, P>;
+    constexpr int kSide = B / P, kPitch = T::kPitch, kParts = P / 4;
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
     float(*as)[kPitch] = reinterpret_cast<float(*)[kPitch]>(smem);                      // [2 * kStep]
@@ -241,13 +283,13 @@ __global__ void __launch_bounds__(Tile32<B>::kThreads, B == 128 ? 2 : 6) gemm32_
     const int64_t m0 = tile_m * B, n0 = tile_n * B;
     const int64_t steps = (g.k + kStep - 1) / kStep;
     const int64_t s0 = steps * rank / ranks, s1 = steps * (rank + 1) / ranks;
-    uint64_t acc[8][4];
+    uint64_t acc[P][P / 2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < P; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = 0ull;
-    Loader32<B, AK, VEC> la;
-    Loader32<B, BK, VEC> lb;
+        for (int j = 0; j < P / 2; ++j) acc[i][j] = 0ull;
+    Loader32<B, P, AK, VEC> la;
+    Loader32<B, P, BK, VEC> lb;
     la.start(g.a, g.a_ld, m0, g.m, s0 * kStep, t);
     lb.start(g.b, g.b_ld, n0, g.n, s0 * kStep, t);
     la.fetch(g.k - s0 * kStep, t);
@@ -263,54 +305,63 @@ __global__ void __launch_bounds__(Tile32<B>::kThreads, B == 128 ? 2 : 6) gemm32_
         }
 #pragma unroll
         for (int k = 0; k < kStep; ++k) {
-            float a[8];
-            uint64_t b[4];
+            float a[P];
+            uint64_t b[P / 2];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                *reinterpret_cast<float4*>(a + 4 * q) = *reinterpret_cast<float4*>(&as[buf + k][B / 2 * q + ty * 4]);
+            for (int q = 0; q < kParts; ++q) {
+                *reinterpret_cast<float4*>(a + 4 * q) =
+                    *reinterpret_cast<float4*>(&as[buf + k][B / kParts * q + ty * 4]);
                 *reinterpret_cast<ulonglong2*>(b + 2 * q) =
-                    *reinterpret_cast<ulonglong2*>(&bs[buf + k][B / 2 * q + tx * 4]);
+                    *reinterpret_cast<ulonglong2*>(&bs[buf + k][B / kParts * q + tx * 4]);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < P; ++i) {
                 const uint64_t twice = pair_of(a[i], a[i]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) multiply_add(acc[i][j], twice, b[j]);
+                for (int j = 0; j < P / 2; ++j) multiply_add(acc[i][j], twice, b[j]);
             }
         }
     }
+    if (ranks == 1) {  // straight from the registers
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int64_t m = m0 + B / kParts * (i / 4) + ty * 4 + i % 4;
+            if (m >= g.m) continue;
+#pragma unroll
+            for (int q = 0; q < kParts; ++q) {
+                float v[4];
+                *reinterpret_cast<ulonglong2*>(v) = make_ulonglong2(acc[i][2 * q], acc[i][2 * q + 1]);
+                finish4(g, m, n0 + B / kParts * q + tx * 4, v);
+            }
+        }
+        return;
+    }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < P; ++i)
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
-            *reinterpret_cast<ulonglong2*>(smem + (B / 2 * (i / 4) + ty * 4 + i % 4) * kPitch + B / 2 * q + tx * 4) =
-                make_ulonglong2(acc[i][2 * q], acc[i][2 * q + 1]);
-    if (ranks > 1)
-        cluster.sync();
-    else
-        __syncthreads();
-    const int rows = B / ranks, first = rank * rows;
-#pragma unroll 4
-    for (int i = t; i < rows * B; i += T::kThreads) {
-        const int r = first + i / B, c = i % B;
-        const int64_t m = m0 + r, n = n0 + c;
-        if (m >= g.m || n >= g.n) continue;
-        float v = 0.0f;
-        for (int k = 0; k < ranks; ++k)
-            v += (ranks > 1 ? cluster.map_shared_rank(smem, k) : smem)[r * kPitch + c];
-        if (g.bias != nullptr) v += g.bias[n];
-        if (g.residual != nullptr) v += g.residual[m * g.residual_ld + n];
-        if (g.pre != nullptr) g.pre[m * g.pre_ld + n] = v;
-        g.out[m * g.out_ld + n] = act_value<false>(v, g.activation);
+        for (int q = 0; q < kParts; ++q)
+            *reinterpret_cast<ulonglong2*>(smem + (B / kParts * (i / 4) + ty * 4 + i % 4) * kPitch + B / kParts * q +
+                                           tx * 4) = make_ulonglong2(acc[i][2 * q], acc[i][2 * q + 1]);
+    cluster.sync();
+    const int quads = B / ranks * (B / 4), first = rank * (B / ranks);
+    for (int i = t; i < quads; i += T::kThreads) {
+        const int r = first + i / (B / 4), c = i % (B / 4) * 4;
+        if (m0 + r >= g.m || n0 + c >= g.n) continue;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < ranks; ++k) {
+            const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(smem, k) + r * kPitch + c);
+            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+        }
+        finish4(g, m0 + r, n0 + c, v);
     }
-    if (ranks > 1) cluster.sync();  // no CTA leaves while another reads its part
+    cluster.sync();  // no CTA leaves while another reads its part
 }
 
-template <int B, bool AK, bool BK, bool VEC>
+template <int B, int P, bool AK, bool BK, bool VEC>
 int launch_gemm32(const Gemm32& g, cudaStream_t s) {
-    using T = Tile32<B>;
-    auto* kernel = gemm32_kernel<B, AK, BK, VEC>;
+    using T = Tile32<B, P>;
+    auto* kernel = gemm32_kernel<B, P, AK, BK, VEC>;
     static bool ready[64] = {};
     if (!once_per_device(ready, [&] {
             return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem) == cudaSuccess &&
@@ -320,10 +371,10 @@ int launch_gemm32(const Gemm32& g, cudaStream_t s) {
     const int64_t tiles_n = (g.n + B - 1) / B, tiles = (g.m + B - 1) / B * tiles_n;
     if (tiles >= (1ll << 31)) return GK_EINVAL;
     const int64_t steps = (g.k + kStep - 1) / kStep;
-    // Parts of four steps or more, until there are two (six of the small tile) CTAs an SM.
-    const int64_t most = (B == 128 ? 2 : 6) * kSmCount;
+    // Parts of three steps or more, until there are 512 threads an SM.
+    const int64_t most = 512 / T::kThreads * kSmCount;
     int ranks = 1;
-    while (ranks < 16 && tiles * ranks * 2 <= most && steps >= ranks * 2 * 4) ranks *= 2;
+    while (ranks < 16 && tiles * ranks * 2 <= most && steps >= ranks * 2 * 3) ranks *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)tiles, 1, (unsigned)ranks);
     cfg.blockDim = dim3(T::kThreads);
@@ -338,13 +389,26 @@ int launch_gemm32(const Gemm32& g, cudaStream_t s) {
     return (int)cudaLaunchKernelEx(&cfg, kernel, g, (int)tiles_n);
 }
 
-template <bool AK, bool BK>
+template <bool AK, bool BK, bool VEC>
 int gemm32(const Gemm32& g, cudaStream_t s) {
+    // Measured (us, 128 x 128 | 64 x 64 | 32 x 32 tiles): 2048^3 388 | 467 | 601,
+    // 1024^3 55 | 68 | 83, 512 x 4096 x 512 83 | 68 | 91, 300 x 700 x 900
+    // 25 | 24 | 25, 4096 x 162 x 82 20 | 19 | 13, 9 x 4000 x 4000 94 | 67 | 48
+    // (m x k x n). Large tiles reuse more of what they read; small ones keep the
+    // SMs busy on little work and waste less of a ragged edge.
+    auto tiles = [&](int64_t b) { return ((g.m + b - 1) / b) * ((g.n + b - 1) / b); };
+    const double work = (double)g.m * (double)g.n * (double)g.k;
+    const double area128 = 16384.0 * tiles(128), area64 = 4096.0 * tiles(64), area32 = 1024.0 * tiles(32);
+    if (work < 134217728.0 || area64 >= 1.5 * area32) return launch_gemm32<32, 4, AK, BK, VEC>(g, s);
+    if (tiles(128) >= 32 && area128 <= 1.1 * area64) return launch_gemm32<128, 8, AK, BK, VEC>(g, s);
+    return launch_gemm32<64, 8, AK, BK, VEC>(g, s);
+}
+template <bool AK, bool BK>
+int gemm32(Gemm32 g, cudaStream_t s) {
+    g.wide = aligned16(g.out) && g.out_ld % 4 == 0 &&
+             (g.pre == nullptr || (aligned16(g.pre) && g.pre_ld % 4 == 0));
     const bool vec = aligned16(g.a) && aligned16(g.b) && g.a_ld % 4 == 0 && g.b_ld % 4 == 0;
-    // The larger tile once its CTAs fill the SMs: half the shared-memory traffic a product.
-    if (((g.m + 127) / 128) * ((g.n + 127) / 128) >= kSmCount)
-        return vec ? launch_gemm32<128, AK, BK, true>(g, s) : launch_gemm32<128, AK, BK, false>(g, s);
-    return vec ? launch_gemm32<64, AK, BK, true>(g, s) : launch_gemm32<64, AK, BK, false>(g, s);
+    return vec ? gemm32<AK, BK, true>(g, s) : gemm32<AK, BK, false>(g, s);
 }
 
 // ------------------------------------------------------------ dz and db
@@ -679,12 +743,12 @@ int backward(const gk_linear_grad_t& p, void* workspace, uint32_t* status, cudaS
         const float* dz = static_cast<const float*>(b.dz.p);
         if (p.dx != nullptr) {
             Gemm32 g{dz, static_cast<const float*>(b.w.p), b.dz.ld, b.w.ld, static_cast<float*>(p.dx),
-                     nullptr, nullptr, nullptr, p.k, 0, 0, p.m, p.k, p.n, GK_ACT_NONE};
+                     nullptr, nullptr, nullptr, p.k, 0, 0, p.m, p.k, p.n, GK_ACT_NONE, 0};
             if ((e = gemm32<true, false>(g, s)) != 0) return e;
         }
         if (p.dw != nullptr) {
             Gemm32 g{dz, static_cast<const float*>(b.x.p), b.dz.ld, b.x.ld, static_cast<float*>(p.dw),
-                     nullptr, nullptr, nullptr, p.k, 0, 0, p.n, p.k, p.m, GK_ACT_NONE};
+                     nullptr, nullptr, nullptr, p.k, 0, 0, p.n, p.k, p.m, GK_ACT_NONE, 0};
             if ((e = gemm32<false, false>(g, s)) != 0) return e;
         }
     }
@@ -718,7 +782,7 @@ int gk_linear_forward(const gk_linear_t* p, void* workspace, uint32_t* status, v
         Gemm32 g{static_cast<const float*>(p->x), static_cast<const float*>(p->w), p->x_stride, p->w_stride,
                  static_cast<float*>(p->y), static_cast<const float*>(p->bias),
                  static_cast<const float*>(p->residual), static_cast<float*>(p->pre), p->n, p->residual_stride, p->n,
-                 p->m, p->n, p->k, p->activation};
+                 p->m, p->n, p->k, p->activation, 0};
         return gemm32<true, true>(g, s);
     }
     int e = copy_if_needed(f.x, p->x, p->x_stride, p->m, p->k, s);
