@@ -40,7 +40,7 @@ struct Epilogue {
     int m, n;
     int activation;
     int bf16;
-    int aligned;  // every row of out, residual and pre, and the bias, start on 16 bytes
+    int out_wide, pre_wide, residual_wide, bias_wide;  // every row (the bias) starts on 16 bytes
 };
 
 // Issue is warp-wide: every lane of a converged warp runs the loops, so that
@@ -199,14 +199,14 @@ struct Split {
 // Bias, residual, activation and stores of four neighbours of a row.
 __device__ __forceinline__ void finish4(const Epilogue& ep, int64_t m, int n, float (&v)[4], bool bf16) {
     const int count = min(4, ep.n - n);
-    const bool whole = ep.aligned && count == 4;
+    const bool whole = count == 4;
     if (ep.bias != nullptr) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (j < count) v[j] += load16(ep.bias, n + j, bf16);
     }
     if (ep.residual != nullptr) {
-        if (whole) {
+        if (whole && ep.residual_wide) {
             const uint2 x =
                 *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(ep.residual) + m * ep.residual_ld + n);
             float lo, hi;
@@ -221,7 +221,7 @@ __device__ __forceinline__ void finish4(const Epilogue& ep, int64_t m, int n, fl
         }
     }
     if (ep.pre != nullptr) {
-        if (whole) {
+        if (whole && ep.pre_wide) {
             *reinterpret_cast<uint2*>(static_cast<uint16_t*>(ep.pre) + m * ep.pre_ld + n) =
                 make_uint2(pack16(v[0], v[1], bf16), pack16(v[2], v[3], bf16));
         } else {
@@ -234,7 +234,7 @@ __device__ __forceinline__ void finish4(const Epilogue& ep, int64_t m, int n, fl
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = act_value<true>(v[j], ep.activation);
     }
-    if (whole) {
+    if (whole && ep.out_wide) {
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(ep.out) + m * ep.out_ld + n) =
             make_uint2(pack16(v[0], v[1], bf16), pack16(v[2], v[3], bf16));
     } else {
@@ -451,7 +451,7 @@ __device__ __forceinline__ void add_row(const uint8_t* patch, int lane, int half
     }
 }
 __device__ __forceinline__ void add_bias(const Epilogue& ep, int n, float (&v)[32], bool bf16) {
-    if (ep.aligned && n + 32 <= ep.n) {  // every lane reads the same 64 bytes
+    if (ep.bias_wide && n + 32 <= ep.n) {  // every lane reads the same 64 bytes
         const uint4* b = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(ep.bias) + n);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -487,25 +487,44 @@ __device__ __forceinline__ void patch_free(int lane) {
     __syncwarp();
 }
 
-// Rows that do not start on 16 bytes: 32 rows by 32 columns of fp32 through the patch, a lane a column.
-__device__ __forceinline__ void finish_ragged(const Epilogue& ep, const float (&v)[32], int row0, int lane, int n,
-                                              uint8_t* patch) {
-    const bool bf16 = ep.bf16 != 0;
-    float* cell = reinterpret_cast<float*>(patch);  // column i of row r lies at i ^ r
+// Rows that do not start on 16 bytes, which TMA cannot write: row by row, a
+// lane two columns, as 32-bit words that are shifted by one column where a row
+// starts between two words.
+__device__ __forceinline__ uint32_t* patch_word(uint8_t* patch, int row, int lane) {
+    return reinterpret_cast<uint32_t*>(patch_chunk(patch, row, lane >> 2)) + (lane & 3);
+}
+__device__ __forceinline__ void write_ragged(void* out, int64_t ld, uint8_t* patch, int n, int row0, int rows,
+                                             int cols, int lane) {
     __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 32; ++i) cell[lane * 32 + (i ^ lane)] = v[i];
+    uint16_t* base = static_cast<uint16_t*>(out) + row0 * ld + n;
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+        if (r >= rows) break;
+        const uint32_t w = *patch_word(patch, r, lane), next = __shfl_down_sync(0xffffffffu, w, 1);
+        uint16_t* to = base + r * ld;
+        if ((reinterpret_cast<uintptr_t>(to) & 2) == 0) {
+            if (2 * lane + 1 < cols)
+                *reinterpret_cast<uint32_t*>(to + 2 * lane) = w;
+            else if (2 * lane < cols)
+                to[2 * lane] = (uint16_t)w;
+        } else {
+            if (lane == 0) to[0] = (uint16_t)w;
+            if (lane < 31 && 2 * lane + 2 < cols)
+                *reinterpret_cast<uint32_t*>(to + 2 * lane + 1) = __funnelshift_r(w, next, 16);
+            else if (2 * lane + 1 < cols)
+                to[2 * lane + 1] = (uint16_t)(w >> 16);
+        }
+    }
     __syncwarp();
-    const int col = n + lane;
-    if (col >= ep.n) return;
-    const int rows = min(32, ep.m - row0);
-#pragma unroll 4
-    for (int r = 0; r < rows; ++r) {
-        const int64_t m = row0 + r;
-        float z = cell[r * 32 + (lane ^ r)];
-        if (ep.residual != nullptr) z += load16(ep.residual, m * ep.residual_ld + col, bf16);
-        if (ep.pre != nullptr) store16(ep.pre, m * ep.pre_ld + col, z, bf16);
-        store16(ep.out, m * ep.out_ld + col, act_value<true>(z, ep.activation), bf16);
+}
+__device__ __forceinline__ void read_ragged(const void* from, int64_t ld, uint8_t* patch, int n, int row0, int rows,
+                                            int cols, int lane) {
+    const uint16_t* base = static_cast<const uint16_t*>(from) + row0 * ld + n + 2 * lane;
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+        const uint32_t lo = r < rows && 2 * lane < cols ? __ldg(base + r * ld) : 0u;
+        const uint32_t hi = r < rows && 2 * lane + 1 < cols ? __ldg(base + r * ld + 1) : 0u;
+        *patch_word(patch, r, lane) = lo | hi << 16;
     }
 }
 
@@ -612,8 +631,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             for (int c = 0; c < BN / 2; c += 64) {
                 const bool in = row0 < ep.m && n0 + c < ep.n;
                 uint4 held[8];
-                const bool residual = in && ep.aligned && ep.residual != nullptr;
-                if (residual) {  // eight lanes a row of 128 bytes, in flight while TMEM is read
+                const bool wide = in && ep.residual != nullptr && ep.residual_wide;
+                if (wide) {  // eight lanes a row of 128 bytes, in flight while TMEM is read
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int row = row0 + i * 4 + (lane >> 3), col = n0 + c + (lane & 7) * 8;
@@ -631,19 +650,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     if (lane == 0) arrive_at(cluster_address(smem_u32(&acc_empty[a]), 0));
                 }
                 if (!in) continue;
+                const int rows = min(32, ep.m - row0), cols = min(64, ep.n - n0 - c);
                 if (ep.bias != nullptr) {
                     add_bias(ep, n0 + c, v0, bf16);
                     add_bias(ep, n0 + c + 32, v1, bf16);
                 }
-                if (!ep.aligned) {
-                    finish_ragged(ep, v0, row0, lane, n0 + c, patch);
-                    if (n0 + c + 32 < ep.n) finish_ragged(ep, v1, row0, lane, n0 + c + 32, patch);
-                    continue;
-                }
                 patch_free(lane);
-                if (residual) {
+                if (ep.residual != nullptr) {
+                    if (wide) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) *patch_chunk(patch, i * 4 + (lane >> 3), lane & 7) = held[i];
+                        for (int i = 0; i < 8; ++i) *patch_chunk(patch, i * 4 + (lane >> 3), lane & 7) = held[i];
+                    } else {
+                        read_ragged(ep.residual, ep.residual_ld, patch, n0 + c, row0, rows, cols, lane);
+                    }
                     __syncwarp();
                     add_row(patch, lane, 0, v0, bf16);
                     add_row(patch, lane, 1, v1, bf16);
@@ -651,17 +670,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 if (ep.pre != nullptr) {  // each lane has read its row of the residual and writes the same row
                     put_row(patch, lane, 0, v0, bf16);
                     put_row(patch, lane, 1, v1, bf16);
-                    store_patch(&t_pre, patch, n0 + c, row0, lane);
-                    activate(v0, ep.activation);
-                    activate(v1, ep.activation);
-                    patch_free(lane);
-                } else {
-                    activate(v0, ep.activation);
-                    activate(v1, ep.activation);
+                    if (ep.pre_wide)
+                        store_patch(&t_pre, patch, n0 + c, row0, lane);
+                    else
+                        write_ragged(ep.pre, ep.pre_ld, patch, n0 + c, row0, rows, cols, lane);
                 }
+                activate(v0, ep.activation);
+                activate(v1, ep.activation);
+                patch_free(lane);
                 put_row(patch, lane, 0, v0, bf16);
                 put_row(patch, lane, 1, v1, bf16);
-                store_patch(&t_out, patch, n0 + c, row0, lane);
+                if (ep.out_wide)
+                    store_patch(&t_out, patch, n0 + c, row0, lane);
+                else
+                    write_ragged(ep.out, ep.out_ld, patch, n0 + c, row0, rows, cols, lane);
             }
         }
         if (lane == 0) bulk_wait<0>();  // the stores are done before the block ends
@@ -709,10 +731,11 @@ bool encode(CUtensorMap* map, const void* p, int64_t ld, int across, int64_t mn,
 
 Epilogue epilogue_of(const GemmArgs& g) {
     Epilogue e{g.out, g.bias, g.residual, g.pre, g.out_ld, g.residual_ld, g.pre_ld, (int)g.m, (int)g.n,
-               g.activation, g.dtype == GK_BF16, 0};
-    e.aligned = aligned16(g.out) && (g.bias == nullptr || aligned16(g.bias)) && g.out_ld % 8 == 0 &&
-                (g.residual == nullptr || (aligned16(g.residual) && g.residual_ld % 8 == 0)) &&
-                (g.pre == nullptr || (aligned16(g.pre) && g.pre_ld % 8 == 0));
+               g.activation, g.dtype == GK_BF16, 0, 0, 0, 0};
+    e.out_wide = aligned16(g.out) && g.out_ld % 8 == 0;
+    e.pre_wide = aligned16(g.pre) && g.pre_ld % 8 == 0;
+    e.residual_wide = aligned16(g.residual) && g.residual_ld % 8 == 0;
+    e.bias_wide = aligned16(g.bias);
     return e;
 }
 
@@ -769,8 +792,8 @@ int launch_pair(const GemmArgs& g, uint32_t* status, cudaStream_t stream) {
         !encode(&tb, g.b, g.b_ld, g.b_across, g.n, g.k, BN / 2, g.dtype))
         return GK_EINVAL;
     // The outputs as [m, n] with n contiguous, in boxes of 64 columns by 32 rows.
-    if (ep.aligned && (!encode(&t_out, g.out, g.out_ld, 0, g.m, g.n, 32, g.dtype) ||
-                       (g.pre != nullptr && !encode(&t_pre, g.pre, g.pre_ld, 0, g.m, g.n, 32, g.dtype))))
+    if ((ep.out_wide && !encode(&t_out, g.out, g.out_ld, 0, g.m, g.n, 32, g.dtype)) ||
+        (g.pre != nullptr && ep.pre_wide && !encode(&t_pre, g.pre, g.pre_ld, 0, g.m, g.n, 32, g.dtype)))
         return GK_EINVAL;
     const int64_t tiles_m = (g.m + 255) / 256, tiles_n = (g.n + BN - 1) / BN;
     if (tiles_m * tiles_n >= (1ll << 31) - kSmCount) return GK_EINVAL;

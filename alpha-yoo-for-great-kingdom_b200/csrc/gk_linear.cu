@@ -36,7 +36,7 @@ struct FewRows {
     const void* residual;
     void* y;
     void* pre;
-    int64_t x_stride, w_stride, residual_stride;
+    int64_t x_stride, w_stride, residual_stride, pre_stride;
     int m, n;
     int64_t k;
     int activation;
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) linear_few_kernel(FewRows p) {
         for (int q = 0; q < p.k_parts; ++q) v += parts[t * p.k_parts + q][r * M + m];
         if (p.bias != nullptr) v += as_float<T>(static_cast<const T*>(p.bias)[n]);
         if (p.residual != nullptr) v += as_float<T>(static_cast<const T*>(p.residual)[m * p.residual_stride + n]);
-        if (p.pre != nullptr) static_cast<T*>(p.pre)[(int64_t)m * p.n + n] = rounded<T>(v);
+        if (p.pre != nullptr) static_cast<T*>(p.pre)[m * p.pre_stride + n] = rounded<T>(v);
         static_cast<T*>(p.y)[(int64_t)m * p.n + n] = rounded<T>(act_value<sizeof(T) == 2>(v, p.activation));
     }
 }
@@ -415,10 +415,10 @@ int gemm32(Gemm32 g, cudaStream_t s) {
 
 struct Slope {
     const void* dy;
-    const void* kept;  // [m, n] contiguous; unused without activation
+    const void* kept;  // [m, n]; unused without activation
     void* dz;          // or nullptr: sums only
     float* sums;       // [slabs, n] column sums of each slab of rows, or nullptr
-    int64_t dy_stride, dz_stride;
+    int64_t dy_stride, kept_stride, dz_stride;
     int64_t m, n, slab;  // rows of a slab
     int activation;
 };
@@ -452,10 +452,10 @@ __global__ void __launch_bounds__(256, 3) linear_slope_kernel(Slope p, int acros
                 if constexpr (V > 1) {
                     *reinterpret_cast<uint4*>(dy[u]) = __ldcs(reinterpret_cast<const uint4*>(dyp + row * p.dy_stride));
                     if constexpr (kSlope)
-                        *reinterpret_cast<uint4*>(kept[u]) = __ldcs(reinterpret_cast<const uint4*>(keptp + row * p.n));
+                        *reinterpret_cast<uint4*>(kept[u]) = __ldcs(reinterpret_cast<const uint4*>(keptp + row * p.kept_stride));
                 } else {
                     dy[u][0] = dyp[row * p.dy_stride];
-                    if constexpr (kSlope) kept[u][0] = keptp[row * p.n];
+                    if constexpr (kSlope) kept[u][0] = keptp[row * p.kept_stride];
                 }
             }
 #pragma unroll
@@ -638,7 +638,8 @@ bool forward_ok(const gk_linear_t* p) {
     if (p == nullptr || !sizes_ok(p->m, p->n, p->k, p->dtype, p->activation)) return false;
     if (p->m == 0) return true;
     return p->x != nullptr && p->w != nullptr && p->y != nullptr && p->x_stride >= 0 && p->w_stride >= 0 &&
-           (p->residual == nullptr || p->residual_stride >= 0);
+           (p->residual == nullptr || p->residual_stride >= 0) &&
+           (p->pre == nullptr || p->pre_stride >= p->n);
 }
 
 struct BackwardPlan {
@@ -682,7 +683,7 @@ BackwardPlan backward_plan(const gk_linear_grad_t& p, void* workspace) {
     if (b.unpacked_ld > 0) b.x = {b.unpacked, b.unpacked_ld, false};
     b.runs_slope = b.forms_dz || p.db != nullptr;
     const bool vec = aligned16(p.dy) && p.dy_stride % kVec<T> == 0 && p.n % kVec<T> == 0 &&
-                     (p.kept == nullptr || aligned16(p.kept)) && (p.dz == nullptr || aligned16(p.dz));
+                     (p.kept == nullptr || (aligned16(p.kept) && p.kept_stride % kVec<T> == 0)) && (p.dz == nullptr || aligned16(p.dz));
     b.slope = slope_plan<T>(p.m, p.n, vec);
     if (p.db != nullptr) b.sums = static_cast<float*>(arena.take((int64_t)b.slope.slabs * p.n * 4));
     b.bytes = arena.used;
@@ -692,7 +693,7 @@ BackwardPlan backward_plan(const gk_linear_grad_t& p, void* workspace) {
 bool backward_ok(const gk_linear_grad_t* p) {
     if (p == nullptr || !sizes_ok(p->m, p->n, p->k, p->dtype, p->activation) || p->m < 1) return false;
     if (p->dy == nullptr || p->dy_stride < 0) return false;
-    if (p->activation != GK_ACT_NONE && p->kept == nullptr) return false;
+    if (p->activation != GK_ACT_NONE && (p->kept == nullptr || p->kept_stride < 0)) return false;
     if (p->activation == GK_ACT_NONE && p->dz != nullptr) return false;
     if (p->dx != nullptr && (p->w == nullptr || p->w_stride < 0)) return false;
     if (p->dw != nullptr && p->x == nullptr && (p->x_codes == nullptr || p->x_scales == nullptr)) return false;
@@ -706,7 +707,7 @@ int backward(const gk_linear_grad_t& p, void* workspace, uint32_t* status, cudaS
     int e = 0;
     if (b.runs_slope) {
         Slope a{p.dy, p.activation == GK_ACT_NONE ? nullptr : p.kept,
-                b.forms_dz ? const_cast<void*>(b.dz.p) : nullptr, b.sums, p.dy_stride, b.dz.ld, p.m, p.n,
+                b.forms_dz ? const_cast<void*>(b.dz.p) : nullptr, b.sums, p.dy_stride, p.kept_stride, b.dz.ld, p.m, p.n,
                 b.slope.slab, p.activation};
         const dim3 grid((unsigned)b.slope.col_blocks, (unsigned)b.slope.slabs);
         if ((e = launch_slope<T>(a, grid, b.slope, s)) != 0) return e;
@@ -773,7 +774,7 @@ int gk_linear_forward(const gk_linear_t* p, void* workspace, uint32_t* status, v
     cudaStream_t s = as_stream(stream);
     if (f.few) {
         FewRows r{p->x, p->w, p->bias, p->residual, p->y, p->pre, p->x_stride, p->w_stride, p->residual_stride,
-                  (int)p->m, (int)p->n, p->k, p->activation, 1};
+                  p->pre_stride, (int)p->m, (int)p->n, p->k, p->activation, 1};
         if (p->dtype == GK_FP32) return few_rows_by_m<float>(r, s);
         if (p->dtype == GK_BF16) return few_rows_by_m<__nv_bfloat16>(r, s);
         return few_rows_by_m<__half>(r, s);
@@ -781,15 +782,15 @@ int gk_linear_forward(const gk_linear_t* p, void* workspace, uint32_t* status, v
     if (p->dtype == GK_FP32) {
         Gemm32 g{static_cast<const float*>(p->x), static_cast<const float*>(p->w), p->x_stride, p->w_stride,
                  static_cast<float*>(p->y), static_cast<const float*>(p->bias),
-                 static_cast<const float*>(p->residual), static_cast<float*>(p->pre), p->n, p->residual_stride, p->n,
-                 p->m, p->n, p->k, p->activation, 0};
+                 static_cast<const float*>(p->residual), static_cast<float*>(p->pre), p->n, p->residual_stride,
+                 p->pre_stride,                 p->m, p->n, p->k, p->activation, 0};
         return gemm32<true, true>(g, s);
     }
     int e = copy_if_needed(f.x, p->x, p->x_stride, p->m, p->k, s);
     if (e == 0) e = copy_if_needed(f.w, p->w, p->w_stride, p->n, p->k, s);
     if (e != 0) return e;
-    GemmArgs g{f.x.p, f.w.p, f.x.ld, f.w.ld, 0, 0, p->y, p->n, p->bias, p->residual, p->residual_stride, p->pre, p->n,
-               p->m, p->n, p->k, p->dtype, p->activation};
+    GemmArgs g{f.x.p, f.w.p, f.x.ld, f.w.ld, 0, 0, p->y, p->n, p->bias, p->residual, p->residual_stride, p->pre,
+               p->pre_stride, p->m, p->n, p->k, p->dtype, p->activation};
     return gemm16(g, status, s);
 }
 

@@ -135,7 +135,8 @@ std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, cons
     const int64_t m = x.size(0), k = x.size(1), n = w.size(0);
     const auto options = x.options().requires_grad(false);
     Tensor y = at::empty({m, n}, options), pre;
-    if (keep_sum) pre = at::empty({m, n}, options);
+    // Its rows start on 16 bytes whatever n is: it is written and read in whole vectors.
+    if (keep_sum) pre = at::empty({m, (n + 7) / 8 * 8}, options).narrow(1, 0, n);
     if (m == 0) return {y, pre};
     gk_linear_t p{};
     p.x = x.data_ptr(), p.w = w.data_ptr(), p.bias = data(bias), p.residual = data(residual);
@@ -143,6 +144,7 @@ std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, cons
     p.m = m, p.n = n, p.k = k;
     p.x_stride = row_stride(x, k), p.w_stride = row_stride(w, k);
     p.residual_stride = has(residual) ? row_stride(*residual, n) : 0;
+    p.pre_stride = pre.defined() ? pre.stride(0) : 0;
     p.dtype = type_of(x.scalar_type());
     p.activation = (int)activation;
     const c10::cuda::CUDAGuard guard(x.device());
@@ -199,6 +201,7 @@ struct Linear : torch::autograd::Function<Linear> {
                 p.dz = activation == GK_ACT_NONE ? nullptr : data(dr);
                 p.m = m, p.n = n, p.k = k;
                 p.dy_stride = row_stride(dy, n);
+                p.kept_stride = saved[2].defined() ? saved[2].stride(0) : 0;
                 p.x_stride = saved[0].defined() ? row_stride(saved[0], k) : 0;
                 p.w_stride = saved[1].defined() ? row_stride(saved[1], k) : 0;
                 p.dtype = type_of(dy.scalar_type());

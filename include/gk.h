@@ -602,9 +602,9 @@ typedef struct {
     const void* bias;        /* [n] or NULL */
     const void* residual;    /* [m, n] or NULL */
     void* y;                 /* [m, n], contiguous */
-    void* pre;               /* [m, n], contiguous: the sum before the activation; or NULL */
+    void* pre;               /* [m, n]: the sum before the activation; or NULL */
     int64_t m, n, k;
-    int64_t x_stride, w_stride, residual_stride; /* elements between rows */
+    int64_t x_stride, w_stride, residual_stride, pre_stride; /* elements between rows */
     int dtype;               /* GK_FP32, GK_BF16, GK_FP16 */
     int activation;
 } gk_linear_t;
@@ -615,7 +615,7 @@ typedef struct {
  * with ceil(k / 32) scales a row). */
 typedef struct {
     const void* dy;          /* [m, n] */
-    const void* kept;        /* [m, n], contiguous; or NULL */
+    const void* kept;        /* [m, n]; or NULL */
     const void* x;           /* [m, k]; or NULL */
     const uint8_t* x_codes;
     const uint8_t* x_scales;
@@ -625,7 +625,7 @@ typedef struct {
     void* db;                /* [n] */
     void* dz;                /* [m, n], contiguous: the residual's gradient; or NULL (always NULL without activation) */
     int64_t m, n, k;
-    int64_t dy_stride, x_stride, w_stride;
+    int64_t dy_stride, kept_stride, x_stride, w_stride;
     int dtype;
     int activation;
 } gk_linear_grad_t;

@@ -60,13 +60,14 @@ class PolicyLossStruct(ctypes.Structure):
 class LinearStruct(ctypes.Structure):
     _fields_ = [("x", c_void_p), ("w", c_void_p), ("bias", c_void_p), ("residual", c_void_p), ("y", c_void_p),
                 ("pre", c_void_p), ("m", c_int64), ("n", c_int64), ("k", c_int64), ("x_stride", c_int64),
-                ("w_stride", c_int64), ("residual_stride", c_int64), ("dtype", c_int), ("activation", c_int)]
+                ("w_stride", c_int64), ("residual_stride", c_int64),
+                ("pre_stride", c_int64), ("dtype", c_int), ("activation", c_int)]
 
 
 class LinearGradStruct(ctypes.Structure):
     _fields_ = [("dy", c_void_p), ("kept", c_void_p), ("x", c_void_p), ("x_codes", c_void_p), ("x_scales", c_void_p),
                 ("w", c_void_p), ("dx", c_void_p), ("dw", c_void_p), ("db", c_void_p), ("dz", c_void_p),
-                ("m", c_int64), ("n", c_int64), ("k", c_int64), ("dy_stride", c_int64), ("x_stride", c_int64),
+                ("m", c_int64), ("n", c_int64), ("k", c_int64), ("dy_stride", c_int64), ("kept_stride", c_int64), ("x_stride", c_int64),
                 ("w_stride", c_int64), ("dtype", c_int), ("activation", c_int)]
 
 
@@ -99,7 +100,8 @@ def linear_struct(**changes):
 
 @pytest.mark.parametrize("changes", [dict(n=0), dict(k=0), dict(m=-1), dict(dtype=3), dict(dtype=-1),
                                      dict(activation=5), dict(activation=-1), dict(x=None), dict(w=None),
-                                     dict(y=None), dict(k=1 << 31), dict(x_stride=-16)])
+                                     dict(y=None), dict(k=1 << 31), dict(x_stride=-16),
+                                     dict(pre=1 << 20, pre_stride=7)])
 def test_linear_entry_refuses(changes):
     lib = library()
     status = ctypes.c_void_p(1 << 20)
@@ -130,7 +132,7 @@ def test_linear_backward_entry_refuses():
         return ctypes.byref(p)
 
     for changes in (dict(m=0), dict(n=0), dict(k=0), dict(dy=None), dict(kept=None), dict(w=None), dict(x=None),
-                    dict(x=None, x_codes=1 << 20), dict(activation=9), dict(dtype=7), dict(dy_stride=-1),
+                    dict(x=None, x_codes=1 << 20), dict(activation=9), dict(dtype=7), dict(dy_stride=-1), dict(kept_stride=-1),
                     dict(activation=0, dz=1 << 20)):
         assert lib.gk_linear_backward(struct(**changes), None, status, None) == EINVAL, changes
     assert lib.gk_linear_backward(struct(), None, status, None) == EINVAL  # dz needs a workspace
