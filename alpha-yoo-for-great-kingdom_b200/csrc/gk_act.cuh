@@ -58,8 +58,9 @@ __device__ __forceinline__ float act_value(float z, int act) {
     }
 }
 
-// The derivative. relu and tanh take the output y, gelu and silu the sum z
-// before the activation: the value that the forward pass kept for them.
+// The derivative, from what the forward pass kept: relu takes the output y,
+// tanh its value in fp32 (1 - y^2 of a rounded y near one has few right bits),
+// gelu and silu the sum z before the activation.
 template <bool QUICK>
 __device__ __forceinline__ float act_slope(float kept, int act) {
     switch (act) {

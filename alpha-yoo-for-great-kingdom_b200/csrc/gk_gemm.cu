@@ -220,7 +220,8 @@ __device__ __forceinline__ void finish4(const Epilogue& ep, int64_t m, int n, fl
                 if (j < count) v[j] += load16(ep.residual, m * ep.residual_ld + n + j, bf16);
         }
     }
-    if (ep.pre != nullptr) {
+    const bool tanh32 = ep.activation == GK_ACT_TANH;  // keeps its fp32 value, not the sum
+    if (ep.pre != nullptr && !tanh32) {
         if (whole && ep.pre_wide) {
             *reinterpret_cast<uint2*>(static_cast<uint16_t*>(ep.pre) + m * ep.pre_ld + n) =
                 make_uint2(pack16(v[0], v[1], bf16), pack16(v[2], v[3], bf16));
@@ -233,6 +234,12 @@ __device__ __forceinline__ void finish4(const Epilogue& ep, int64_t m, int n, fl
     if (ep.activation != GK_ACT_NONE) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = act_value<true>(v[j], ep.activation);
+    }
+    if (ep.pre != nullptr && tanh32) {
+        float* kept = static_cast<float*>(ep.pre) + m * ep.pre_ld + n;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < count) kept[j] = v[j];
     }
     if (whole && ep.out_wide) {
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(ep.out) + m * ep.out_ld + n) =
@@ -517,6 +524,11 @@ __device__ __forceinline__ void write_ragged(void* out, int64_t ld, uint8_t* pat
     }
     __syncwarp();
 }
+__device__ __forceinline__ void keep_row(float* to, int cols, const float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        if (i < cols) to[i] = v[i];
+}
 __device__ __forceinline__ void read_ragged(const void* from, int64_t ld, uint8_t* patch, int n, int row0, int rows,
                                             int cols, int lane) {
     const uint16_t* base = static_cast<const uint16_t*>(from) + row0 * ld + n + 2 * lane;
@@ -616,7 +628,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     } else if (warp >= 4) {
         const int quadrant = warp & 3, half = (warp - 4) >> 2;
         uint8_t* patch = base + P::kStages * P::kStage + (warp - 4) * P::kPatch;
-        const bool bf16 = ep.bf16 != 0;
+        const bool bf16 = ep.bf16 != 0, tanh32 = ep.activation == GK_ACT_TANH;  // tanh keeps its fp32 value
         int n = 0;
         for (int t = pair; t < tiles; t += pairs, ++n) {
             const int a = n & 1, use = n >> 1;
@@ -667,7 +679,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     add_row(patch, lane, 0, v0, bf16);
                     add_row(patch, lane, 1, v1, bf16);
                 }
-                if (ep.pre != nullptr) {  // each lane has read its row of the residual and writes the same row
+                if (ep.pre != nullptr && !tanh32) {  // each lane has read its row of the residual and writes the same row
                     put_row(patch, lane, 0, v0, bf16);
                     put_row(patch, lane, 1, v1, bf16);
                     if (ep.pre_wide)
@@ -677,6 +689,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 }
                 activate(v0, ep.activation);
                 activate(v1, ep.activation);
+                if (ep.pre != nullptr && tanh32 && lane < rows) {
+                    float* kept = static_cast<float*>(ep.pre) + (row0 + lane) * ep.pre_ld + n0 + c;
+                    keep_row(kept, cols, v0);
+                    keep_row(kept + 32, cols - 32, v1);
+                }
                 patch_free(lane);
                 put_row(patch, lane, 0, v0, bf16);
                 put_row(patch, lane, 1, v1, bf16);
@@ -793,7 +810,7 @@ int launch_pair(const GemmArgs& g, uint32_t* status, cudaStream_t stream) {
         return GK_EINVAL;
     // The outputs as [m, n] with n contiguous, in boxes of 64 columns by 32 rows.
     if ((ep.out_wide && !encode(&t_out, g.out, g.out_ld, 0, g.m, g.n, 32, g.dtype)) ||
-        (g.pre != nullptr && ep.pre_wide && !encode(&t_pre, g.pre, g.pre_ld, 0, g.m, g.n, 32, g.dtype)))
+        (g.pre != nullptr && ep.pre_wide && g.activation != GK_ACT_TANH && !encode(&t_pre, g.pre, g.pre_ld, 0, g.m, g.n, 32, g.dtype)))
         return GK_EINVAL;
     const int64_t tiles_m = (g.m + 255) / 256, tiles_n = (g.n + BN - 1) / BN;
     if (tiles_m * tiles_n >= (1ll << 31) - kSmCount) return GK_EINVAL;

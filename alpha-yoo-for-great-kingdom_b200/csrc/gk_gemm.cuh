@@ -22,7 +22,7 @@ struct GemmArgs {
     const void* bias;      // or nullptr
     const void* residual;  // or nullptr
     int64_t residual_ld;
-    void* pre;             // the sum before the activation, or nullptr
+    void* pre;             // the sum before the activation (tanh: its value in fp32), or nullptr
     int64_t pre_ld;
     int64_t m, n, k;       // each below 2^31, k >= 1
     int dtype;             // GK_BF16 or GK_FP16

@@ -105,8 +105,14 @@ __global__ void __launch_bounds__(256) linear_few_kernel(FewRows p) {
         for (int q = 0; q < p.k_parts; ++q) v += parts[t * p.k_parts + q][r * M + m];
         if (p.bias != nullptr) v += as_float<T>(static_cast<const T*>(p.bias)[n]);
         if (p.residual != nullptr) v += as_float<T>(static_cast<const T*>(p.residual)[m * p.residual_stride + n]);
-        if (p.pre != nullptr) static_cast<T*>(p.pre)[m * p.pre_stride + n] = rounded<T>(v);
-        static_cast<T*>(p.y)[(int64_t)m * p.n + n] = rounded<T>(act_value<sizeof(T) == 2>(v, p.activation));
+        const float y = act_value<sizeof(T) == 2>(v, p.activation);
+        if (p.pre != nullptr) {
+            if (p.activation == GK_ACT_TANH)
+                static_cast<float*>(p.pre)[m * p.pre_stride + n] = y;
+            else
+                static_cast<T*>(p.pre)[m * p.pre_stride + n] = rounded<T>(v);
+        }
+        static_cast<T*>(p.y)[(int64_t)m * p.n + n] = rounded<T>(y);
     }
 }
 
@@ -251,19 +257,22 @@ __device__ __forceinline__ void finish4(const Gemm32& g, int64_t m, int64_t n, f
     }
     float* pre = g.pre == nullptr ? nullptr : g.pre + m * g.pre_ld + n;
     float* out = g.out + m * g.out_ld + n;
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = g.activation == GK_ACT_NONE ? v[j] : act_value<false>(v[j], g.activation);
+    if (g.activation == GK_ACT_TANH) {  // keeps its value, not the sum
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = y[j];
+    }
     if (whole) {
         if (pre != nullptr) *reinterpret_cast<float4*>(pre) = make_float4(v[0], v[1], v[2], v[3]);
-        if (g.activation != GK_ACT_NONE) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = act_value<false>(v[j], g.activation);
-        }
-        *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(out) = make_float4(y[0], y[1], y[2], y[3]);
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (j >= count) break;
             if (pre != nullptr) pre[j] = v[j];
-            out[j] = g.activation == GK_ACT_NONE ? v[j] : act_value<false>(v[j], g.activation);
+            out[j] = y[j];
         }
     }
 }
@@ -429,6 +438,7 @@ struct Slope {
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(256, 3) linear_slope_kernel(Slope p, int across) {
     constexpr bool kSlope = ACT != GK_ACT_NONE;
+    using K = typename std::conditional<ACT == GK_ACT_TANH, float, T>::type;  // tanh keeps fp32
     __shared__ float sums[8][32 * V];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int side = warp % across, down = warp / across, step = 8 / across;
@@ -440,19 +450,24 @@ __global__ void __launch_bounds__(256, 3) linear_slope_kernel(Slope p, int acros
     for (int i = 0; i < V; ++i) sum[i] = 0.0f;
     if (c < p.n) {
         const T* dyp = static_cast<const T*>(p.dy) + c;
-        const T* keptp = static_cast<const T*>(p.kept) + c;
+        const K* keptp = static_cast<const K*>(p.kept) + c;
         T* dzp = static_cast<T*>(p.dz) + c;
         constexpr int U = 4;  // rows in flight
         for (int64_t r = r0 + down; r < r1; r += U * step) {
-            alignas(16) T dy[U][V], kept[U][V];
+            alignas(16) T dy[U][V];
+            alignas(16) K kept[U][V];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int64_t row = r + u * step;
                 if (row >= r1) continue;
                 if constexpr (V > 1) {
                     *reinterpret_cast<uint4*>(dy[u]) = __ldcs(reinterpret_cast<const uint4*>(dyp + row * p.dy_stride));
-                    if constexpr (kSlope)
-                        *reinterpret_cast<uint4*>(kept[u]) = __ldcs(reinterpret_cast<const uint4*>(keptp + row * p.kept_stride));
+                    if constexpr (kSlope) {
+#pragma unroll
+                        for (int i = 0; i < (int)(V * sizeof(K) / 16); ++i)
+                            reinterpret_cast<uint4*>(kept[u])[i] =
+                                __ldcs(reinterpret_cast<const uint4*>(keptp + row * p.kept_stride) + i);
+                    }
                 } else {
                     dy[u][0] = dyp[row * p.dy_stride];
                     if constexpr (kSlope) kept[u][0] = keptp[row * p.kept_stride];
@@ -466,7 +481,7 @@ __global__ void __launch_bounds__(256, 3) linear_slope_kernel(Slope p, int acros
                 for (int i = 0; i < V; ++i) {
                     float z = as_float<T>(dy[u][i]);
                     if constexpr (kSlope) {
-                        z *= act_slope<sizeof(T) == 2>(as_float<T>(kept[u][i]), ACT);
+                        z *= act_slope<sizeof(T) == 2>(as_float<K>(kept[u][i]), ACT);
                         dy[u][i] = rounded<T>(z);
                     }
                     sum[i] += z;

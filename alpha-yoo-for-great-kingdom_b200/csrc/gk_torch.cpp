@@ -128,7 +128,7 @@ Tensor unpack(const Tensor& codes, const Tensor& scales, at::IntArrayRef shape, 
 
 // ---------------------------------------------------------------- linear
 
-// y and, if asked for, the sum before the activation.
+// y and, if asked for, what the derivative takes: the sum before the activation, or tanh in fp32.
 std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, const OptTensor& bias,
                                           const OptTensor& residual, int64_t activation, bool keep_sum,
                                           const Tensor& status) {
@@ -136,7 +136,9 @@ std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, cons
     const auto options = x.options().requires_grad(false);
     Tensor y = at::empty({m, n}, options), pre;
     // Its rows start on 16 bytes whatever n is: it is written and read in whole vectors.
-    if (keep_sum) pre = at::empty({m, (n + 7) / 8 * 8}, options).narrow(1, 0, n);
+    if (keep_sum)
+        pre = at::empty({m, (n + 7) / 8 * 8}, activation == GK_ACT_TANH ? options.dtype(at::kFloat) : options)
+                  .narrow(1, 0, n);
     if (m == 0) return {y, pre};
     gk_linear_t p{};
     p.x = x.data_ptr(), p.w = w.data_ptr(), p.bias = data(bias), p.residual = data(residual);
@@ -165,7 +167,9 @@ struct Linear : torch::autograd::Function<Linear> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias,
                           const OptTensor& residual, int64_t activation, bool packed, const Tensor& status) {
         auto [y, pre] = linear_forward(x, w, bias, residual, activation,
-                                       activation == GK_ACT_GELU || activation == GK_ACT_SILU, status);
+                                       activation == GK_ACT_GELU || activation == GK_ACT_SILU ||
+                                           (activation == GK_ACT_TANH && x.scalar_type() != at::kFloat),
+                                       status);
         const int64_t m = x.size(0), k = x.size(1);
         const bool need_x = x.requires_grad(), need_w = w.requires_grad();
         Tensor codes, scales;

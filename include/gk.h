@@ -602,15 +602,15 @@ typedef struct {
     const void* bias;        /* [n] or NULL */
     const void* residual;    /* [m, n] or NULL */
     void* y;                 /* [m, n], contiguous */
-    void* pre;               /* [m, n]: the sum before the activation; or NULL */
+    void* pre;               /* [m, n]: the sum before the activation; for tanh its value in fp32; or NULL */
     int64_t m, n, k;
     int64_t x_stride, w_stride, residual_stride, pre_stride; /* elements between rows */
     int dtype;               /* GK_FP32, GK_BF16, GK_FP16 */
     int activation;
 } gk_linear_t;
 
-/* Its gradients from dy. dz = dy act'(.) is formed from `kept`: y for relu and
- * tanh, `pre` for gelu and silu, unused without an activation. dx, dw, db may
+/* Its gradients from dy. dz = dy act'(.) is formed from `kept`: y for relu,
+ * `pre` for tanh, gelu and silu, unused without an activation. dx, dw, db may
  * be NULL. x is given as it is or packed by gk_pack (x_codes, x_scales: [m, k]
  * with ceil(k / 32) scales a row). */
 typedef struct {

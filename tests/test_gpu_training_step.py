@@ -161,7 +161,7 @@ def test_captured_step_updates_the_weights(batch):
     torch.cuda.synchronize()
     for a, b in zip(eager.parameters(), model.parameters()):
         # Three updates of at most 0.05 |g|; cuDNN may pick another algorithm under capture.
-        assert float((a - b).abs().max()) <= 1e-3 * (1 + float(a.abs().max()))
+        assert float((a - b).abs().max().detach()) <= 1e-3 * (1 + float(a.abs().max().detach()))
 
 
 def test_refusals(batch):
