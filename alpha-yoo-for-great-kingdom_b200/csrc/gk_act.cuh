@@ -67,15 +67,16 @@ __device__ __forceinline__ float act_slope(float kept, int act) {
         case GK_ACT_RELU: return kept > 0.0f ? 1.0f : 0.0f;
         case GK_ACT_TANH: return 1.0f - kept * kept;
         case GK_ACT_GELU: {
-            if (kept != kept) return kept;
-            // Far out z e^(-z^2/2) is 0, but inf * 0 is not.
+            // Far out z e^(-z^2/2) is 0, but inf * 0 is not; the clamp drops a NaN, which is added again.
             const float z = fminf(fmaxf(kept, -32.0f), 32.0f);
+            const float not_a_number = kept != kept ? kept : 0.0f;
             if (QUICK) {
                 float e;
                 const float cdf = quick_cdf(z, e);
-                return fmaf(z * 0.39894228040143268f, e, cdf);
+                return fmaf(z * 0.39894228040143268f, e, cdf) + not_a_number;
             }
-            return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+            return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f +
+                   not_a_number;
         }
         case GK_ACT_SILU: {
             const float s = QUICK ? quick_rcp(1.0f + quick_ex2(kept * -1.4426950408889634f))

@@ -436,7 +436,7 @@ struct Slope {
 // eight warps lie side by side (whole lines of a row next to one another), the
 // others take rows in turn.
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(256, 3) linear_slope_kernel(Slope p, int across) {
+__global__ void __launch_bounds__(256, 4) linear_slope_kernel(Slope p, int across) {
     constexpr bool kSlope = ACT != GK_ACT_NONE;
     using K = typename std::conditional<ACT == GK_ACT_TANH, float, T>::type;  // tanh keeps fp32
     __shared__ float sums[8][32 * V];
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(256, 3) linear_slope_kernel(Slope p, int acros
         const T* dyp = static_cast<const T*>(p.dy) + c;
         const K* keptp = static_cast<const K*>(p.kept) + c;
         T* dzp = static_cast<T*>(p.dz) + c;
-        constexpr int U = 4;  // rows in flight
+        constexpr int U = 2;  // rows in flight
         for (int64_t r = r0 + down; r < r1; r += U * step) {
             alignas(16) T dy[U][V];
             alignas(16) K kept[U][V];
@@ -540,8 +540,8 @@ SlopePlan slope_plan(int64_t m, int64_t n, bool vec) {
     p.across = 1;
     while (p.across < 8 && (int64_t)p.across * 32 * p.vec < n) p.across *= 2;
     p.col_blocks = (n + 32 * p.vec * p.across - 1) / (32 * p.vec * p.across);
-    // One round of the three blocks that an SM holds, in slabs of 16 rows or more.
-    int64_t slabs = 3 * kSmCount / p.col_blocks;
+    // One round of the four blocks that an SM holds, in slabs of 16 rows or more.
+    int64_t slabs = 4 * kSmCount / p.col_blocks;
     if (slabs > (m + 15) / 16) slabs = (m + 15) / 16;
     if (slabs < 1) slabs = 1;
     p.slab = (m + slabs - 1) / slabs;

@@ -79,15 +79,18 @@ struct Exp {
         correct = fabsf(rest) < 1.0f ? ex2(-rest) : 1.0f;  // not a number for an infinite m
     }
     __device__ __forceinline__ float operator()(float x) const { return ex2(fmaf(x, scale, -offset)); }
+    __device__ __forceinline__ float term(float x) const { return (*this)(x); }  // of the sum
 };
 // fp32 logits: the difference first, which keeps the exponent's error at the
-// last bit of x - m.
+// last bit of x - m; in the row's sum, which every log-probability is taken
+// from, also without the small bias of the quick 2^x.
 template <>
 struct Exp<float> {
     float m;
     static constexpr float correct = 1.0f;
     __device__ __forceinline__ explicit Exp(float top) : m(top) {}
     __device__ __forceinline__ float operator()(float x) const { return ex2((x - m) * 1.4426950408889634f); }
+    __device__ __forceinline__ float term(float x) const { return expf(x - m); }
 };
 
 // Elements of one 16-byte vector of logits.
@@ -431,7 +434,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) policy_loss_rows_kernel(gk_pol
         float e[NPL], s = 0.0f;
 #pragma unroll
         for (int k = 0; k < NPL; ++k) {
-            e[k] = exp_m(x[k]);
+            e[k] = exp_m.term(x[k]);
             s += e[k];
         }
         s = warp_sum(s) * exp_m.correct;
@@ -584,7 +587,7 @@ __global__ void __launch_bounds__(THREADS, 3 * kLongThreads / THREADS) policy_lo
             float s2 = 0.0f;
             groups([&](const Group<TL, V>& h, int first, bool edge) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) (i & 1 ? s2 : acc.s) += e(h.x(i));
+                for (int i = 0; i < V; ++i) (i & 1 ? s2 : acc.s) += e.term(h.x(i));
                 if constexpr (kTarget) {
                     float t[V];
                     load_target<TT, V>(part.trow, h.legal, first, edge, t);
