@@ -110,6 +110,34 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const T* x, int64_t stri
     }
 }
 
+// The largest magnitude of a vector, with infinities and NaN; 16-bit values stay packed.
+template <typename T>
+__device__ __forceinline__ float vector_top(uint4 raw);
+template <>
+__device__ __forceinline__ float vector_top<float>(uint4 raw) {
+    // As bits, which order like the magnitudes and put NaN above infinity.
+    const uint32_t m = 0x7fffffffu;
+    return __uint_as_float(max(max(raw.x & m, raw.y & m), max(raw.z & m, raw.w & m)));
+}
+template <typename P>
+__device__ __forceinline__ P packed_top(uint4 raw) {
+    const uint32_t m = 0x7fff7fffu;
+    uint32_t w[4] = {raw.x & m, raw.y & m, raw.z & m, raw.w & m};
+    const P* v = reinterpret_cast<const P*>(w);
+    return __hmax2_nan(__hmax2_nan(v[0], v[1]), __hmax2_nan(v[2], v[3]));
+}
+__device__ __forceinline__ float greater_or_nan(float a, float b) { return a > b || a != a ? a : b; }
+template <>
+__device__ __forceinline__ float vector_top<__half>(uint4 raw) {
+    const float2 f = __half22float2(packed_top<__half2>(raw));
+    return greater_or_nan(f.x, f.y);
+}
+template <>
+__device__ __forceinline__ float vector_top<__nv_bfloat16>(uint4 raw) {
+    const float2 f = __bfloat1622float2(packed_top<__nv_bfloat162>(raw));
+    return greater_or_nan(f.x, f.y);
+}
+
 // Whole blocks of aligned rows: 16 bytes a thread, 32 * sizeof(T) / 16 threads
 // a block of 32, four vectors a thread in flight.
 template <typename T>
@@ -132,19 +160,39 @@ __global__ void __launch_bounds__(256) pack_vectors_kernel(const T* x, int64_t v
     for (int u = 0; u < kUnroll; ++u) {
         const int64_t i = start + u * 256;
         const T* v = reinterpret_cast<const T*>(&raw[u]);
-        float top = 0.0f;
+        float top = vector_top<T>(raw[u]);  // not finite if any value is not
 #pragma unroll
-        for (int k = 0; k < V; ++k) top = fmaxf(top, finite_magnitude(as_float<T>(v[k])));
-#pragma unroll
-        for (int o = kTeam / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
-        const int s = scale_exponent<T>(top);
-        const float inverse = power_of_two(-s);
+        for (int o = kTeam / 2; o; o >>= 1) {
+            const float other = __shfl_xor_sync(kFull, top, o);
+            top = other > top || other != other ? other : top;
+        }
         uint32_t word[V / 4];
+        int s;
+        if (top <= 3.4028234663852886e38f) {
+            s = scale_exponent<T>(top);
+            const float inverse = power_of_two(-s);
 #pragma unroll
-        for (int k = 0; k < V / 4; ++k)
-            word[k] = code_of(as_float<T>(v[4 * k]), inverse) | code_of(as_float<T>(v[4 * k + 1]), inverse) << 8 |
-                      code_of(as_float<T>(v[4 * k + 2]), inverse) << 16 |
-                      code_of(as_float<T>(v[4 * k + 3]), inverse) << 24;
+            for (int k = 0; k < V / 4; ++k) {
+                const float2 a = make_float2(as_float<T>(v[4 * k]) * inverse, as_float<T>(v[4 * k + 1]) * inverse);
+                const float2 b = make_float2(as_float<T>(v[4 * k + 2]) * inverse, as_float<T>(v[4 * k + 3]) * inverse);
+                word[k] = (uint32_t)__nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3) |
+                          (uint32_t)__nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3) << 16;
+            }
+        } else {  // the whole team is here: an infinity or a NaN among the block's values
+            top = 0.0f;
+#pragma unroll
+            for (int k = 0; k < V; ++k) top = fmaxf(top, finite_magnitude(as_float<T>(v[k])));
+            const unsigned team = __activemask();
+#pragma unroll
+            for (int o = kTeam / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(team, top, o));
+            s = scale_exponent<T>(top);
+            const float inverse = power_of_two(-s);
+#pragma unroll
+            for (int k = 0; k < V / 4; ++k)
+                word[k] = code_of(as_float<T>(v[4 * k]), inverse) | code_of(as_float<T>(v[4 * k + 1]), inverse) << 8 |
+                          code_of(as_float<T>(v[4 * k + 2]), inverse) << 16 |
+                          code_of(as_float<T>(v[4 * k + 3]), inverse) << 24;
+        }
         if (i < vectors) {
             if constexpr (V == 4)
                 reinterpret_cast<uint32_t*>(codes)[i] = word[0];
@@ -215,8 +263,20 @@ __global__ void __launch_bounds__(256) unpack_vectors_kernel(const uint8_t* code
         const int64_t i = start + u * 256;
         if (i >= vectors) continue;
         alignas(16) T out[V];
+        // No value is above 448 scale, so below this scale none has to be cut off.
+        if (scale[u] <= kLargest<T> / 512.0f) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) out[k] = held<T>((word[u][k / 4] >> (8 * (k % 4))) & 0xffu, scale[u]);
+            for (int k = 0; k < V; k += 2) {
+                const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
+                    (__nv_fp8x2_storage_t)(word[u][k / 4] >> (8 * (k % 4))), __NV_E4M3);
+                const float2 f = __half22float2(__half2(h));
+                out[k] = rounded<T>(f.x * scale[u]);
+                out[k + 1] = rounded<T>(f.y * scale[u]);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < V; ++k) out[k] = held<T>((word[u][k / 4] >> (8 * (k % 4))) & 0xffu, scale[u]);
+        }
         reinterpret_cast<uint4*>(x)[i] = *reinterpret_cast<uint4*>(out);
     }
 }
