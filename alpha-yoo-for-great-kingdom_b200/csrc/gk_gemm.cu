@@ -771,7 +771,7 @@ int launch_split(const GemmArgs& g, uint32_t* status, cudaStream_t stream) {
     if (!once_per_device(ready, [&] {
             return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) == cudaSuccess;
         }))
-        return launch_status();
+        return setup_failed();
     CUtensorMap ta, tb;
     if (!encode(&ta, g.a, g.a_ld, g.a_across, g.m, g.k, 128, g.dtype) ||
         !encode(&tb, g.b, g.b_ld, g.b_across, g.n, g.k, BN, g.dtype))
@@ -802,7 +802,7 @@ int launch_pair(const GemmArgs& g, uint32_t* status, cudaStream_t stream) {
     if (!once_per_device(ready, [&] {
             return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kSmem) == cudaSuccess;
         }))
-        return launch_status();
+        return setup_failed();
     const Epilogue ep = epilogue_of(g);
     CUtensorMap ta, tb, t_out = {}, t_pre = {};
     if (!encode(&ta, g.a, g.a_ld, g.a_across, g.m, g.k, 128, g.dtype) ||

@@ -18,6 +18,12 @@ inline int launch_status() {
     return e == cudaSuccess ? 0 : (int)e;
 }
 
+// The error that a launch's set-up left, or GK_EINVAL if it left none: never success.
+inline int setup_failed() {
+    const int e = launch_status();
+    return e != 0 ? e : GK_EINVAL;
+}
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -376,7 +376,7 @@ int launch_gemm32(const Gemm32& g, cudaStream_t s) {
             return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem) == cudaSuccess &&
                    cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
         }))
-        return launch_status();
+        return setup_failed();
     const int64_t tiles_n = (g.n + B - 1) / B, tiles = (g.m + B - 1) / B * tiles_n;
     if (tiles >= (1ll << 31)) return GK_EINVAL;
     const int64_t steps = (g.k + kStep - 1) / kStep;
@@ -679,7 +679,7 @@ BackwardPlan backward_plan(const gk_linear_grad_t& p, void* workspace) {
     b.dz = {p.dy, p.dy_stride, false};
     if (b.forms_dz) {
         // The residual's gradient serves as dz where its rows are aligned.
-        if (p.dz != nullptr && (!k16 || p.n % 8 == 0))
+        if (p.dz != nullptr && (!k16 || tma_rows(p.dz, p.n, p.n)))
             b.dz = {p.dz, p.n, false};
         else
             b.dz = {arena.take(p.m * pad8(p.n) * (int64_t)sizeof(T)), pad8(p.n), false};

@@ -844,8 +844,8 @@ int launch_long(const gk_policy_loss_t& p, const LongPlan& plan, int* clusters, 
             }
             return true;
         }))
-        return launch_status();
-    if (cudaGetDevice(&dev) != cudaSuccess) return launch_status();
+        return setup_failed();
+    if (cudaGetDevice(&dev) != cudaSuccess) return setup_failed();
     // GPCs of an odd number of SMs leave some out of a cluster: a grid that is
     // resident at once has no second round for the rest.
     const int64_t most = resident[dev][plan.log_cluster] > 0 ? resident[dev][plan.log_cluster] : 1;

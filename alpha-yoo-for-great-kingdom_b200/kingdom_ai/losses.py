@@ -69,6 +69,12 @@ def policy_loss(logits, *, legal_mask=None, actions=None, old_log_probs=None, ad
     wider whatever the logits' type; only ``logits`` get a gradient. The
     gradient of a row with no target mass and no action is zero.
 
+    The gradient is made with the loss, for an upstream gradient of one, and
+    handed out by the first backward pass (any other upstream gradient, a later
+    pass over a retained graph, and fp16, whose losses are scaled, form it in
+    the backward pass). ``logits`` and the other arguments must not change in
+    place before that.
+
     Rows with unit column stride are read in place; others are copied first.
     """
     global _operator

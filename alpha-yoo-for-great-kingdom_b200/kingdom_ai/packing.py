@@ -60,9 +60,9 @@ def pack_activation(x: torch.Tensor) -> PackedActivation:
 
 
 def _is_parameter(t: torch.Tensor) -> bool:
-    """A leaf that is being trained, a view of one, or one cast to another type (autocast)."""
+    """A parameter, a leaf that is being trained, a view of one, or one cast to another type (autocast)."""
     base = t if t._base is None else t._base
-    if base.is_leaf and base.requires_grad:
+    if isinstance(base, torch.nn.Parameter) or (base.is_leaf and base.requires_grad):
         return True
     fn = t.grad_fn
     if fn is None or not fn.name().startswith("ToCopyBackward"):
@@ -75,9 +75,11 @@ def _is_parameter(t: torch.Tensor) -> bool:
 def packed_activations(min_elements: int = 1 << 16):
     """Within the context, what operators keep for the backward pass is packed:
     CUDA tensors of fp32, bf16 or fp16 with at least ``min_elements`` values,
-    parameters excepted (also their views and casts). Gradients are then those
-    of the held values; the forward pass computes with the exact ones. A relu
-    that keeps its output passes no gradient where the packed output is zero.
+    parameters excepted (frozen ones, views, and casts of those in training; a
+    cast of a frozen weight cannot be told from an activation, so keep such a
+    layer outside). Gradients are then those of the held values; the forward
+    pass computes with the exact ones. A relu that keeps its output passes no
+    gradient where the packed output is zero.
     ``linear`` and ``policy_loss`` keep their tensors as they are (``linear``
     has its own ``checkpoint``)."""
     if isinstance(min_elements, bool) or not isinstance(min_elements, int) or min_elements < 1:

@@ -301,6 +301,38 @@ def test_another_stream_and_two_captured_graphs():
                 assert torch.equal(got, value)
 
 
+def test_calls_on_two_streams_at_once():
+    """Workspaces belong to their call: interleaved launches on two streams do not meet."""
+    from kingdom_ai import linear
+    args = [make(600, 1003, 517, torch.bfloat16, seed=s) for s in (1, 2)]
+    want = [run(*a, "gelu", "e4m3") for a in args]
+    streams = [torch.cuda.Stream() for _ in args]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(8):
+        for i, (a, s) in enumerate(zip(args, streams)):
+            with torch.cuda.stream(s):
+                y = linear(a[0], a[1], a[2], activation="gelu", residual=a[3], checkpoint="e4m3")
+                got[i].append((y.detach(), *torch.autograd.grad(y, a[:4], a[4])))
+    torch.cuda.synchronize()
+    for w, rows in zip(want, got):
+        for row in rows:
+            assert all(torch.equal(t, w[k]) for t, k in zip(row, ("y", "x", "w", "b", "r")))
+
+
+def test_no_backward_memory_is_kept_or_lost():
+    """Repeated steps leave the allocator where it was."""
+    args = make(512, 333, 257, torch.float16)
+    run(*args, "silu", "e4m3")
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(5):
+        run(*args, "silu", "e4m3")
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before
+
+
 def test_the_same_call_gives_the_same_bits():
     args = make(700, 2000, 130, torch.bfloat16)
     first = run(*args, "gelu", "e4m3")

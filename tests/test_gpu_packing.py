@@ -155,6 +155,17 @@ def test_packed_activations_saves_memory_and_keeps_cast_parameters():
     assert torch.equal(g, torch.ones_like(y) @ w.detach().to(torch.bfloat16).t())
 
 
+def test_frozen_parameters_are_kept():
+    from kingdom_ai import packed_activations
+    layer = torch.nn.Linear(512, 512, bias=False).cuda()
+    layer.weight.requires_grad_(False)
+    h = torch.randn(64, 512, device="cuda", requires_grad=True)
+    with packed_activations(min_elements=1024):
+        y = layer(h)
+    g, = torch.autograd.grad(y, h, torch.ones_like(y))
+    assert torch.equal(g, torch.ones_like(y) @ layer.weight)
+
+
 def test_linear_and_policy_loss_keep_their_tensors_inside():
     from kingdom_ai import linear, packed_activations, policy_loss
     x = torch.randn(256, 512, device="cuda")
