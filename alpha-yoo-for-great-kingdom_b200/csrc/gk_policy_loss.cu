@@ -362,9 +362,11 @@ __device__ __forceinline__ void gradient_group(const Group<TL, V>& h, const floa
     }
 }
 
-// t (log t - d), with d the entry's log-probability or its distance to a maximum.
+// t (log t - d), with d the entry's log-probability or its distance to a
+// maximum; 0 for t = 0 whatever d is, not a number for a t below 0.
 __device__ __forceinline__ float target_term(float t, float d) {
-    return t > 0.0f ? t * (__logf(t) - d) : (t == 0.0f ? 0.0f : nanf(""));
+    const float term = t * (__logf(t) - d);
+    return t == 0.0f ? 0.0f : term;
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -647,35 +649,36 @@ __global__ void __launch_bounds__(THREADS, 3 * kLongThreads / THREADS) policy_lo
                 gradient_group<TL, TT, V>(h, t, e, kp, kt, g);
                 store_group<TL, V>(grow, first, cols, edge, g);
             };
-            constexpr int U = 4;
-            int k = tid;
-            const int whole = next_count > 0 ? min(count, next_count) : count;
-            for (; k + (U - 1) * THREADS < whole; k += U * THREADS) {
-                Group<TL, V> h[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (part.mrow == nullptr)
-                        h[u].template load<false>(from + (k + u * THREADS) * V, nullptr);
-                    else
-                        h[u].template load<true>(from + (k + u * THREADS) * V, mask + (k + u * THREADS) * V);
-                }
-#pragma unroll
-                for (int u = 0; u < U; ++u) finish(h[u], base + (k + u * THREADS) * V, false);
-                if (next_count > 0) {
+            // The mask's presence is settled outside the loops, so that without one nothing is left of it inside.
+            auto last_pass = [&](auto masked) {
+                constexpr bool kMask = decltype(masked)::value;
+                constexpr int U = 4;
+                int k = tid;
+                const int whole = next_count > 0 ? min(count, next_count) : count;
+                for (; k + (U - 1) * THREADS < whole; k += U * THREADS) {
+                    Group<TL, V> h[U];
 #pragma unroll
                     for (int u = 0; u < U; ++u)
-                        copy_async(staged + k + u * THREADS, next_from + (k + u * THREADS) * V);
+                        h[u].template load<kMask>(from + (k + u * THREADS) * V, mask + (k + u * THREADS) * V);
+#pragma unroll
+                    for (int u = 0; u < U; ++u) finish(h[u], base + (k + u * THREADS) * V, false);
+                    if (next_count > 0) {
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+                            copy_async(staged + k + u * THREADS, next_from + (k + u * THREADS) * V);
+                    }
                 }
-            }
-            for (; k < count; k += THREADS) {
-                Group<TL, V> h;
-                if (part.mrow == nullptr)
-                    h.template load<false>(from + k * V, nullptr);
-                else
-                    h.template load<true>(from + k * V, mask + k * V);
-                finish(h, base + k * V, false);
-                if (k < next_count) copy_async(staged + k, next_from + k * V);
-            }
+                for (; k < count; k += THREADS) {
+                    Group<TL, V> h;
+                    h.template load<kMask>(from + k * V, mask + k * V);
+                    finish(h, base + k * V, false);
+                    if (k < next_count) copy_async(staged + k, next_from + k * V);
+                }
+            };
+            if (part.mrow == nullptr)
+                last_pass(std::false_type());
+            else
+                last_pass(std::true_type());
             // An odd row's part may be a group longer than the one before it.
             if (count < next_count && tid == count % THREADS) copy_async(staged + count, next_from + count * V);
             edges(finish);
