@@ -185,52 +185,64 @@ __device__ __forceinline__ bool warp_wait(bool ready, uint32_t bar, uint32_t par
 // tile along k. Every CTA of the cluster leaves its fp32 part in its shared
 // memory, and each then adds up, in rank order, and finishes a share of the
 // tile's rows: no workspace, no atomics, one launch.
-// Warp 0 loads, warp 1 issues the MMAs, warps 2-5 drain TMEM, all finish.
-constexpr int kSplitThreads = 192;
-struct Split {
-    static constexpr int kBN = 64;
-    static constexpr int kStages = 4;
-    static constexpr int kA = 128 * kBK * 2, kB = kBN * kBK * 2, kStage = kA + kB;
-    static constexpr int kPitch = kBN + 4;  // fp32 row pitch of the part: rows 16 bytes apart modulo the banks
-    static constexpr int kSmem = kStages * kStage + 1024;
-    static_assert(128 * kPitch * 4 <= kStages * kStage, "the part reuses the stages");
+//
+// THIN: a product of at most 128 rows reads B (the weight) once and is bound by
+// that. It runs with the operands exchanged, 128 rows of B to a tile and all
+// rows of A beside them, so that a stage is mostly weight and the stages hold
+// some 100 KB of it in flight; the accumulator is out^T and is turned through
+// shared memory. A load of A takes only the rows there are: boxes that lie mostly
+// outside the tensor halved the speed (12 x 4096 x 12288: 55 us, 16 rows 27).
+//
+// Warp 0 loads, warp 1 issues the MMAs, warps 2-9 drain TMEM (two a quadrant of
+// its rows, every other 32 columns each), all finish.
+constexpr int kSplitThreads = 320;
+constexpr int kSplitSmem = 112 * 1024;  // two CTAs an SM
+constexpr int kMostStages = 8;
+struct SplitShape {
+    int bn;  // rows of the second operand in a tile
+    __host__ __device__ int stage_bytes() const { return (128 + bn) * kBK * 2; }
+    __host__ __device__ int stages() const {
+        const int fit = (kSplitSmem - 1024) / stage_bytes();
+        return fit < kMostStages ? fit : kMostStages;
+    }
+    __host__ __device__ int smem() const { return stages() * stage_bytes() + 1024; }
+    // fp32 pitch of the part, [128][bn] or THIN [bn][128]: rows 16 bytes apart modulo the banks
+    __host__ __device__ static constexpr int pitch(bool thin) { return (thin ? 128 : 64) + 4; }
 };
+constexpr int kSplitBN = 64;
 
-// Bias, residual, activation and stores of four neighbours of a row.
-__device__ __forceinline__ void finish4(const Epilogue& ep, int64_t m, int n, float (&v)[4], bool bf16) {
-    const int count = min(4, ep.n - n);
-    const bool whole = count == 4;
-    if (ep.bias != nullptr) {
+// Four neighbours of a row, `count` of which there are (fewer at a row's end).
+__device__ __forceinline__ void add4(const void* p, int64_t at, int count, bool wide, float (&v)[4], bool bf16) {
+    if (wide && count == 4) {
+        const uint2 x = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at));
+        float lo, hi;
+        unpack16(x.x, bf16, lo, hi);
+        v[0] += lo, v[1] += hi;
+        unpack16(x.y, bf16, lo, hi);
+        v[2] += lo, v[3] += hi;
+    } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (j < count) v[j] += load16(ep.bias, n + j, bf16);
+            if (j < count) v[j] += load16(p, at + j, bf16);
     }
-    if (ep.residual != nullptr) {
-        if (whole && ep.residual_wide) {
-            const uint2 x =
-                *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(ep.residual) + m * ep.residual_ld + n);
-            float lo, hi;
-            unpack16(x.x, bf16, lo, hi);
-            v[0] += lo, v[1] += hi;
-            unpack16(x.y, bf16, lo, hi);
-            v[2] += lo, v[3] += hi;
-        } else {
+}
+__device__ __forceinline__ void put4(void* p, int64_t at, int count, bool wide, const float (&v)[4], bool bf16) {
+    if (wide && count == 4) {
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + at) =
+            make_uint2(pack16(v[0], v[1], bf16), pack16(v[2], v[3], bf16));
+    } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j < count) v[j] += load16(ep.residual, m * ep.residual_ld + n + j, bf16);
-        }
+        for (int j = 0; j < 4; ++j)
+            if (j < count) store16(p, at + j, v[j], bf16);
     }
+}
+// Bias, residual, activation and stores.
+__device__ __forceinline__ void finish4(const Epilogue& ep, int64_t m, int n, float (&v)[4], bool bf16) {
+    const int count = min(4, ep.n - n);
+    if (ep.bias != nullptr) add4(ep.bias, n, count, ep.bias_wide, v, bf16);
+    if (ep.residual != nullptr) add4(ep.residual, m * ep.residual_ld + n, count, ep.residual_wide, v, bf16);
     const bool tanh32 = ep.activation == GK_ACT_TANH;  // keeps its fp32 value, not the sum
-    if (ep.pre != nullptr && !tanh32) {
-        if (whole && ep.pre_wide) {
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(ep.pre) + m * ep.pre_ld + n) =
-                make_uint2(pack16(v[0], v[1], bf16), pack16(v[2], v[3], bf16));
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j < count) store16(ep.pre, m * ep.pre_ld + n + j, v[j], bf16);
-        }
-    }
+    if (ep.pre != nullptr && !tanh32) put4(ep.pre, m * ep.pre_ld + n, count, ep.pre_wide, v, bf16);
     if (ep.activation != GK_ACT_NONE) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = act_value<true>(v[j], ep.activation);
@@ -241,40 +253,37 @@ __device__ __forceinline__ void finish4(const Epilogue& ep, int64_t m, int n, fl
         for (int j = 0; j < 4; ++j)
             if (j < count) kept[j] = v[j];
     }
-    if (whole && ep.out_wide) {
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(ep.out) + m * ep.out_ld + n) =
-            make_uint2(pack16(v[0], v[1], bf16), pack16(v[2], v[3], bf16));
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < count) store16(ep.out, m * ep.out_ld + n + j, v[j], bf16);
-    }
+    put4(ep.out, m * ep.out_ld + n, count, ep.out_wide, v, bf16);
 }
 
-__global__ void __launch_bounds__(kSplitThreads) gemm_split_kernel(const __grid_constant__ CUtensorMap ta,
+template <bool THIN>
+__global__ void __launch_bounds__(kSplitThreads, 2) gemm_split_kernel(const __grid_constant__ CUtensorMap ta,
                                                                    const __grid_constant__ CUtensorMap tb,
-                                                                   Epilogue ep, int tiles_n, int k_blocks,
-                                                                   int a_across, int b_across, uint32_t* status) {
-    using S = Split;
-    constexpr int BN = S::kBN;
+                                                                   Epilogue ep, int thin_rows, int tiles_n,
+                                                                   int k_blocks, int a_across, int b_across,
+                                                                   uint32_t* status) {
+    constexpr int kA = 128 * kBK * 2, kPitch = SplitShape::pitch(THIN);
+    const SplitShape shape{THIN ? thin_rows : kSplitBN};
+    const int count = shape.stages(), stage_bytes = shape.stage_bytes();
     extern __shared__ uint8_t raw[];
-    __shared__ alignas(8) uint64_t full[S::kStages], empty[S::kStages], done;
+    __shared__ alignas(8) uint64_t full[kMostStages], empty[kMostStages], done;
     __shared__ uint32_t tmem_slot;
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t stages = smem_u32(base);
-    const int tile_m = blockIdx.x / tiles_n, m0 = tile_m * 128, n0 = (blockIdx.x - tile_m * tiles_n) * BN;
+    const uint32_t tmem_cols = shape.bn <= 32 ? 32 : shape.bn <= 64 ? 64 : 128;
+    const int tile_a = blockIdx.x / tiles_n, a_row0 = tile_a * 128, b_row0 = (blockIdx.x - tile_a * tiles_n) * kSplitBN;
     const int kb0 = (int)((int64_t)rank * k_blocks / ranks), kb1 = (int)((int64_t)(rank + 1) * k_blocks / ranks);
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::kStages; ++s) mbar_init(smem_u32(&full[s]), 1), mbar_init(smem_u32(&empty[s]), 1);
+        for (int s = 0; s < count; ++s) mbar_init(smem_u32(&full[s]), 1), mbar_init(smem_u32(&empty[s]), 1);
         mbar_init(smem_u32(&done), 1);
         fence_mbar_init();
     }
     if (warp == 1) {
-        tmem_alloc(smem_u32(&tmem_slot), BN);
+        tmem_alloc(smem_u32(&tmem_slot), tmem_cols);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -289,31 +298,34 @@ __global__ void __launch_bounds__(kSplitThreads) gemm_split_kernel(const __grid_
         for (int kb = kb0; kb < kb1 && ok; ++kb) {
             ok = warp_wait(ready, smem_u32(&empty[s]), (turn - 1) & 1, status);
             if (!ok) break;
-            const int next = s + 1 == S::kStages ? 0 : s + 1, next_turn = next == 0 ? turn + 1 : turn;
+            const int next = s + 1 == count ? 0 : s + 1, next_turn = next == 0 ? turn + 1 : turn;
             ready = next_turn == 0 || mbar_look(smem_u32(&empty[next]), (next_turn - 1) & 1);
-            const uint32_t bar = smem_u32(&full[s]), at = stages + s * S::kStage;
-            expect_tx(one, bar, S::kStage);
-            load_stage<128, false>(one, at, &ta, a_across, m0, kb * kBK, bar);
-            load_stage<BN, false>(one, at + S::kA, &tb, b_across, n0, kb * kBK, bar);
+            const uint32_t bar = smem_u32(&full[s]), at = stages + s * stage_bytes;
+            expect_tx(one, bar, stage_bytes);
+            load_stage<128, false>(one, at, &ta, a_across, a_row0, kb * kBK, bar);
+            if constexpr (THIN)  // one box of bn rows, k contiguous
+                tma_load<false>(one, at + kA, &tb, kb * kBK, 0, bar);
+            else
+                load_stage<kSplitBN, false>(one, at + kA, &tb, b_across, b_row0, kb * kBK, bar);
             s = next, turn = next_turn;
         }
         // After a wait that gave up: the copies in flight land before the block may end.
         if (!ok)
-            for (int i = max(0, turn * S::kStages + s - S::kStages); i < turn * S::kStages + s; ++i)
-                mbar_wait(smem_u32(&full[i % S::kStages]), (i / S::kStages) & 1, status);
+            for (int i = max(0, turn * count + s - count); i < turn * count + s; ++i)
+                mbar_wait(smem_u32(&full[i % count]), (i / count) & 1, status);
     } else if (warp == 1) {
-        const uint32_t idesc = idesc16(128, BN, ep.bf16, a_across, b_across);
+        const uint32_t idesc = idesc16(128, shape.bn, ep.bf16, a_across, b_across);
         const uint32_t step_a = k_step(a_across), step_b = k_step(b_across);
-        const uint32_t a0 = desc_low(stages, a_across), b0 = desc_low(stages + S::kA, b_across);
+        const uint32_t a0 = desc_low(stages, a_across), b0 = desc_low(stages + kA, b_across);
         int s = 0, parity = 0;
         bool ready = false;
         const uint32_t one = elect_one();
         for (int kb = kb0; kb < kb1; ++kb) {
             if (!warp_wait(ready, smem_u32(&full[s]), parity, status)) break;
-            const int next = s + 1 == S::kStages ? 0 : s + 1, next_parity = next == 0 ? parity ^ 1 : parity;
+            const int next = s + 1 == count ? 0 : s + 1, next_parity = next == 0 ? parity ^ 1 : parity;
             ready = mbar_look(smem_u32(&full[next]), next_parity);
             tc_fence_after();
-            mma_stage<false>(one, tmem, a0 + s * (S::kStage >> 4), b0 + s * (S::kStage >> 4), step_a, step_b, idesc,
+            mma_stage<false>(one, tmem, a0 + s * (stage_bytes >> 4), b0 + s * (stage_bytes >> 4), step_a, step_b, idesc,
                              kb > kb0 ? 1u : 0u, smem_u32(&empty[s]));
             s = next, parity = next_parity;
         }
@@ -326,14 +338,19 @@ __global__ void __launch_bounds__(kSplitThreads) gemm_split_kernel(const __grid_
     float* part = reinterpret_cast<float*>(base);
     if (warp >= 2) {
         const int quadrant = warp & 3, row = quadrant * 32 + lane;
-#pragma unroll
-        for (int c = 0; c < BN; c += 32) {
+        for (int c = (warp - 2) / 4 * 32; c < shape.bn; c += 64) {
             float v[32];
             tmem_ld32(tmem + ((uint32_t)(quadrant * 32) << 16) + c, v);
+            if constexpr (THIN) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<float4*>(part + row * S::kPitch + c + i) =
-                    make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                for (int i = 0; i < 32; ++i)
+                    if (c + i < shape.bn) part[(c + i) * kPitch + row] = v[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4)
+                    *reinterpret_cast<float4*>(part + row * kPitch + c + i) =
+                        make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            }
         }
     }
     tc_fence_before();
@@ -343,29 +360,37 @@ __global__ void __launch_bounds__(kSplitThreads) gemm_split_kernel(const __grid_
         __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, BN);
+        tmem_dealloc(tmem, tmem_cols);
     }
-    const int rows = 128 / ranks, first = rank * rows;
+    // Each rank finishes its share of the tile, four neighbours of an output row
+    // at a time: a warp then reads whole lines of a part (with eight, the reads of
+    // other CTAs' shared memory in steps of 32 bytes took twice as long).
+    constexpr int kQuads = (THIN ? 128 : kSplitBN) / 4;
+    const int m0 = THIN ? 0 : a_row0, n0 = THIN ? a_row0 : b_row0;
+    const int work = min(THIN ? shape.bn : 128, ep.m - m0) * kQuads;
     const bool bf16 = ep.bf16 != 0;
     if (ranks == 1) {
-#pragma unroll 4
-        for (int i = threadIdx.x; i < 128 * (BN / 4); i += kSplitThreads) {
-            const int r = i / (BN / 4), c = (i % (BN / 4)) * 4;
-            if (m0 + r >= ep.m || n0 + c >= ep.n) continue;
-            const float4 x = *reinterpret_cast<const float4*>(part + r * S::kPitch + c);
+        for (int i = threadIdx.x; i < work; i += kSplitThreads) {
+            const int r = i / kQuads, c = (i % kQuads) * 4;
+            if (n0 + c >= ep.n) continue;
+            const float4 x = *reinterpret_cast<const float4*>(part + r * kPitch + c);
             float v[4] = {x.x, x.y, x.z, x.w};
             finish4(ep, m0 + r, n0 + c, v, bf16);
         }
         return;
     }
-    for (int i = threadIdx.x; i < rows * (BN / 4); i += kSplitThreads) {
-        const int r = first + i / (BN / 4), c = (i % (BN / 4)) * 4;
-        if (m0 + r >= ep.m || n0 + c >= ep.n) continue;
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int k = 0; k < ranks; ++k) {
-            const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(part, k) + r * S::kPitch + c);
-            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
-        }
+    const int from = (int)((int64_t)work * rank / ranks), to = (int)((int64_t)work * (rank + 1) / ranks);
+    for (int i = from + threadIdx.x; i < to; i += kSplitThreads) {
+        const int r = i / kQuads, c = (i % kQuads) * 4;
+        if (n0 + c >= ep.n) continue;
+        float4 x[8];  // the parts of all ranks in flight
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < ranks) x[k] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(part, k) + r * kPitch + c);
+        float v[4] = {};
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < ranks) v[0] += x[k].x, v[1] += x[k].y, v[2] += x[k].z, v[3] += x[k].w;
         finish4(ep, m0 + r, n0 + c, v, bf16);
     }
     cluster.sync();  // no CTA leaves while another reads its part
@@ -763,26 +788,39 @@ int split_ranks(int64_t tiles, int64_t stages) {
     return ranks;
 }
 
+// The same for thin products, of any size up to eight and short of two to an
+// SM: clusters of some sizes do not pack the last slots.
+int thin_ranks(int64_t tiles, int64_t stages) {
+    int64_t ranks = 256 / tiles;
+    if (ranks > 8) ranks = 8;
+    if (ranks > stages / 4) ranks = stages / 4;
+    return ranks < 1 ? 1 : (int)ranks;
+}
+
+template <bool THIN>
 int launch_split(const GemmArgs& g, uint32_t* status, cudaStream_t stream) {
-    using S = Split;
-    constexpr int BN = S::kBN;
-    auto* kernel = gemm_split_kernel;
+    auto* kernel = gemm_split_kernel<THIN>;
     static bool ready[64] = {};
     if (!once_per_device(ready, [&] {
-            return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) == cudaSuccess;
+            return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitSmem) == cudaSuccess;
         }))
         return setup_failed();
+    // THIN: the weight is the first operand, and the tile holds all rows of the other.
+    const SplitShape shape{THIN ? (int)((g.m + 15) / 16 * 16) : kSplitBN};
     CUtensorMap ta, tb;
-    if (!encode(&ta, g.a, g.a_ld, g.a_across, g.m, g.k, 128, g.dtype) ||
-        !encode(&tb, g.b, g.b_ld, g.b_across, g.n, g.k, BN, g.dtype))
+    if (THIN ? !encode(&ta, g.b, g.b_ld, g.b_across, g.n, g.k, 128, g.dtype) ||
+                   !encode(&tb, g.a, g.a_ld, 0, g.m, g.k, shape.bn, g.dtype)
+             : !encode(&ta, g.a, g.a_ld, g.a_across, g.m, g.k, 128, g.dtype) ||
+                   !encode(&tb, g.b, g.b_ld, g.b_across, g.n, g.k, shape.bn, g.dtype))
         return GK_EINVAL;
-    const int64_t tiles_m = (g.m + 127) / 128, tiles_n = (g.n + BN - 1) / BN, blocks = (g.k + kBK - 1) / kBK;
-    const int ranks = split_ranks(tiles_m * tiles_n, blocks);
+    const int64_t tiles_a = ((THIN ? g.n : g.m) + 127) / 128, tiles_b = THIN ? 1 : (g.n + kSplitBN - 1) / kSplitBN;
+    const int64_t blocks = (g.k + kBK - 1) / kBK;
+    const int ranks = THIN ? thin_ranks(tiles_a, blocks) : split_ranks(tiles_a * tiles_b, blocks);
     cudaLaunchConfig_t cfg = {};
-    if (tiles_m * tiles_n >= (1ll << 31)) return GK_EINVAL;
-    cfg.gridDim = dim3((unsigned)(tiles_n * tiles_m), 1, (unsigned)ranks);
+    if (tiles_a * tiles_b >= (1ll << 31)) return GK_EINVAL;
+    cfg.gridDim = dim3((unsigned)(tiles_a * tiles_b), 1, (unsigned)ranks);
     cfg.blockDim = dim3(kSplitThreads);
-    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.dynamicSmemBytes = shape.smem();
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -790,8 +828,8 @@ int launch_split(const GemmArgs& g, uint32_t* status, cudaStream_t stream) {
     attr[0].val.clusterDim.z = ranks;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, ta, tb, epilogue_of(g), (int)tiles_n,
-                                   (int)blocks, g.a_across, g.b_across, status);
+    return (int)cudaLaunchKernelEx(&cfg, kernel, ta, tb, epilogue_of(g), shape.bn, (int)tiles_b, (int)blocks,
+                                   THIN ? g.b_across : g.a_across, THIN ? 0 : g.b_across, status);
 }
 
 template <int BN>
@@ -843,7 +881,14 @@ int gemm16(const GemmArgs& g, uint32_t* status, cudaStream_t stream) {
                          (g.m <= 64 ? 1.3 : 0.0);
     const double narrow = 5.3 + rounds(tiles_m * ((g.n + 127) / 128), kSmCount / 2) * fmax(stages * 0.233, 1.3);
     const double wide = 5.6 + rounds(tiles_m * ((g.n + 255) / 256), kSmCount / 2) * fmax(stages * 0.28, 2.0);
-    if (split <= narrow && split <= wide) return launch_split(g, status, stream);
+    // The thin form, where the weight's bytes bound the product (thin | best of the
+    // others, us; m x k x n): 12 x 4096 x 12288 20.5 | 54, 37 x 8192 x 4096 17.7 | 18.3,
+    // 37 x 4096 x 32000 45.5 | 53.5, 64 x 4096 x 4096 13.6 | 12.9, 128 x 4096 x 12288
+    // 27.6 | 29.3, 128 x 512 x 16384 13.7 | 11.4, 128 x 4096 x 4096 17.2 | 14.1 (its
+    // outputs go through other CTAs' shared memory as often as ranks share a tile).
+    if (g.a_across == 0 && (g.m <= 48 || (g.m <= 128 && g.n >= 64 * 128 && g.k >= 1024)))
+        return launch_split<true>(g, status, stream);
+    if (split <= narrow && split <= wide) return launch_split<false>(g, status, stream);
     return narrow <= wide ? launch_pair<128>(g, status, stream) : launch_pair<256>(g, status, stream);
 }
 

@@ -6,7 +6,8 @@
 // the fp32 units: its callers train the network's heads in fp32, and one tf32
 // or bf16 product would lose the bits that they keep fp32 for. A product with
 // at most eight rows reads each weight once and is bound by that: it runs as
-// dot products on the cores whatever the type.
+// dot products on the cores, but for weights so wide that tcgen05 streams them
+// faster (few_rows_win).
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -45,7 +46,13 @@ struct FewRows {
 
 // A warp (or k_parts of them) takes R rows of W; its lanes run along k, 16
 // bytes of each row at a time where V > 1, and every value of W meets the M
-// rows of x (held by L1) in registers.
+// rows of x (held by L1) in registers. Bound by the bytes of W for one row (4096
+// -> 12288 bf16 19 us, 5.3 TB/s; 32000: 5.6 TB/s), then by the loads of x.
+// Steps unrolled, measured: 16 bytes at a time 2 for one row (1: 29 us, 4: 25)
+// and 1 for more (8 rows of 4096 -> 12288: 43, unrolled 55 us); single values 4
+// (4097 -> 12288, one row: 32 us, by 2 152 us).
+template <int M, int V>
+constexpr int kFewUnroll = V == 1 ? 4 : M == 1 ? 2 : 1;
 template <typename T, int M, int R, int V>
 __global__ void __launch_bounds__(256) linear_few_kernel(FewRows p) {
     __shared__ float parts[8][R * M];
@@ -62,8 +69,11 @@ __global__ void __launch_bounds__(256) linear_few_kernel(FewRows p) {
     const T* wr[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) wr[r] = w + (n0 + r < p.n ? n0 + r : p.n - 1) * p.w_stride;
+    const T* xr[M];  // a row that is not there repeats the last: no branch stands between the loads
+#pragma unroll
+    for (int m = 0; m < M; ++m) xr[m] = x + (m < p.m ? m : p.m - 1) * p.x_stride;
     const int64_t step = (int64_t)32 * V * p.k_parts;
-#pragma unroll 2
+#pragma unroll kFewUnroll<M, V>
     for (int64_t k = ((int64_t)part * 32 + lane) * V; k < p.k; k += step) {
         alignas(16) T wv[R][V];
 #pragma unroll
@@ -71,16 +81,17 @@ __global__ void __launch_bounds__(256) linear_few_kernel(FewRows p) {
             if constexpr (V > 1)
                 *reinterpret_cast<uint4*>(wv[r]) = __ldcs(reinterpret_cast<const uint4*>(wr[r] + k));
             else
-                wv[r][0] = wr[r][k];
+                wv[r][0] = __ldg(wr[r] + k);
         }
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-            if (m >= p.m) break;
+            // Never taken; with one row it keeps the loads of W together (4096 x 12288: 20.8 -> 19.0 us).
+            if (M == 1 && p.m < 1) break;
             alignas(16) T xv[V];
             if constexpr (V > 1)
-                *reinterpret_cast<uint4*>(xv) = __ldg(reinterpret_cast<const uint4*>(x + m * p.x_stride + k));
+                *reinterpret_cast<uint4*>(xv) = __ldg(reinterpret_cast<const uint4*>(xr[m] + k));
             else
-                xv[0] = x[m * p.x_stride + k];
+                xv[0] = __ldg(xr[m] + k);
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -625,6 +636,22 @@ int copy_if_needed(const Operand& o, const void* p, int64_t stride, int64_t rows
     return launch_status();
 }
 
+// Whether dot products on the cores are the faster form. fp32: up to eight rows.
+// 16-bit types, against the thin product on tcgen05 that costs a start of some
+// 5 us and then the bytes of W whatever the rows (cores | tcgen05, us): one row
+// of 4096 -> 4096 7.9 | 10.6, 8192 -> 8192 23.1 | 24.5, 4096 -> 32000 47 | 43;
+// two rows of 4096 -> 4096 8.6 | 10.6, 4096 -> 12288 21 | 20; four of 512 -> 16384
+// 7.8 | 7.8, 4096 -> 4096 12.7 | 10.9; eight of 4096 -> 512 4.4 | 6.0, 512 -> 16384
+// 11.1 | 8.0. Rows that TMA cannot read have to be copied for it first: one row
+// of 4097 -> 12288 32 | 62, four 51 | 64, eight 90 | 64, eight of 517 -> 16384 19 | 18.
+bool few_rows_win(const gk_linear_t& p) {
+    if (p.m > kFewRows) return false;
+    if (p.dtype == GK_FP32) return true;
+    const double work = (double)p.m * (double)p.n * (double)p.k;
+    if (!tma_rows(p.x, p.x_stride, p.k) || !tma_rows(p.w, p.w_stride, p.k)) return p.m <= 4 || work <= 1 << 26;
+    return work <= (p.m == 1 ? 8e7 : 1 << 25);
+}
+
 struct ForwardPlan {
     Operand x, w;
     size_t bytes;
@@ -633,7 +660,7 @@ struct ForwardPlan {
 ForwardPlan forward_plan(const gk_linear_t& p, void* workspace) {
     ForwardPlan f{};
     Arena arena(workspace);
-    f.few = p.m <= kFewRows;
+    f.few = few_rows_win(p);
     if (!f.few && p.dtype != GK_FP32) {
         f.x = operand(arena, p.x, p.x_stride, p.m, p.k);
         f.w = operand(arena, p.w, p.w_stride, p.n, p.k);
@@ -645,6 +672,7 @@ ForwardPlan forward_plan(const gk_linear_t& p, void* workspace) {
 template <typename T>
 int few_rows_by_m(const FewRows& f, cudaStream_t s) {
     if (f.m <= 1) return few_rows<T, 1>(f, s);
+    if (f.m <= 2) return few_rows<T, 2>(f, s);
     if (f.m <= 4) return few_rows<T, 4>(f, s);
     return few_rows<T, 8>(f, s);
 }

@@ -154,6 +154,31 @@ def test_tile_pairs(m, k, n, dtype):
     compare(make(m, k, n, dtype, bias=False), "tanh")
 
 
+# Few rows against wide weights: dot products, and tiles that hold all rows and
+# 128 weight rows, k shared by 1 to 8 CTAs in unequal parts; rows TMA cannot read.
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n", [(1, 8200, 24), (2, 4096, 160), (4, 4097, 1031), (8, 4104, 1100), (6, 4097, 4100),
+                                   (9, 64, 8), (12, 1000, 392), (16, 2048, 5000), (33, 4104, 129), (48, 640, 2048),
+                                   (47, 5000, 136), (49, 1024, 8192), (100, 1032, 8200), (128, 1025, 8193)])
+def test_few_rows_against_wide_weights(m, k, n, dtype):
+    compare(make(m, k, n, dtype), "gelu")
+    compare(make(m, k, n, dtype, bias=False, residual=False), "tanh")
+
+
+def test_rows_of_a_thin_product_do_not_touch_each_other():
+    """A row that is not a number, beside the last row and in front of none."""
+    x, w, b, _, _ = make(37, 512, 1000, torch.bfloat16, residual=False, grad=False)
+    from kingdom_ai import linear
+    want = linear(x, w, b)
+    spoilt = x.clone()
+    spoilt[36] = float("nan")
+    got = linear(spoilt, w, b)
+    assert torch.equal(got[:36], want[:36]) and bool(got[36].isnan().all())
+    wide = torch.full((37, 640), float("nan"), dtype=x.dtype, device="cuda")
+    wide[:, :512] = x
+    assert torch.equal(linear(wide[:, :512], w, b), want)
+
+
 @pytest.mark.parametrize("m,k,n", [(1025, 70, 1100), (3000, 48, 1300)])
 def test_large_fp32_tiles(m, k, n):
     compare(make(m, k, n, torch.float32), "tanh")
