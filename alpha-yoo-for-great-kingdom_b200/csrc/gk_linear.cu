@@ -154,9 +154,9 @@ int few_rows(FewRows p, cudaStream_t s) {
 
 struct Gemm32 {
     const float* a;
-    const float* b;
+    const void* b;       // of the kernel's type E, like out
     int64_t a_ld, b_ld;  // elements between rows of A and B, or between their k where m or n is contiguous
-    float* out;
+    void* out;
     const float* bias;
     const float* residual;
     float* pre;
@@ -180,12 +180,13 @@ struct Tile32 {
 };
 
 // One operand's B x 16 step, four neighbours at a time along its contiguous
-// dimension: k (K) or the row. VEC: those four are one aligned 16-byte load.
-template <int B, int P, bool K, bool VEC>
+// dimension: k (K) or the row. VEC: those four are one aligned load. 16-bit
+// elements (E) become fp32 as they arrive.
+template <typename E, int B, int P, bool K, bool VEC>
 struct Loader32 {
     using T = Tile32<B, P>;
     float v[T::kQuads][4];
-    const float* at[T::kQuads];  // this thread's first element of each group, now
+    const E* at[T::kQuads];  // this thread's first element of each group, now
     int left;                    // rows of the tile
     int64_t step;
     __device__ __forceinline__ static void place(int t, int i, int& row, int& k) {
@@ -195,7 +196,7 @@ struct Loader32 {
         else
             row = (q % (B / 4)) * 4, k = q / (B / 4);
     }
-    __device__ __forceinline__ void start(const float* p, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int t) {
+    __device__ __forceinline__ void start(const E* p, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int t) {
         step = K ? kStep : kStep * ld;
         left = rows - row0 < B ? (int)(rows - row0) : B;
 #pragma unroll
@@ -210,11 +211,16 @@ struct Loader32 {
         if (left == B && k_left >= kStep) {
 #pragma unroll
             for (int i = 0; i < T::kQuads; ++i) {
-                if (VEC) {
+                if constexpr (VEC && sizeof(E) == 4) {
                     *reinterpret_cast<float4*>(v[i]) = __ldg(reinterpret_cast<const float4*>(at[i]));
+                } else if constexpr (VEC) {
+                    alignas(8) E four[4];
+                    *reinterpret_cast<uint2*>(four) = __ldg(reinterpret_cast<const uint2*>(at[i]));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[i][j] = as_float<E>(four[j]);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[i][j] = __ldg(at[i] + j);
+                    for (int j = 0; j < 4; ++j) v[i][j] = as_float<E>(__ldg(at[i] + j));
                 }
                 at[i] += step;
             }
@@ -227,7 +233,7 @@ struct Loader32 {
             place(t, i, row, k);
             const int count = K ? (row < left ? k_end - k : 0) : (k < k_end ? left - row : 0);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[i][j] = j < count ? __ldg(at[i] + j) : 0.0f;
+            for (int j = 0; j < 4; ++j) v[i][j] = j < count ? as_float<E>(__ldg(at[i] + j)) : 0.0f;
             at[i] += step;
         }
     }
@@ -256,7 +262,7 @@ __device__ __forceinline__ void multiply_add(uint64_t& acc, uint64_t a, uint64_t
 }
 
 // Bias, residual, activation and stores of four neighbours of a row.
-__device__ __forceinline__ void finish4(const Gemm32& g, int64_t m, int64_t n, float (&v)[4]) {
+__device__ __forceinline__ void finish4_fp32(const Gemm32& g, int64_t m, int64_t n, float (&v)[4]) {
     const bool whole = g.wide && n + 4 <= g.n;
     const int count = g.n - n < 4 ? (int)(g.n - n) : 4;
 #pragma unroll
@@ -267,7 +273,7 @@ __device__ __forceinline__ void finish4(const Gemm32& g, int64_t m, int64_t n, f
         }
     }
     float* pre = g.pre == nullptr ? nullptr : g.pre + m * g.pre_ld + n;
-    float* out = g.out + m * g.out_ld + n;
+    float* out = static_cast<float*>(g.out) + m * g.out_ld + n;
     float y[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) y[j] = g.activation == GK_ACT_NONE ? v[j] : act_value<false>(v[j], g.activation);
@@ -288,7 +294,27 @@ __device__ __forceinline__ void finish4(const Gemm32& g, int64_t m, int64_t n, f
     }
 }
 
-template <int B, int P, bool AK, bool BK, bool VEC>
+// 16-bit results are gradients and have nothing but the rounding.
+template <typename E>
+__device__ __forceinline__ void finish4(const Gemm32& g, int64_t m, int64_t n, float (&v)[4]) {
+    if constexpr (sizeof(E) == 4) {
+        finish4_fp32(g, m, n, v);
+    } else {
+        E* out = static_cast<E*>(g.out) + m * g.out_ld + n;
+        alignas(8) E four[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) four[j] = rounded<E>(v[j]);
+        if (g.wide && n + 4 <= g.n) {
+            *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(four);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n + j < g.n) out[j] = four[j];
+        }
+    }
+}
+
+template <typename E, int B, int P, bool AK, bool BK, bool VEC>
 __global__ void __launch_bounds__(Tile32<B, P>::kThreads, P == 8 ? 512 / Tile32<B, P>::kThreads : 1)
     gemm32_kernel(Gemm32 g, int tiles_n) {
     extern __shared__ float smem[];
@@ -308,10 +334,10 @@ __global__ void __launch_bounds__(Tile32<B, P>::kThreads, P == 8 ? 512 / Tile32<
     for (int i = 0; i < P; ++i)
 #pragma unroll
         for (int j = 0; j < P / 2; ++j) acc[i][j] = 0ull;
-    Loader32<B, P, AK, VEC> la;
-    Loader32<B, P, BK, VEC> lb;
+    Loader32<float, B, P, AK, VEC> la;
+    Loader32<E, B, P, BK, VEC> lb;
     la.start(g.a, g.a_ld, m0, g.m, s0 * kStep, t);
-    lb.start(g.b, g.b_ld, n0, g.n, s0 * kStep, t);
+    lb.start(static_cast<const E*>(g.b), g.b_ld, n0, g.n, s0 * kStep, t);
     la.fetch(g.k - s0 * kStep, t);
     lb.fetch(g.k - s0 * kStep, t);
     for (int64_t s = s0; s < s1; ++s) {
@@ -351,7 +377,7 @@ __global__ void __launch_bounds__(Tile32<B, P>::kThreads, P == 8 ? 512 / Tile32<
             for (int q = 0; q < kParts; ++q) {
                 float v[4];
                 *reinterpret_cast<ulonglong2*>(v) = make_ulonglong2(acc[i][2 * q], acc[i][2 * q + 1]);
-                finish4(g, m, n0 + B / kParts * q + tx * 4, v);
+                finish4<E>(g, m, n0 + B / kParts * q + tx * 4, v);
             }
         }
         return;
@@ -373,15 +399,15 @@ __global__ void __launch_bounds__(Tile32<B, P>::kThreads, P == 8 ? 512 / Tile32<
             const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(smem, k) + r * kPitch + c);
             v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
         }
-        finish4(g, m0 + r, n0 + c, v);
+        finish4<E>(g, m0 + r, n0 + c, v);
     }
     cluster.sync();  // no CTA leaves while another reads its part
 }
 
-template <int B, int P, bool AK, bool BK, bool VEC>
+template <typename E, int B, int P, bool AK, bool BK, bool VEC>
 int launch_gemm32(const Gemm32& g, cudaStream_t s) {
     using T = Tile32<B, P>;
-    auto* kernel = gemm32_kernel<B, P, AK, BK, VEC>;
+    auto* kernel = gemm32_kernel<E, B, P, AK, BK, VEC>;
     static bool ready[64] = {};
     if (!once_per_device(ready, [&] {
             return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem) == cudaSuccess &&
@@ -419,9 +445,9 @@ int gemm32(const Gemm32& g, cudaStream_t s) {
     auto tiles = [&](int64_t b) { return ((g.m + b - 1) / b) * ((g.n + b - 1) / b); };
     const double work = (double)g.m * (double)g.n * (double)g.k;
     const double area128 = 16384.0 * tiles(128), area64 = 4096.0 * tiles(64), area32 = 1024.0 * tiles(32);
-    if (work < 134217728.0 || area64 >= 1.5 * area32) return launch_gemm32<32, 4, AK, BK, VEC>(g, s);
-    if (tiles(128) >= 32 && area128 <= 1.1 * area64) return launch_gemm32<128, 8, AK, BK, VEC>(g, s);
-    return launch_gemm32<64, 8, AK, BK, VEC>(g, s);
+    if (work < 134217728.0 || area64 >= 1.5 * area32) return launch_gemm32<float, 32, 4, AK, BK, VEC>(g, s);
+    if (tiles(128) >= 32 && area128 <= 1.1 * area64) return launch_gemm32<float, 128, 8, AK, BK, VEC>(g, s);
+    return launch_gemm32<float, 64, 8, AK, BK, VEC>(g, s);
 }
 template <bool AK, bool BK>
 int gemm32(Gemm32 g, cudaStream_t s) {
@@ -431,14 +457,23 @@ int gemm32(Gemm32 g, cudaStream_t s) {
     return vec ? gemm32<AK, BK, true>(g, s) : gemm32<AK, BK, false>(g, s);
 }
 
+// A small product of 16-bit gradients with dz in fp32.
+template <typename E, bool AK>
+int gemm32_narrow(Gemm32 g, cudaStream_t s) {
+    g.wide = aligned16(g.out) && g.out_ld % 4 == 0;
+    const bool vec = aligned16(g.a) && aligned16(g.b) && g.a_ld % 4 == 0 && g.b_ld % 4 == 0;
+    return vec ? launch_gemm32<E, 32, 4, AK, false, true>(g, s) : launch_gemm32<E, 32, 4, AK, false, false>(g, s);
+}
+
 // ------------------------------------------------------------ dz and db
 
 struct Slope {
     const void* dy;
     const void* kept;  // [m, n]; unused without activation
-    void* dz;          // or nullptr: sums only
+    void* dz;          // or nullptr
+    float* dz32;       // dz before its rounding, or nullptr
     float* sums;       // [slabs, n] column sums of each slab of rows, or nullptr
-    int64_t dy_stride, kept_stride, dz_stride;
+    int64_t dy_stride, kept_stride, dz_stride, dz32_stride;
     int64_t m, n, slab;  // rows of a slab
     int activation;
 };
@@ -446,6 +481,8 @@ struct Slope {
 // A warp goes down a slab of rows along 32 V columns; `across` of a block's
 // eight warps lie side by side (whole lines of a row next to one another), the
 // others take rows in turn.
+template <int ACT>
+constexpr bool kBends = ACT == GK_ACT_TANH || ACT == GK_ACT_GELU || ACT == GK_ACT_SILU;  // dz has more bits than dy
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(256, 4) linear_slope_kernel(Slope p, int across) {
     constexpr bool kSlope = ACT != GK_ACT_NONE;
@@ -488,14 +525,27 @@ __global__ void __launch_bounds__(256, 4) linear_slope_kernel(Slope p, int acros
             for (int u = 0; u < U; ++u) {
                 const int64_t row = r + u * step;
                 if (row >= r1) continue;
+                alignas(16) float z[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    float z = as_float<T>(dy[u][i]);
+                    z[i] = as_float<T>(dy[u][i]);
                     if constexpr (kSlope) {
-                        z *= act_slope<sizeof(T) == 2>(as_float<K>(kept[u][i]), ACT);
-                        dy[u][i] = rounded<T>(z);
+                        z[i] *= act_slope<sizeof(T) == 2>(as_float<K>(kept[u][i]), ACT);
+                        dy[u][i] = rounded<T>(z[i]);
                     }
-                    sum[i] += z;
+                    sum[i] += z[i];
+                }
+                if constexpr (kBends<ACT> && sizeof(T) == 2) {
+                    if (p.dz32 != nullptr) {
+                        float* at = p.dz32 + row * p.dz32_stride + c;
+                        if constexpr (V > 1) {
+#pragma unroll
+                            for (int i = 0; i < V; i += 4)
+                                *reinterpret_cast<float4*>(at + i) = make_float4(z[i], z[i + 1], z[i + 2], z[i + 3]);
+                        } else {
+                            at[0] = z[0];
+                        }
+                    }
                 }
                 if (p.dz != nullptr) {
                     if constexpr (V > 1)
@@ -688,6 +738,9 @@ bool forward_ok(const gk_linear_t* p) {
 struct BackwardPlan {
     bool forms_dz;    // dz is another matrix than dy
     Operand x, w, dz;
+    // Products of few outputs that take dz before its rounding, on the fp32 units.
+    bool narrow_dx, narrow_dw;
+    float* dz32;
     void* unpacked;   // x from its codes
     int64_t unpacked_ld;
     float* sums;
@@ -696,19 +749,39 @@ struct BackwardPlan {
     size_t bytes;
 };
 
+// The rounding of dz to 16 bits puts an error into a gradient as large as the
+// gradient's own rounding, 1.4 times in all; tcgen05 takes 16-bit operands, so a
+// product that it runs has to bear that. A narrow one, of few outputs or from
+// few dz (a head's, a short batch's), takes as long on the fp32 units and gets
+// dz in fp32 there, and its operands as they lie. Measured (us, fp32 units |
+// tcgen05 with its aligned copies): 7 x 4756 -> 17 both gradients 5.7 | 12.3, dw of
+// 1024 x 4000 -> 4 13.3 | 8.6, of 12616 x 2 -> 4 31 | 14, of 16384 x 128 -> 128 45 | 14,
+// dx of 4 x 4096 -> 4096 46 | 10: hence the bounds on the contraction and the work.
+bool narrow(int64_t rows, int64_t cols, int64_t contraction, int64_t dz) {
+    return (rows * cols <= 1 << 14 || dz <= 1 << 12) && contraction <= 4096 &&
+           (double)rows * (double)cols * (double)contraction <= 1 << 23;
+}
+
 template <typename T>
 BackwardPlan backward_plan(const gk_linear_grad_t& p, void* workspace) {
     constexpr bool k16 = sizeof(T) == 2;
     BackwardPlan b{};
     Arena arena(workspace);
-    const bool products = p.dx != nullptr || p.dw != nullptr;
+    if (k16 && (p.activation == GK_ACT_TANH || p.activation == GK_ACT_GELU || p.activation == GK_ACT_SILU)) {
+        b.narrow_dx = p.dx != nullptr && narrow(p.m, p.k, p.n, p.m * p.n);
+        b.narrow_dw = p.dw != nullptr && narrow(p.n, p.k, p.m, p.m * p.n);
+        if (b.narrow_dx || b.narrow_dw) b.dz32 = static_cast<float*>(arena.take(p.m * pad8(p.n) * 4));
+    }
+    const bool products = (p.dx != nullptr && !b.narrow_dx) || (p.dw != nullptr && !b.narrow_dw);
     // Without an activation dz is dy, unless the product needs its rows aligned.
     b.forms_dz = p.activation != GK_ACT_NONE || (k16 && products && !tma_rows(p.dy, p.dy_stride, p.n));
     b.dz = {p.dy, p.dy_stride, false};
     if (b.forms_dz) {
         // The residual's gradient serves as dz where its rows are aligned.
-        if (p.dz != nullptr && (!k16 || tma_rows(p.dz, p.n, p.n)))
+        if (p.dz != nullptr && (!k16 || !products || tma_rows(p.dz, p.n, p.n)))
             b.dz = {p.dz, p.n, false};
+        else if (b.dz32 != nullptr && !products)
+            b.dz = {nullptr, 0, false};
         else
             b.dz = {arena.take(p.m * pad8(p.n) * (int64_t)sizeof(T)), pad8(p.n), false};
     }
@@ -717,8 +790,12 @@ BackwardPlan backward_plan(const gk_linear_grad_t& p, void* workspace) {
         b.unpacked = arena.take(p.m * b.unpacked_ld * (int64_t)sizeof(T));
     }
     if (k16) {
-        if (p.dw != nullptr && p.x_codes == nullptr) b.x = operand(arena, p.x, p.x_stride, p.m, p.k);
-        if (p.dx != nullptr) b.w = operand(arena, p.w, p.w_stride, p.n, p.k);
+        if (p.dw != nullptr && !b.narrow_dw && p.x_codes == nullptr)
+            b.x = operand(arena, p.x, p.x_stride, p.m, p.k);
+        else
+            b.x = {p.x, p.x_stride, false};
+        b.w = {p.w, p.w_stride, false};
+        if (p.dx != nullptr && !b.narrow_dx) b.w = operand(arena, p.w, p.w_stride, p.n, p.k);
     } else {
         b.x = {p.x, p.x_stride, false};
         b.w = {p.w, p.w_stride, false};
@@ -750,7 +827,8 @@ int backward(const gk_linear_grad_t& p, void* workspace, uint32_t* status, cudaS
     int e = 0;
     if (b.runs_slope) {
         Slope a{p.dy, p.activation == GK_ACT_NONE ? nullptr : p.kept,
-                b.forms_dz ? const_cast<void*>(b.dz.p) : nullptr, b.sums, p.dy_stride, p.kept_stride, b.dz.ld, p.m, p.n,
+                b.forms_dz ? const_cast<void*>(b.dz.p) : nullptr, b.dz32, b.sums, p.dy_stride, p.kept_stride, b.dz.ld,
+                pad8(p.n), p.m, p.n,
                 b.slope.slab, p.activation};
         const dim3 grid((unsigned)b.slope.col_blocks, (unsigned)b.slope.slabs);
         if ((e = launch_slope<T>(a, grid, b.slope, s)) != 0) return e;
@@ -771,13 +849,24 @@ int backward(const gk_linear_grad_t& p, void* workspace, uint32_t* status, cudaS
         if (e != 0) return e;
     }
     if constexpr (k16) {
-        if (p.dx != nullptr) {
+        const Gemm32 none{};
+        if (b.narrow_dx) {
+            Gemm32 g = none;
+            g.a = b.dz32, g.b = b.w.p, g.a_ld = pad8(p.n), g.b_ld = b.w.ld, g.out = p.dx, g.out_ld = p.k;
+            g.m = p.m, g.n = p.k, g.k = p.n;
+            if ((e = gemm32_narrow<T, true>(g, s)) != 0) return e;
+        } else if (p.dx != nullptr) {
             if ((e = copy_if_needed(b.w, p.w, p.w_stride, p.n, p.k, s)) != 0) return e;
             GemmArgs g{b.dz.p, b.w.p, b.dz.ld, b.w.ld, 0, 1, p.dx, p.k, nullptr, nullptr, 0, nullptr, 0,
                        p.m, p.k, p.n, p.dtype, GK_ACT_NONE};
             if ((e = gemm16(g, status, s)) != 0) return e;
         }
-        if (p.dw != nullptr) {
+        if (b.narrow_dw) {
+            Gemm32 g = none;
+            g.a = b.dz32, g.b = b.x.p, g.a_ld = pad8(p.n), g.b_ld = b.x.ld, g.out = p.dw, g.out_ld = p.k;
+            g.m = p.n, g.n = p.k, g.k = p.m;
+            if ((e = gemm32_narrow<T, false>(g, s)) != 0) return e;
+        } else if (p.dw != nullptr) {
             if (p.x_codes == nullptr && (e = copy_if_needed(b.x, p.x, p.x_stride, p.m, p.k, s)) != 0) return e;
             GemmArgs g{b.dz.p, b.x.p, b.dz.ld, b.x.ld, 1, 1, p.dw, p.k, nullptr, nullptr, 0, nullptr, 0,
                        p.n, p.k, p.m, p.dtype, GK_ACT_NONE};

@@ -165,6 +165,25 @@ def test_few_rows_against_wide_weights(m, k, n, dtype):
     compare(make(m, k, n, dtype, bias=False, residual=False), "tanh")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n", [(7, 4000, 17), (1000, 64, 82), (4096, 3, 5), (1, 700, 300), (33, 81, 64)])
+def test_narrow_gradients_come_from_unrounded_dz(m, k, n, dtype):
+    """Few outputs or few dz: the gradients bear one rounding, their own (tanh keeps its value in fp32)."""
+    x, w, b, r, dy = make(m, k, n, dtype, residual=False)
+    got = run(x, w, b, r, dy, "tanh")
+    xd, wd, dyd = x.double(), w.double(), dy.double()
+    z, size = xd @ wd.t() + b.double(), xd.abs() @ wd.abs().t() + b.double().abs()
+    y, slope = act(z, "tanh")
+    dz = dyd * slope
+    # As in reference(), without the step that stores dz.
+    edz = dyd.abs() * (2 * (1.2 * (k + 4) * STEP * size + 2.0 ** -20) + 2.0 ** -20)
+    for key, a, ea, c, count in (("x", dz, edz, wd, n + 4), ("w", dz.t(), edz.t(), xd, m + 4)):
+        if got[key].numel() > 1 << 14 and m * n > 1 << 12:  # runs on 16-bit operands
+            continue
+        value, bound = a @ c, (ea + count * STEP * (a.abs() + ea)) @ c.abs()
+        check(got[key], value, stored(value, bound, dtype))
+
+
 def test_rows_of_a_thin_product_do_not_touch_each_other():
     """A row that is not a number, beside the last row and in front of none."""
     x, w, b, _, _ = make(37, 512, 1000, torch.bfloat16, residual=False, grad=False)
