@@ -402,7 +402,9 @@ __global__ void __launch_bounds__(kSplitThreads, 2) gemm_split_kernel(const __gr
 // A and half of B's rows, and the tensor cores of both read both halves, so an
 // SM stages half of what a tile of its own would need. Persistent: a pair walks
 // the tiles, and two accumulators in TMEM let the epilogue of one tile run
-// under the products of the next.
+// under the products of the next. Bound by the tensor cores: 8192 x 4096 -> 8192
+// bf16 with bias, residual, gelu and the kept sum 405 us (1360 TFLOP/s), dx 335
+// (1640), dW 383 (1435, both operands across).
 // Warp 0 loads, warp 1 of the even CTA issues the MMAs, warp 2 owns TMEM, warps
 // 4-11 are the epilogue: two warps a quadrant of 32 rows, each with half the columns.
 constexpr int kPairThreads = 384;

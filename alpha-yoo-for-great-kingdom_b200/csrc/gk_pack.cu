@@ -2,10 +2,11 @@
 //
 // A block of 32 values shares a power-of-two scale 2^s with
 // 448 2^(s-1) < max |x| <= 448 2^s, so a value x is held as e4m3(x 2^-s): three
-// fraction bits (relative step 2^-4) down to max |x| 2^-15, then evenly spaced
+// fraction bits (off by at most 2^-4 of itself) down to max |x| 2^-15, then evenly spaced
 // to 2^-18 of the maximum, below which it is held as zero. The scale being a
 // power of two, every held value is a bf16, fp16 and fp32 value: unpacking
-// rounds nothing. Memory traffic bounds both directions.
+// rounds nothing. Memory traffic bounds both directions: 8192 x 4096 bf16 packed
+// in 18 us (5.6 TB/s) and unpacked in 17 (6.0), 4096 x 5184 fp32 in 19 and 15.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

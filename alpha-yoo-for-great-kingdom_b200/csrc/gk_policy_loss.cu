@@ -400,7 +400,9 @@ __global__ void __launch_bounds__(256) policy_loss_sum_kernel(gk_policy_loss_t p
 
 // Rows of at most 32 * NPL entries: a warp holds its row in registers, so
 // logits, mask and target are read once and the gradient is written in the
-// same pass. Lane l holds entries l, l + 32, ...
+// same pass. Lane l holds entries l, l + 32, ... Bound by instructions (four
+// selects by mask and target an entry): 65536 x 82 fp32 with mask and target
+// 44 us, 1.6 TB/s of what it has to move; 256 rows 2.7 us.
 template <typename TL, typename TT, int NPL>
 __global__ void __launch_bounds__(kRowWarps * 32) policy_loss_rows_kernel(gk_policy_loss_t p) {
     __shared__ double sums[kRowWarps];
@@ -518,7 +520,11 @@ __device__ __forceinline__ void copy_async(uint4* to, const void* from) {
 // and a slot takes the next row's group as soon as this row's last pass has
 // read it: the loads of one row run under the stores of the row before.
 // Otherwise (a part past the shared memory, or rows that are not aligned) each
-// pass reads the row itself, from L2 where it fits.
+// pass reads the row itself, from L2 where it fits. Three CTAs of 256 threads an
+// SM: one's barrier and loads hide under the passes of the others. Bound by
+// instructions (some 17 an entry over its passes), close to HBM:
+// 4096 x 128000 bf16 433 us, 4.8 TB/s; 8192 x 1000 23 us; 1024 x 32771 fp16 with
+// target, which reads the target beside, 55 us; 7 x 100003, a few rows' latency, 6.7.
 template <typename TL, typename TT, int V, bool STAGED, int THREADS>
 __global__ void __launch_bounds__(THREADS, 3 * kLongThreads / THREADS) policy_loss_long_kernel(gk_policy_loss_t p,
                                                                                              int log_ranks) {
@@ -715,7 +721,9 @@ __global__ void __launch_bounds__(THREADS, 3 * kLongThreads / THREADS) policy_lo
 
 // The gradient from the saved row statistics, scaled by the upstream
 // gradient. A gradient that the forward pass wrote is for an upstream of one,
-// and is left as it is when that holds (`written`).
+// and is left as it is when that holds (`written`: 1.5 to 4 us for the blocks to
+// see it). fp16 gradients are made here only, where the upstream gradient (a loss
+// scale) is known: 1024 x 32771 with target 44 us, 4.5 TB/s.
 template <typename TL, typename TT, int V>
 __global__ void __launch_bounds__(256) policy_loss_backward_kernel(gk_policy_loss_t p, const float* upstream,
                                                                    int written) {
