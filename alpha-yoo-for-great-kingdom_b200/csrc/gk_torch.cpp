@@ -60,8 +60,13 @@ void used(const OptTensor& t, const c10::cuda::CUDAStream& stream) {
     if (has(t)) used(*t, stream);
 }
 
+// The kernels read memory: a lazily negated view (the imaginary part of a
+// conjugate) is negated first.
+Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+Tensor dense(const Tensor& t) { return plain(t).contiguous(); }
 // [rows, cols] with contiguous rows: a view where the layout allows, else a copy.
-Tensor rows_of(const Tensor& t, int64_t cols) {
+Tensor rows_of(const Tensor& given, int64_t cols) {
+    const Tensor t = plain(given);
     if (t.dim() != 2) return t.contiguous().view({-1, cols});
     return (t.stride(1) == 1 || cols == 1) && t.stride(0) >= 0 ? t : t.contiguous();
 }
@@ -107,7 +112,7 @@ std::tuple<Tensor, Tensor> pack(const Tensor& x) {
     TORCH_CHECK_VALUE(x.is_cuda() && type_of(x.scalar_type()) >= 0,
                       "pack_activation packs CUDA tensors of float32, bfloat16 or float16");
     const at::NoGradGuard no_grad;
-    const Tensor flat = x.contiguous();
+    const Tensor flat = dense(x);
     return pack_rows(flat, 1, flat.numel(), flat.numel());
 }
 
@@ -251,7 +256,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, cons
     const Tensor rows = rows_of(x, k), w = rows_of(weight, k);
     TORCH_CHECK_VALUE(rows.size(0) <= kMost && n <= kMost && k <= kMost, "linear takes sizes below 2**31");
     OptTensor b, r;
-    if (has(bias)) b = bias->contiguous();
+    if (has(bias)) b = dense(*bias);
     if (has(residual)) r = rows_of(*residual, n);
     Tensor y;
     if (at::GradMode::is_enabled() && (rows.requires_grad() || w.requires_grad() || (has(b) && b->requires_grad()) ||
@@ -362,7 +367,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
                 grad = at::empty(s[0].sizes(), s[0].options().requires_grad(false));
             }
             if (s[0].size(0) > 0) {
-                const Tensor upstream = grads[0].contiguous();
+                const Tensor upstream = dense(grads[0]);
                 gk_policy_loss_t p = loss_struct(s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7],
                                                  LossScalars{o[0], o[1], o[2], o[3], o[4]}, s[8]);
                 p.loss = p.stats;  // not written by the backward pass
@@ -389,7 +394,7 @@ OptTensor column(const char* name, const OptTensor& t, const Tensor& logits, at:
                       std::string(name) + " must have shape (" + std::to_string(logits.size(0)) + ",), dtype " +
                           c10::toString(dtype) + " and the logits' device");
     TORCH_CHECK_VALUE(!t->requires_grad(), std::string(name) + kNoGradient);
-    return t->contiguous();
+    return dense(*t);
 }
 
 OptTensor matrix(const char* name, const OptTensor& t, const Tensor& logits, bool fits) {

@@ -58,8 +58,9 @@ def linear(x, weight, bias=None, *, activation=None, residual=None, checkpoint=N
     for the backward pass in 8 bits (``pack_activation``, blocks along its last
     dimension): the weight's gradient is then that of the packed input, every
     other gradient is unchanged. The gradient of the sum is rounded to the
-    inputs' dtype before the products of the backward pass, and gelu and silu
-    take their derivative from the rounded sum. For that they keep one more
+    inputs' dtype before the products of the backward pass (not before narrow
+    ones, of few outputs), and gelu and silu take their derivative from the
+    rounded sum. For that they keep one more
     tensor of the output's size (tanh keeps one in fp32).
 
     Call it once on a device before capturing it in a CUDA graph. As with any

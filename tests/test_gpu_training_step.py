@@ -176,3 +176,26 @@ def test_refusals(batch):
             model, batch, value_weight="1"), lambda: policy_value_loss(model, batch.features)):
         with pytest.raises(TypeError):
             bad()
+
+
+def test_lazily_negated_views():
+    """The imaginary part of a conjugate holds the negated values."""
+    from kingdom_ai import linear, pack_activation, policy_loss
+    g = torch.Generator(device="cuda").manual_seed(0)
+
+    def negated(*shape):
+        t = torch.randn(shape, generator=g, device="cuda")
+        view = torch.complex(t, t).conj().imag
+        assert view.is_neg()
+        return view, torch.imag(torch.complex(t, t)).neg()
+
+    (x, x1), (w, w1), (b, b1), (r, r1) = negated(40, 64), negated(24, 64), negated(24), negated(40, 24)
+    assert torch.equal(linear(x, w, b, residual=r), linear(x1, w1, b1, residual=r1))
+    w2 = w1.clone().requires_grad_()
+    dy, dy1 = torch._neg_view(r), r1.neg()
+    assert torch.equal(torch.autograd.grad(linear(x, w2), w2, dy)[0], torch.autograd.grad(linear(x1, w2), w2, dy1)[0])
+    assert torch.equal(pack_activation(x).unpack(), pack_activation(x1).unpack())
+    actions = torch.arange(40, device="cuda") % 64
+    (old, old1), (adv, adv1) = negated(40), negated(40)
+    assert torch.equal(policy_loss(x, actions=actions, old_log_probs=old, advantages=adv).loss,
+                       policy_loss(x1, actions=actions, old_log_probs=old1, advantages=adv1).loss)
