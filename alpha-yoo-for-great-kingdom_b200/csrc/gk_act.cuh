@@ -58,6 +58,60 @@ __device__ __forceinline__ float act_value(float z, int act) {
     }
 }
 
+// Two floats in the halves of a register pair; an instruction on both rounds each like one of its own.
+__device__ __forceinline__ uint64_t two(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void halves(uint64_t v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float clamped_size(float z) {  // min(|z|, 32), NaN kept
+    float r;
+    asm("min.NaN.f32 %0, %1, 0f42000000;" : "=f"(r) : "f"(fabsf(z)));
+    return r;
+}
+// The quick gelu's derivative Phi(z) + z phi(z) for two values. With a = |z| and
+// h = e^(-a^2/2) (t Q(t) / 2 - a / sqrt(2 pi)) it is h for z < 0 and 1 - h for
+// z > 0, which 1/2 + copysign(1/2 - h, z) is on both sides. Past a = 32 h is 0.
+__device__ __forceinline__ void quick_gelu_slopes(float& z0, float& z1) {
+    const float a0 = clamped_size(z0), a1 = clamped_size(z1);
+    const uint64_t a = two(a0, a1);
+    float u0, u1, x0, x1;
+    halves(fma2(a, two(0.31819805153394639f, 0.31819805153394639f), two(1.0f, 1.0f)), u0, u1);
+    halves(mul2(mul2(a, two(-0.72134752044448170f, -0.72134752044448170f)), a), x0, x1);
+    const uint64_t t = two(quick_rcp(u0), quick_rcp(u1)), e = two(quick_ex2(x0), quick_ex2(x1));
+    uint64_t q = two(0.5f * 0.06631925f, 0.5f * 0.06631925f);
+    q = fma2(q, t, two(0.5f * -0.23788772f, 0.5f * -0.23788772f));
+    q = fma2(q, t, two(0.5f * 0.20455141f, 0.5f * 0.20455141f));
+    q = fma2(q, t, two(0.5f * 0.04441312f, 0.5f * 0.04441312f));
+    q = fma2(q, t, two(0.5f * 0.18637764f, 0.5f * 0.18637764f));
+    q = fma2(q, t, two(0.5f * 0.22879136f, 0.5f * 0.22879136f));
+    q = fma2(q, t, two(0.5f * 0.25351842f, 0.5f * 0.25351842f));
+    q = fma2(q, t, two(0.5f * 0.25391682f, 0.5f * 0.25391682f));
+    const uint64_t h = mul2(e, fma2(q, t, mul2(a, two(-0.39894228040143268f, -0.39894228040143268f))));
+    float d0, d1;
+    halves(fma2(h, two(-1.0f, -1.0f), two(0.5f, 0.5f)), d0, d1);
+    z0 = 0.5f + copysignf(d0, z0);
+    z1 = 0.5f + copysignf(d1, z1);
+}
+
 // The derivative, from what the forward pass kept: relu takes the output y,
 // tanh its value in fp32 (1 - y^2 of a rounded y near one has few right bits),
 // gelu and silu the sum z before the activation.

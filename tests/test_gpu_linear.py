@@ -310,6 +310,30 @@ def test_not_a_number_and_infinities_pass_through(dtype):
         assert bool(y[3].isinf().all()) and bool(y[rows].isfinite().all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("name", ["relu", "tanh", "gelu", "silu"])
+@pytest.mark.parametrize("cols", [64, 63])
+def test_derivative_of_every_value(cols, name, dtype):
+    """Every 16-bit value as the sum: in whole 16-byte groups, and one by one."""
+    from kingdom_ai import check_linear, linear
+    bits = torch.arange(-(1 << 15), 1 << 15, dtype=torch.int32).to(torch.int16).view(dtype).cuda()
+    bits = torch.cat([bits, bits.new_zeros(-len(bits) % cols)]).view(-1, cols)
+    r = bits.clone().requires_grad_()
+    zero = torch.zeros(len(bits), 8, dtype=dtype, device="cuda"), torch.zeros(cols, 8, dtype=dtype, device="cuda")
+    y = linear(*zero, activation=name, residual=r)
+    got, = torch.autograd.grad(y, r, torch.ones_like(y))
+    check_linear()
+    assert torch.equal(got.isnan(), bits.isnan() & torch.tensor(name != "relu", device="cuda"))
+    finite = bits.isfinite()
+    value = act(bits.double(), name)[1]
+    # 2^-20 of the derivative's terms, none above 1.2; tanh's own 2^-20 moves 1 - y^2 by twice that.
+    error = stored(value, torch.full_like(value, 1.2 * 2.0 ** -20 * (2 if name == "tanh" else 1)), dtype)
+    check(torch.where(finite, got, 0.0), torch.where(finite, value, 0.0), error.nan_to_num(0.0))
+    if name in ("gelu", "silu", "tanh"):
+        ends = got[bits == math.inf], got[bits == -math.inf]
+        assert ends[0].tolist() == [0.0 if name == "tanh" else 1.0] and ends[1].tolist() == [0.0]
+
+
 def test_another_stream_and_two_captured_graphs():
     from kingdom_ai import linear
     args = [make(300, 81, 64, torch.float16, residual=False, seed=s) for s in (1, 2)]
