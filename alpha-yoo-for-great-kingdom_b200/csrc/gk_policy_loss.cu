@@ -24,6 +24,7 @@
 #include <type_traits>
 
 #include "../../include/gk.h"
+#include "gk_act.cuh"
 #include "gk_launch.cuh"
 
 namespace gk {
@@ -80,6 +81,11 @@ struct Exp {
     }
     __device__ __forceinline__ float operator()(float x) const { return ex2(fmaf(x, scale, -offset)); }
     __device__ __forceinline__ float term(float x) const { return (*this)(x); }  // of the sum
+    __device__ __forceinline__ uint64_t pair(float x, float y) const {          // of both
+        float a, b;
+        halves(fma2(two(x, y), two(scale, scale), two(-offset, -offset)), a, b);
+        return two(ex2(a), ex2(b));
+    }
 };
 // fp32 logits: the difference first, which keeps the exponent's error at the
 // last bit of x - m; in the row's sum, which every log-probability is taken
@@ -355,10 +361,19 @@ __device__ __forceinline__ float inverse_denominator(const gk_policy_loss_t& p) 
 template <typename TL, typename TT, int V>
 __device__ __forceinline__ void gradient_group(const Group<TL, V>& h, const float (&t)[V], const Exp<TL>& e, float kp,
                                                float kt, float (&g)[V]) {
+    if constexpr (V > 1 && sizeof(TL) == 2) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        g[i] = kp * e(h.x(i));
-        if constexpr (!std::is_same<TT, None>::value) g[i] -= kt * t[i];
+        for (int i = 0; i < V; i += 2) {
+            uint64_t v = mul2(e.pair(h.x(i), h.x(i + 1)), two(kp, kp));
+            if constexpr (!std::is_same<TT, None>::value) v = fma2(two(t[i], t[i + 1]), two(-kt, -kt), v);
+            halves(v, g[i], g[i + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            g[i] = kp * e(h.x(i));
+            if constexpr (!std::is_same<TT, None>::value) g[i] -= kt * t[i];
+        }
     }
 }
 
@@ -521,10 +536,11 @@ __device__ __forceinline__ void copy_async(uint4* to, const void* from) {
 // read it: the loads of one row run under the stores of the row before.
 // Otherwise (a part past the shared memory, or rows that are not aligned) each
 // pass reads the row itself, from L2 where it fits. Three CTAs of 256 threads an
-// SM: one's barrier and loads hide under the passes of the others. Bound by
-// instructions (some 17 an entry over its passes), close to HBM:
-// 4096 x 128000 bf16 433 us, 4.8 TB/s; 8192 x 1000 23 us; 1024 x 32771 fp16 with
-// target, which reads the target beside, 55 us; 7 x 100003, a few rows' latency, 6.7.
+// SM: one's barrier and loads hide under the passes of the others. Issue slots are
+// 58% busy (some 17 instructions an entry over its passes, exponentials of 16-bit
+// logits in pairs) and HBM runs at three quarters of a copy's rate: 4096 x 128000
+// bf16 428 us, 4.9 TB/s; 8192 x 1000 23 us; 1024 x 32771 fp16 with target, which
+// reads the target beside, 52 us; 7 x 100003, a few rows' latency, 6.7.
 template <typename TL, typename TT, int V, bool STAGED, int THREADS>
 __global__ void __launch_bounds__(THREADS, 3 * kLongThreads / THREADS) policy_loss_long_kernel(gk_policy_loss_t p,
                                                                                              int log_ranks) {
@@ -592,10 +608,16 @@ __global__ void __launch_bounds__(THREADS, 3 * kLongThreads / THREADS) policy_lo
         for (int o = 16; o; o >>= 1) acc.m = fmaxf(acc.m, __shfl_xor_sync(kFull, acc.m, o));
         {
             const Exp<TL> e(acc.m);
-            float s2 = 0.0f;
+            uint64_t s2 = two(0.0f, 0.0f);
             groups([&](const Group<TL, V>& h, int first, bool edge) {
+                if constexpr (V > 1 && sizeof(TL) == 2) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) (i & 1 ? s2 : acc.s) += e.term(h.x(i));
+                    for (int i = 0; i < V; i += 2) s2 = add2(s2, e.pair(h.x(i), h.x(i + 1)));
+                } else {
+#pragma unroll
+                    for (int i = 0; i + 1 < V; i += 2) s2 = add2(s2, two(e.term(h.x(i)), e.term(h.x(i + 1))));
+                    if constexpr (V == 1) acc.s += e.term(h.x(0));
+                }
                 if constexpr (kTarget) {
                     float t[V];
                     load_target<TT, V>(part.trow, h.legal, first, edge, t);
@@ -606,7 +628,9 @@ __global__ void __launch_bounds__(THREADS, 3 * kLongThreads / THREADS) policy_lo
                     }
                 }
             });
-            acc.s = warp_sum(acc.s + s2) * e.correct;
+            float even, odd;
+            halves(s2, even, odd);
+            acc.s = warp_sum(acc.s + even + odd) * e.correct;
         }
         if (kTarget) {
             total_t = warp_sum(total_t);
