@@ -87,17 +87,13 @@ __device__ __forceinline__ float clamped_size(float z) {  // min(|z|, 32), NaN k
     asm("min.NaN.f32 %0, %1, 0f42000000;" : "=f"(r) : "f"(fabsf(z)));
     return r;
 }
-// The quick gelu's derivative Phi(z) + z phi(z) for two values. With a = |z| and
-// h = e^(-a^2/2) (t Q(t) / 2 - a / sqrt(2 pi)) it is h for z < 0 and 1 - h for
-// z > 0, which 1/2 + copysign(1/2 - h, z) is on both sides. Past a = 32 h is 0.
-__device__ __forceinline__ void quick_gelu_slopes(float& z0, float& z1) {
-    const float a0 = clamped_size(z0), a1 = clamped_size(z1);
-    const uint64_t a = two(a0, a1);
+// e^(-a^2/2) and t Q(t) / 2 (see quick_cdf) for two a = min(|z|, 32), where both have long been 0 beyond.
+__device__ __forceinline__ void quick_tails(uint64_t a, uint64_t& e, uint64_t& t, uint64_t& q) {
     float u0, u1, x0, x1;
     halves(fma2(a, two(0.31819805153394639f, 0.31819805153394639f), two(1.0f, 1.0f)), u0, u1);
     halves(mul2(mul2(a, two(-0.72134752044448170f, -0.72134752044448170f)), a), x0, x1);
-    const uint64_t t = two(quick_rcp(u0), quick_rcp(u1)), e = two(quick_ex2(x0), quick_ex2(x1));
-    uint64_t q = two(0.5f * 0.06631925f, 0.5f * 0.06631925f);
+    t = two(quick_rcp(u0), quick_rcp(u1)), e = two(quick_ex2(x0), quick_ex2(x1));
+    q = two(0.5f * 0.06631925f, 0.5f * 0.06631925f);
     q = fma2(q, t, two(0.5f * -0.23788772f, 0.5f * -0.23788772f));
     q = fma2(q, t, two(0.5f * 0.20455141f, 0.5f * 0.20455141f));
     q = fma2(q, t, two(0.5f * 0.04441312f, 0.5f * 0.04441312f));
@@ -105,6 +101,24 @@ __device__ __forceinline__ void quick_gelu_slopes(float& z0, float& z1) {
     q = fma2(q, t, two(0.5f * 0.22879136f, 0.5f * 0.22879136f));
     q = fma2(q, t, two(0.5f * 0.25351842f, 0.5f * 0.25351842f));
     q = fma2(q, t, two(0.5f * 0.25391682f, 0.5f * 0.25391682f));
+}
+// The quick gelu for two values: z Phi(z) = (z + |z|) / 2 - |z| Phi(-|z|), which keeps
+// the far negative side's relative accuracy, and NaN for -inf as the product has it.
+__device__ __forceinline__ void quick_gelus(float& z0, float& z1) {
+    const uint64_t a = two(clamped_size(z0), clamped_size(z1)), half = two(0.5f, 0.5f);
+    uint64_t e, t, q;
+    quick_tails(a, e, t, q);
+    const uint64_t positive = fma2(two(fabsf(z0), fabsf(z1)), half, mul2(two(z0, z1), half));
+    const uint64_t h = mul2(mul2(e, t), q);
+    halves(fma2(mul2(a, two(-1.0f, -1.0f)), h, positive), z0, z1);
+}
+// The quick gelu's derivative Phi(z) + z phi(z) for two values. With a = |z| and
+// h = e^(-a^2/2) (t Q(t) / 2 - a / sqrt(2 pi)) it is h for z < 0 and 1 - h for
+// z > 0, which 1/2 + copysign(1/2 - h, z) is on both sides.
+__device__ __forceinline__ void quick_gelu_slopes(float& z0, float& z1) {
+    const uint64_t a = two(clamped_size(z0), clamped_size(z1));
+    uint64_t e, t, q;
+    quick_tails(a, e, t, q);
     const uint64_t h = mul2(e, fma2(q, t, mul2(a, two(-0.39894228040143268f, -0.39894228040143268f))));
     float d0, d1;
     halves(fma2(h, two(-1.0f, -1.0f), two(0.5f, 0.5f)), d0, d1);

@@ -472,7 +472,12 @@ __device__ __forceinline__ void tile_at(int id, int tiles_m, int tiles_n, int& t
 template <int ACT>
 __device__ __forceinline__ void activate(float (&v)[32]) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = act_value<true>(v[i], ACT);
+    for (int i = 0; i < 32; i += 2) {
+        if constexpr (ACT == GK_ACT_GELU)
+            quick_gelus(v[i], v[i + 1]);
+        else
+            v[i] = act_value<true>(v[i], ACT), v[i + 1] = act_value<true>(v[i + 1], ACT);
+    }
 }
 __device__ __forceinline__ void activate(float (&v)[32], int act) {
     switch (act) {
