@@ -704,13 +704,14 @@ __global__ void __launch_bounds__(THREADS, 3 * kLongThreads / THREADS) policy_lo
                     finish(h, base + k * V, false);
                     if (k < next_count) copy_async(staged + k, next_from + k * V);
                 }
+                // And its slots past this row's part: where the next row's shift saves a group, every part but the
+                // last can be one shorter, so the last begins earlier and can be up to ranks - 1 longer.
+                for (; k < next_count; k += THREADS) copy_async(staged + k, next_from + k * V);
             };
             if (part.mrow == nullptr)
                 last_pass(std::false_type());
             else
                 last_pass(std::true_type());
-            // An odd row's part may be a group longer than the one before it.
-            if (count < next_count && tid == count % THREADS) copy_async(staged + count, next_from + count * V);
             edges(finish);
             if (o.action >= 0) {
                 // The action's own part: the thread that wrote its group writes it again.

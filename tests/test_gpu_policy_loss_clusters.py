@@ -1,0 +1,30 @@
+"""policy_loss on rows that a cluster of CTAs shares, with more rows than the
+clusters that the device holds at once: each CTA then takes its part of the
+next row while it finishes this one. Compared with the formula in 64 bits, at
+the tolerances of test_gpu_policy_loss.py."""
+
+import pytest
+import torch
+
+from test_gpu_policy_loss import compare, make
+
+pytestmark = pytest.mark.gpu
+
+
+# Four and eight CTAs a row and an odd stride, so that rows start at every
+# shift to a 16-byte boundary. At these lengths the number of 16-byte groups of
+# a row passes a multiple of the CTAs with its shift, and with it where every
+# part begins: the last CTA's part of the next row is up to seven groups longer.
+ODD = [(300, 131071, torch.bfloat16), (1000, 83197, torch.bfloat16), (600, 99999, torch.bfloat16),
+       (480, 229375, torch.bfloat16), (300, 65535, torch.float32), (600, 50255, torch.float32),
+       (400, 99999, torch.float32)]
+
+
+@pytest.mark.parametrize("n,a,dtype", ODD)
+def test_parts_that_grow_from_row_to_row(n, a, dtype):
+    compare(*make(n, a, dtype))
+
+
+@pytest.mark.parametrize("n,a,dtype", [(300, 131071, torch.bfloat16), (300, 65535, torch.float32)])
+def test_parts_that_grow_with_mask_and_target(n, a, dtype):
+    compare(*make(n, a, dtype, mask=True, clipped=True, target=dtype))
