@@ -546,6 +546,10 @@ __global__ void __launch_bounds__(THREADS, 3 * kLongThreads / THREADS) policy_lo
                                                                                              int log_ranks) {
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = 1 << log_ranks, rank = log_ranks == 0 ? 0 : (int)cluster.block_rank();
+    // Another CTA's shared memory may be written once that CTA runs: all arrive here, and wait for the others
+    // under the first row's loads.
+    bool all_run = ranks == 1;
+    if (!all_run) cluster.barrier_arrive();
     constexpr bool kTarget = !std::is_same<TT, None>::value;
     constexpr int kWarps = THREADS / 32;
     extern __shared__ uint4 staged[];
@@ -638,6 +642,8 @@ __global__ void __launch_bounds__(THREADS, 3 * kLongThreads / THREADS) policy_lo
         }
         const float4 mine = make_float4(acc.m, acc.s, total_t, kl);
         if (ranks > 1) {
+            if (!all_run) cluster.barrier_wait();
+            all_run = true;
             if (lane < ranks) cluster.map_shared_rank(found[turn], lane)[rank * kWarps + warp] = mine;
             cluster.sync();
         } else {

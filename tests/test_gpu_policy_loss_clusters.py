@@ -6,7 +6,7 @@ the tolerances of test_gpu_policy_loss.py."""
 import pytest
 import torch
 
-from test_gpu_policy_loss import compare, make
+from test_gpu_policy_loss import compare, make, run
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +28,16 @@ def test_parts_that_grow_from_row_to_row(n, a, dtype):
 @pytest.mark.parametrize("n,a,dtype", [(300, 131071, torch.bfloat16), (300, 65535, torch.float32)])
 def test_parts_that_grow_with_mask_and_target(n, a, dtype):
     compare(*make(n, a, dtype, mask=True, clipped=True, target=dtype))
+
+
+# Two, four and eight CTAs a row with the fewest and with many rows each, the same parts in every row: the
+# exchange of what the CTAs found, from the first row on.
+@pytest.mark.parametrize("n,a,dtype", [(1, 131072, torch.bfloat16), (40, 65536, torch.bfloat16),
+                                       (900, 65536, torch.bfloat16), (500, 131072, torch.bfloat16),
+                                       (300, 98304, torch.float32), (3, 20000, torch.float32)])
+def test_parts_meet_from_the_first_row_on(n, a, dtype):
+    logits, args = make(n, a, dtype)
+    first = compare(logits, args)
+    for _ in range(5):
+        again = run(logits, args)
+        assert torch.equal(again[0].loss.detach(), first[0].loss) and torch.equal(again[1], first[1])
