@@ -358,11 +358,12 @@ __global__ void __launch_bounds__(kSplitThreads, 2) gemm_split_kernel(const __gr
         commit<false>(smem_u32(&done));
     }
     __syncwarp();
-    // Everyone waits for the accumulator: the parts overwrite the stages.
-    mbar_wait(smem_u32(&done), 0, status);
+    // Everyone waits for the accumulator: the parts overwrite the stages. The verdict is the warp's, which the
+    // loads from TMEM need whole. Where it did not come, MMAs may still read the stages: they are left as they are.
+    const bool complete = __all_sync(0xffffffffu, mbar_wait(smem_u32(&done), 0, status));
     tc_fence_after();
     float* part = reinterpret_cast<float*>(base);
-    if (warp >= 2) {
+    if (warp >= 2 && complete) {
         const int quadrant = warp & 3, row = quadrant * 32 + lane;
         for (int c = (warp - 2) / 4 * 32; c < shape.bn; c += 64) {
             float v[32];
