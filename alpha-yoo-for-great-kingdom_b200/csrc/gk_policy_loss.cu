@@ -26,6 +26,7 @@
 #include "../../include/gk.h"
 #include "gk_act.cuh"
 #include "gk_launch.cuh"
+#include "gk_row_part.cuh"
 
 namespace gk {
 namespace {
@@ -500,26 +501,17 @@ __global__ void __launch_bounds__(kRowWarps * 32) policy_loss_rows_kernel(gk_pol
     }
 }
 
-// The part of a row that one CTA of a cluster takes: groups of V entries that
-// start on 16-byte boundaries of the logits. Groups [full, full_end) lie in the
-// row; a group before or after them is the row's ragged edge.
+// The part of a row that one CTA of a cluster takes, and its operands' rows.
 template <typename TL, typename TT, int V>
-struct Part {
+struct Part : RowPart<V> {
     const TL* lrow;
     const uint8_t* mrow;
     const TT* trow;
-    int shift, begin, end, full, full_end;
-    __device__ __forceinline__ Part(const gk_policy_loss_t& p, int64_t r, int rank, int log_ranks) {
+    __device__ __forceinline__ Part(const gk_policy_loss_t& p, int64_t r, int rank, int log_ranks)
+        : RowPart<V>(r, p.logits_stride, (int)p.cols, rank, log_ranks) {
         lrow = static_cast<const TL*>(p.logits) + r * p.logits_stride;
         mrow = p.mask == nullptr ? nullptr : p.mask + r * p.mask_stride;
         trow = std::is_same<TT, None>::value ? nullptr : static_cast<const TT*>(p.target) + r * p.target_stride;
-        const int cols = (int)p.cols;
-        shift = (int)((uint32_t)r * (uint32_t)p.logits_stride % V);
-        const int groups = (cols + shift + V - 1) / V, each = (groups + (1 << log_ranks) - 1) >> log_ranks;
-        begin = min(groups, rank * each);
-        end = min(groups, begin + each);
-        full = max(begin, shift > 0 ? 1 : 0);
-        full_end = min(end, (cols + shift) / V);
     }
 };
 
@@ -710,9 +702,7 @@ __global__ void __launch_bounds__(THREADS, 3 * kLongThreads / THREADS) policy_lo
                     finish(h, base + k * V, false);
                     if (k < next_count) copy_async(staged + k, next_from + k * V);
                 }
-                // And its slots past this row's part: where the next row's shift saves a group, every part but the
-                // last can be one shorter, so the last begins earlier and can be up to ranks - 1 longer.
-                for (; k < next_count; k += THREADS) copy_async(staged + k, next_from + k * V);
+                fill_past<THREADS>(tid, count, next_count, [&](int q) { copy_async(staged + q, next_from + q * V); });
             };
             if (part.mrow == nullptr)
                 last_pass(std::false_type());
