@@ -90,6 +90,14 @@ variable_list once(variable_list grads, const char* name) {
     return grads;
 }
 
+// There are no forward-mode derivatives. An output without a tangent would stand for a derivative of zero.
+bool tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool tangent(const OptTensor& t) { return t.has_value() && tangent(*t); }
+template <typename... T>
+void no_tangent(const char* name, const T&... inputs) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!(tangent(inputs) || ...), std::string(name) + " has no forward-mode derivative");
+}
+
 // ------------------------------------------------------------------ pack
 
 // Codes, then scales, of [rows, cols] with rows `stride` elements apart.
@@ -253,6 +261,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, cons
                               residual->sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1),
                           "residual must have the output's shape");
     }
+    no_tangent("linear", x, weight, bias, residual);
     const Tensor rows = rows_of(x, k), w = rows_of(weight, k);
     TORCH_CHECK_VALUE(rows.size(0) <= kMost && n <= kMost && k <= kMost, "linear takes sizes below 2**31");
     OptTensor b, r;
@@ -427,6 +436,7 @@ std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits, const OptTensor& le
                           "denominator must hold one float32 on the logits' device");
         TORCH_CHECK_VALUE(!denominator_tensor->requires_grad(), "denominator must not require a gradient");
     }
+    no_tangent("policy_loss", logits, old, advantages, reference, target, denominator_tensor);
     const Tensor z = rows_of(logits, logits.size(1));
     const OptTensor mask = matrix("legal_mask", legal_mask, logits,
                                   has(legal_mask) && legal_mask->scalar_type() == at::kBool);

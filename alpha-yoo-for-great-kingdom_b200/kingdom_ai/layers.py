@@ -63,6 +63,9 @@ def linear(x, weight, bias=None, *, activation=None, residual=None, checkpoint=N
     rounded sum. For that they keep one more
     tensor of the output's size (tanh keeps one in fp32).
 
+    Second derivatives and forward-mode ones (a tensor that carries a tangent)
+    are refused.
+
     Call it once on a device before capturing it in a CUDA graph. As with any
     operator, capture a backward pass only when no graph of the same leaves
     made outside the capture is alive (drop earlier outputs first): autograd

@@ -75,6 +75,9 @@ def policy_loss(logits, *, legal_mask=None, actions=None, old_log_probs=None, ad
     the backward pass). ``logits`` and the other arguments must not change in
     place before that.
 
+    Second derivatives and forward-mode ones (a tensor that carries a tangent)
+    are refused.
+
     Rows with unit column stride are read in place; others are copied first.
     """
     global _operator

@@ -1,0 +1,31 @@
+"""The training-step operators among PyTorch's own machinery: forward-mode
+derivatives, saved-tensor hooks, inference mode, layouts that a view can have."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def test_forward_mode_derivatives_are_refused():
+    """An output without a tangent would stand for a derivative of zero."""
+    import torch.autograd.forward_ad as forward_ad
+    from kingdom_ai import linear, policy_loss
+    x, w, b, r = (torch.randn(s, device="cuda") for s in ((12, 16), (8, 16), (8,), (12, 8)))
+    target = torch.softmax(torch.randn(12, 16, device="cuda"), 1)
+    want, loss = linear(x, w, b, residual=r), policy_loss(x, target=target).loss
+    with forward_ad.dual_level():
+        for i in range(4):
+            args = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate((x, w, b, r))]
+            for grad in (False, True):  # whether autograd records or not
+                args[0 if i else 1] = args[0 if i else 1].detach().requires_grad_(grad)
+                with pytest.raises(NotImplementedError):
+                    linear(*args[:3], residual=args[3])
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError):
+            policy_loss(dual, target=target)
+        with pytest.raises(NotImplementedError):
+            policy_loss(x, target=forward_ad.make_dual(target, torch.ones_like(target)))
+        # Without a tangent they run inside the level too.
+        assert torch.equal(linear(x, w, b, residual=r), want) and torch.equal(policy_loss(x, target=target).loss, loss)
+        assert torch.equal(linear(forward_ad.unpack_dual(dual).primal, w, b, residual=r), want)
