@@ -100,8 +100,12 @@ void no_tangent(const char* name, const T&... inputs) {
 
 // ------------------------------------------------------------------ pack
 
-// Codes, then scales, of [rows, cols] with rows `stride` elements apart.
-std::tuple<Tensor, Tensor> pack_rows(const Tensor& x, int64_t rows, int64_t cols, int64_t stride) {
+// Codes, then scales, of [rows, cols] with rows `stride` elements apart. Rows that lie over one another (an
+// expanded or unfolded tensor) are copied apart first, which gk_pack asks for.
+std::tuple<Tensor, Tensor> pack_rows(const Tensor& given, int64_t rows, int64_t cols, int64_t given_stride) {
+    const bool apart = rows <= 1 || given_stride >= cols;
+    const Tensor x = apart ? given : given.contiguous();
+    const int64_t stride = apart ? given_stride : cols;
     const int64_t scales = rows * ((cols + 31) / 32);
     Tensor buffer = bytes_on(rows * cols + scales, x);
     Tensor codes = buffer.narrow(0, 0, rows * cols), factor = buffer.narrow(0, rows * cols, scales);

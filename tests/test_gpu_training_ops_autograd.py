@@ -29,3 +29,18 @@ def test_forward_mode_derivatives_are_refused():
         # Without a tangent they run inside the level too.
         assert torch.equal(linear(x, w, b, residual=r), want) and torch.equal(policy_loss(x, target=target).loss, loss)
         assert torch.equal(linear(forward_ad.unpack_dual(dual).primal, w, b, residual=r), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_packed_inputs_whose_rows_lie_over_one_another(dtype):
+    """Expanded and unfolded inputs, as linear takes them without a checkpoint."""
+    from kingdom_ai import linear
+    g = torch.Generator(device="cuda").manual_seed(1)
+    flat = torch.randn(400, generator=g, device="cuda").to(dtype)
+    w = (torch.randn((24, 40), generator=g, device="cuda") * 0.2).to(dtype).requires_grad_()
+    dy = torch.randn((64, 24), generator=g, device="cuda").to(dtype)
+    for x in (flat[:40].expand(64, 40), flat.unfold(0, 40, 5)[:64], torch.as_strided(flat, (64, 40), (0, 1), 7)):
+        y, z = linear(x, w, activation="gelu", checkpoint="e4m3"), linear(x.contiguous(), w, activation="gelu",
+                                                                          checkpoint="e4m3")
+        assert torch.equal(y, z)
+        assert torch.equal(torch.autograd.grad(y, w, dy)[0], torch.autograd.grad(z, w, dy)[0])
