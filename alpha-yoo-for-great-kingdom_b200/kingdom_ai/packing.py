@@ -88,7 +88,7 @@ def packed_activations(min_elements: int = 1 << 16):
     def pack(t):
         if (t.device.type != "cuda" or t.dtype not in _PACKED_TYPES or t.numel() < min_elements
                 or t.layout != torch.strided or _is_parameter(t)):
-            return t
+            return t.detach()  # an operator's own output would keep itself alive
         return pack_activation(t)
 
     def unpack(kept):
@@ -110,6 +110,6 @@ def packing_active() -> bool:
 
 def keep_saved_tensors():
     """A context in which saved tensors are kept as they are inside packed_activations."""
-    return torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t)
+    return torch.autograd.graph.saved_tensors_hooks(torch.Tensor.detach, lambda t: t)
 
 

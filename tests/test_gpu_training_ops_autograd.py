@@ -44,3 +44,24 @@ def test_packed_inputs_whose_rows_lie_over_one_another(dtype):
                                                                           checkpoint="e4m3")
         assert torch.equal(y, z)
         assert torch.equal(torch.autograd.grad(y, w, dy)[0], torch.autograd.grad(z, w, dy)[0])
+
+
+@pytest.mark.parametrize("name", ["relu", "tanh", None])
+def test_graphs_dropped_inside_packed_activations_are_freed(name):
+    from kingdom_ai import linear, packed_activations, policy_loss
+    x = torch.randn(64, 96, device="cuda")
+    w = torch.randn(32, 96, device="cuda", requires_grad=True)
+    target = torch.softmax(torch.randn(64, 32, device="cuda"), 1)
+
+    def forward():  # an evaluation that never runs its backward pass
+        with packed_activations():
+            y = linear(x, w, activation=name)
+            policy_loss(torch.relu(y), target=target)
+
+    forward()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(5):
+        forward()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before
