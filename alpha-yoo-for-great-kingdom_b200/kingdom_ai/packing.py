@@ -59,6 +59,24 @@ def pack_activation(x: torch.Tensor) -> PackedActivation:
     return PackedActivation(codes, scales, x.shape, x.dtype)
 
 
+class _Kept:
+    """A saved tensor as it is. Detached, for an operator's own output would
+    keep itself alive; with its version, which autograd does not check where
+    hooks save."""
+
+    __slots__ = ("tensor", "version")
+
+    def __init__(self, t):
+        self.tensor, self.version = t.detach(), t._version
+
+    def unpack(self) -> torch.Tensor:
+        if self.tensor._version != self.version:
+            raise RuntimeError(f"a tensor of shape {tuple(self.tensor.shape)} that was kept for the backward pass has "
+                               f"been modified by an inplace operation: it is at version {self.tensor._version}, and "
+                               f"was kept at version {self.version}")
+        return self.tensor
+
+
 def _is_parameter(t: torch.Tensor) -> bool:
     """A parameter, a leaf that is being trained, a view of one, or one cast to another type (autocast)."""
     base = t if t._base is None else t._base
@@ -88,14 +106,11 @@ def packed_activations(min_elements: int = 1 << 16):
     def pack(t):
         if (t.device.type != "cuda" or t.dtype not in _PACKED_TYPES or t.numel() < min_elements
                 or t.layout != torch.strided or _is_parameter(t)):
-            return t.detach()  # an operator's own output would keep itself alive
+            return _Kept(t)
         return pack_activation(t)
 
-    def unpack(kept):
-        return kept.unpack() if isinstance(kept, PackedActivation) else kept
-
     depth = getattr(_active, "depth", 0)
-    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda kept: kept.unpack()):
         _active.depth = depth + 1
         try:
             yield
@@ -110,6 +125,6 @@ def packing_active() -> bool:
 
 def keep_saved_tensors():
     """A context in which saved tensors are kept as they are inside packed_activations."""
-    return torch.autograd.graph.saved_tensors_hooks(torch.Tensor.detach, lambda t: t)
+    return torch.autograd.graph.saved_tensors_hooks(_Kept, lambda kept: kept.unpack())
 
 

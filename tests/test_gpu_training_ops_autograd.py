@@ -65,3 +65,19 @@ def test_graphs_dropped_inside_packed_activations_are_freed(name):
         forward()
     torch.cuda.synchronize()
     assert torch.cuda.memory_allocated() == before
+
+
+def test_changes_in_place_are_refused_inside_packed_activations():
+    from kingdom_ai import linear, packed_activations, policy_loss
+    x = torch.randn(20, 32, device="cuda")
+    w = torch.randn(16, 32, device="cuda", requires_grad=True)
+    target = torch.softmax(torch.randn(20, 16, device="cuda"), 1)
+    with packed_activations():
+        y = linear(x, w, activation="relu")
+        y.neg_()  # its slope is taken from the kept output
+        z = linear(x, w)
+        loss = policy_loss(z, target=target).loss
+        z.add_(1)
+    for out in (y.sum(), loss):
+        with pytest.raises(RuntimeError, match="inplace"):
+            out.backward()
