@@ -192,7 +192,8 @@ struct Linear : torch::autograd::Function<Linear> {
         Tensor codes, scales;
         if (need_w && packed) std::tie(codes, scales) = pack_rows(x, m, k, row_stride(x, k));
         ctx->save_for_backward({need_w && !packed ? x : Tensor(), need_x ? w : Tensor(),
-                                activation == GK_ACT_NONE ? Tensor() : (pre.defined() ? pre : y), codes, scales, status});
+                                activation == GK_ACT_NONE ? Tensor() : (pre.defined() ? pre : y), codes, scales});
+        ctx->saved_data["status"] = status;  // not an input: a call may have made it in inference mode, another may clear it
         ctx->saved_data["sizes"] = std::vector<int64_t>{m, w.size(0), k, activation, need_x, need_w,
                                                         has(bias) && bias->requires_grad(),
                                                         has(residual) && residual->requires_grad()};
@@ -234,7 +235,7 @@ struct Linear : torch::autograd::Function<Linear> {
                 if (size > 0) workspace = bytes_on((int64_t)size, dy);
                 used(dy, stream);
                 ran("gk_linear_backward",
-                    gk_linear_backward(&p, data(workspace), static_cast<uint32_t*>(saved[5].data_ptr()),
+                    gk_linear_backward(&p, data(workspace), static_cast<uint32_t*>(ctx->saved_data["status"].toTensor().data_ptr()),
                                        stream.stream()));
             }
         }

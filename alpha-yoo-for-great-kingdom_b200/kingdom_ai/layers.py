@@ -24,7 +24,8 @@ def _status_words(device) -> torch.Tensor:
     if words is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("call linear once on this device before capturing it in a CUDA graph")
-        words = torch.zeros(2, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # check_linear clears it in any mode
+            words = torch.zeros(2, dtype=torch.int32, device=device)
         torch.cuda.current_stream(device).synchronize()
         words = _status.setdefault(device.index, words)
     return words

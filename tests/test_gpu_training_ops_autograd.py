@@ -81,3 +81,27 @@ def test_changes_in_place_are_refused_inside_packed_activations():
     for out in (y.sum(), loss):
         with pytest.raises(RuntimeError, match="inplace"):
             out.backward()
+
+
+def test_training_after_a_first_call_in_inference_mode():
+    from kingdom_ai import check_linear, layers, linear
+    x = torch.randn(20, 32, device="cuda")
+    w = torch.randn(16, 32, device="cuda", requires_grad=True)
+    want, = torch.autograd.grad(linear(x, w, activation="tanh").sum(), w)
+    kept = dict(layers._status)
+    layers._status.clear()
+    try:
+        with torch.inference_mode():  # serving comes first
+            linear(x, w, activation="tanh")
+        got, = torch.autograd.grad(linear(x, w, activation="tanh").sum(), w)
+        assert torch.equal(got, want)
+        # An error of another call, reported and cleared between forward and backward pass.
+        y = linear(x, w, activation="tanh")
+        layers._status[0][0] = 4
+        with pytest.raises(RuntimeError, match="linear reported error bits 0x4"):
+            check_linear()
+        assert torch.equal(torch.autograd.grad(y.sum(), w)[0], want)
+        check_linear()
+    finally:
+        layers._status.clear()
+        layers._status.update(kept)
