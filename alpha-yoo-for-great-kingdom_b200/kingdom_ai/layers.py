@@ -33,11 +33,12 @@ def _status_words(device) -> torch.Tensor:
 
 def check_linear(device="cuda") -> None:
     """Raise if a product on this device reported a bounded wait that gave up
-    since the last check (synchronises)."""
+    since the last check (waits for all of the device's streams)."""
     device = native.require_cuda(device)
     words = _status.get(device.index)
     if words is None:
         return
+    torch.cuda.synchronize(device)
     code, where = (int(v) for v in words.tolist())
     if code:
         words.zero_()

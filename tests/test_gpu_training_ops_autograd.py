@@ -105,3 +105,16 @@ def test_training_after_a_first_call_in_inference_mode():
     finally:
         layers._status.clear()
         layers._status.update(kept)
+
+
+def test_check_linear_waits_for_every_stream():
+    from kingdom_ai import check_linear, layers, linear
+    linear(torch.randn(4, 8, device="cuda"), torch.randn(8, 8, device="cuda"))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # a tenth of a second of work before a product that gives up
+        layers._status[0][:1].fill_(4)  # which does not wait, as an assignment of a number would
+    with pytest.raises(RuntimeError, match="linear reported error bits 0x4"):
+        check_linear()
+    check_linear()
