@@ -31,6 +31,7 @@ using torch::autograd::variable_list;
 
 constexpr int64_t kMost = (1ll << 31) - 1;
 constexpr int64_t kMostColumns = 1ll << 30;
+constexpr int64_t kMostValues = 1ll << 40;
 
 int type_of(at::ScalarType t) {
     switch (t) {
@@ -130,6 +131,18 @@ std::tuple<Tensor, Tensor> pack(const Tensor& x) {
 
 Tensor unpack(const Tensor& codes, const Tensor& scales, at::IntArrayRef shape, at::ScalarType dtype) {
     const at::NoGradGuard no_grad;
+    int64_t count = 1;
+    for (const int64_t size : shape) {
+        TORCH_CHECK_VALUE(size >= 0 && (size == 0 || count <= kMostValues / size),
+                          "a packed activation has up to 2**40 values");
+        count *= size;
+    }
+    TORCH_CHECK_VALUE(type_of(dtype) >= 0, "unpack gives float32, bfloat16 or float16");
+    TORCH_CHECK_VALUE(codes.is_cuda() && scales.device() == codes.device() && codes.scalar_type() == at::kByte &&
+                          scales.scalar_type() == at::kByte && codes.is_contiguous() && scales.is_contiguous() &&
+                          codes.numel() == count && scales.numel() == (count + 31) / 32,
+                      "a packed activation holds a contiguous CUDA uint8 code for each of its shape's values, and a "
+                      "scale for every 32 of them");
     Tensor out = at::empty(shape, codes.options().dtype(dtype));
     if (out.numel() > 0) {
         const c10::cuda::CUDAGuard guard(out.device());

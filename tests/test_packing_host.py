@@ -53,7 +53,8 @@ def test_kept_tensors_give_first_and_second_derivatives(which):
 @pytest.mark.parametrize("which", [0, 1])
 def test_kept_tensors_that_change_in_place_are_refused(which):
     x = torch.randn(40, requires_grad=True)
-    for change in (lambda a, y: a.mul_(2), lambda a, y: y.add_(1), lambda a, y: a[:3].zero_(), lambda a, y: y.detach().neg_()):
+    for change in (lambda a, y: a.mul_(2), lambda a, y: y.add_(1), lambda a, y: a[:3].zero_(),
+                   lambda a, y: y.detach().neg_()):
         a = x * 2
         with contexts()[which]():
             y = torch.tanh(a)
@@ -89,3 +90,10 @@ def test_operators_that_change_their_own_input_run_as_before():
     import contextlib
     for a, b in zip(gradients(contextlib.nullcontext()), gradients(packed_activations(1))):
         assert torch.equal(a, b)
+
+
+def test_a_packed_form_that_is_not_on_a_device_is_refused():
+    from kingdom_ai import PackedActivation
+    codes, scales = torch.zeros(64, dtype=torch.uint8), torch.zeros(2, dtype=torch.uint8)
+    with pytest.raises(ValueError):
+        PackedActivation(codes, scales, torch.Size([64]), torch.float32).unpack()
