@@ -28,11 +28,15 @@ class PolicyLoss(NamedTuple):
     log_probs: torch.Tensor | None   # fp32 [N], log p of the actions (0 for skipped rows); None without actions
 
 
-def _scalar(name, value, least=None):
+_FLOAT = torch.finfo(torch.float32)  # what the kernels take the weights and the denominator in
+
+
+def _scalar(name, value, least=None, most=math.inf):
     if isinstance(value, bool) or not isinstance(value, Real):
         raise TypeError(f"{name} must be a real number")
-    if not math.isfinite(value) or (least is not None and value < least):
-        raise ValueError(f"{name} must be finite" + ("" if least is None else f" and at least {least}"))
+    if not math.isfinite(value) or abs(value) > most or (least is not None and value < least):
+        raise ValueError(f"{name} must be finite" + ("" if most == math.inf else " in fp32")
+                         + ("" if least is None else f" and at least {least}"))
     return float(value)
 
 
@@ -88,14 +92,14 @@ def policy_loss(logits, *, legal_mask=None, actions=None, old_log_probs=None, ad
         if t is not None and not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a tensor")
     low, high = _clip(clip)
-    kl_weight, target_weight = _scalar("kl_weight", kl_weight), _scalar("target_weight", target_weight)
+    kl_weight = _scalar("kl_weight", kl_weight, most=_FLOAT.max)
+    target_weight = _scalar("target_weight", target_weight, most=_FLOAT.max)
     divisor = 1.0
     if denominator is None:
         divisor = float(max(logits.shape[0], 1)) if logits.dim() else 1.0
     elif not isinstance(denominator, torch.Tensor):
-        divisor, denominator = _scalar("denominator", denominator), None
-        if divisor <= 0:
-            raise ValueError("denominator must be positive")
+        # From the smallest normal number on, its inverse is finite too.
+        divisor, denominator = _scalar("denominator", denominator, _FLOAT.tiny, _FLOAT.max), None
     if _operator is None:
         _operator = native.operators().policy_loss.default
     arguments = (logits, legal_mask, actions, old_log_probs, advantages, reference_log_probs, target, low, high,
