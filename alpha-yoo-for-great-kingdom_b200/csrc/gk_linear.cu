@@ -810,7 +810,7 @@ BackwardPlan backward_plan(const gk_linear_grad_t& p, void* workspace) {
         // The residual's gradient serves as dz where its rows are aligned.
         if (p.dz != nullptr && (!k16 || !products || tma_rows(p.dz, p.n, p.n)))
             b.dz = {p.dz, p.n, false};
-        else if (b.dz32 != nullptr && !products)
+        else if ((b.narrow_dx || b.narrow_dw) && !products)  // all who read dz read it in fp32
             b.dz = {nullptr, 0, false};
         else
             b.dz = {arena.take(p.m * pad8(p.n) * (int64_t)sizeof(T)), pad8(p.n), false};
