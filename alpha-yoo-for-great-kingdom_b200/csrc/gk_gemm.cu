@@ -820,7 +820,8 @@ Epilogue epilogue_of(const GemmArgs& g) {
                g.activation, g.dtype == GK_BF16, 0, 0, 0, 0};
     e.out_wide = aligned16(g.out) && g.out_ld % 8 == 0;
     e.pre_wide = aligned16(g.pre) && g.pre_ld % 8 == 0;
-    e.residual_wide = aligned16(g.residual) && g.residual_ld % 8 == 0;
+    // Read in whole 16 bytes, which must not reach past a row: it may be the last of its storage (an expanded one is).
+    e.residual_wide = aligned16(g.residual) && g.residual_ld % 8 == 0 && g.n % 8 == 0;
     e.bias_wide = aligned16(g.bias);
     return e;
 }

@@ -1,6 +1,7 @@
 """linear on tiles that CTAs share along k: every width of a tile that holds
 all rows, from one stage of k to more than a CTA's stages, and the same bits
-from every call. Compared with the formula in 64 bits, at the tolerances of
+from every call; residuals whose rows are no whole 16 bytes, with aligned or no
+steps between them. Compared with the formula in 64 bits, at the tolerances of
 test_gpu_linear.py."""
 
 import pytest
@@ -27,3 +28,16 @@ def test_shared_tiles_repeat_their_bits(m, k, n):
     for _ in range(10):
         again = run(*args, "gelu")
         assert all(torch.equal(first[key], again[key]) for key in first)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n", [(2560, 192, 2052), (300, 96, 100), (40, 64, 1001)])
+def test_residual_rows_that_end_inside_16_bytes(m, k, n, dtype):
+    """A padded matrix, and one row for all: nothing behind a row's end is taken, and its gradient is the row's."""
+    x, w, b, r, dy = make(m, k, n, dtype, grad=False)
+    wide = torch.full((m, (n + 8) // 8 * 8), float("nan"), dtype=dtype, device="cuda")
+    wide[:, :n] = r
+    compare((x, w, b, wide[:, :n].requires_grad_(), dy), "gelu")
+    row = r[0].clone()
+    got, want = (run(x, w, b, t.requires_grad_(), dy, "tanh") for t in (row.expand(m, n), row.expand(m, n).contiguous()))
+    assert all(torch.equal(got[key], want[key]) for key in want)
