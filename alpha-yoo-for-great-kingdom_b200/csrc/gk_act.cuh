@@ -10,7 +10,8 @@ namespace gk {
 
 // Activations of values that end in 16 bits are evaluated to about 2^-20 of
 // themselves (a 16-bit type keeps 2^-9 or 2^-12); those of fp32 with CUDA's
-// erff and expf. The quick gelu has one exponential for both of its parts:
+// erff and expf. (Below 2^-126 the quick exponential and reciprocal are 0, and so is silu from -87.4 on, where
+// its value is below 2^-119 in size.) The quick gelu has one exponential for both of its parts:
 //   Phi(-a) = e^(-a^2/2) t Q(t) / 2,  t = 1 / (1 + 0.45 a / sqrt 2),  a >= 0,
 // with Q the degree-7 minimax fit of erfc(x) e^(x^2) / t over x in [0, 9.5]
 // (relative error 3e-7), so the far negative side keeps its relative accuracy.

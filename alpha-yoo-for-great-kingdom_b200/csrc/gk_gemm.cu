@@ -921,6 +921,9 @@ int gemm16(const GemmArgs& given, uint32_t* status, cudaStream_t stream) {
     // 256 x 4096 x 4096 17.0 | 21.5 | 25.3, 1024 x 256 x 4096 14.3 | 8.9 | 8.6,
     // 1024 x 1024 x 1024 10.5 | 9.7 | 11.7, 2048^3 29.5 | 22.7 | 17.8,
     // 4096^3 161 | 123 | 95, 16384 x 1024 x 256 21.2 | 14.8 | 12.5.
+    // Up to 64 rows fill half of a split tile, and the estimate takes 1.3 us off it. Where that decides between the
+    // forms (split | the pairs that would run instead): 64 x 512 x 128 4.3 | 5.1, 64 x 1024 x 256 4.8 | 5.6,
+    // 64 x 4096 x 512 6.3 | 6.7, 49 x 64 x 512 5.5 | 5.9, 49 x 4096 x 512 7.1 | 7.1.
     const double stages = (double)((g.k + kBK - 1) / kBK);
     auto rounds = [](int64_t work, int64_t at_once) { return (double)((work + at_once - 1) / at_once); };
     const int64_t tiles_m = (g.m + 255) / 256, split_tiles = ((g.m + 127) / 128) * ((g.n + 63) / 64);

@@ -183,7 +183,8 @@ __global__ void __launch_bounds__(256) pack_vectors_kernel(const T* x, int64_t v
             top = 0.0f;
 #pragma unroll
             for (int k = 0; k < V; ++k) top = fmaxf(top, finite_magnitude(as_float<T>(v[k])));
-            const unsigned team = ((1u << kTeam) - 1u) << (threadIdx.x & 31 & ~(kTeam - 1));  // its lanes, together or not
+            // Its own lanes, whichever others are here.
+            const unsigned team = ((1u << kTeam) - 1u) << (threadIdx.x & 31 & ~(kTeam - 1));
 #pragma unroll
             for (int o = kTeam / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(team, top, o));
             s = scale_exponent<T>(top);

@@ -206,7 +206,7 @@ struct Linear : torch::autograd::Function<Linear> {
         if (need_w && packed) std::tie(codes, scales) = pack_rows(x, m, k, row_stride(x, k));
         ctx->save_for_backward({need_w && !packed ? x : Tensor(), need_x ? w : Tensor(),
                                 activation == GK_ACT_NONE ? Tensor() : (pre.defined() ? pre : y), codes, scales});
-        ctx->saved_data["status"] = status;  // not an input: a call may have made it in inference mode, another may clear it
+        ctx->saved_data["status"] = status;  // no saved input: check_linear may clear it before the backward pass
         ctx->saved_data["sizes"] = std::vector<int64_t>{m, w.size(0), k, activation, need_x, need_w,
                                                         has(bias) && bias->requires_grad(),
                                                         has(residual) && residual->requires_grad()};

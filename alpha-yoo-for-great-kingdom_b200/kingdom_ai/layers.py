@@ -66,7 +66,7 @@ def linear(x, weight, bias=None, *, activation=None, residual=None, checkpoint=N
     tensor of the output's size (tanh keeps one in fp32).
 
     Second derivatives and forward-mode ones (a tensor that carries a tangent)
-    are refused.
+    are refused. torch.compile cannot trace the call: keep it outside.
 
     Call it once on a device before capturing it in a CUDA graph. As with any
     operator, capture a backward pass only when no graph of the same leaves

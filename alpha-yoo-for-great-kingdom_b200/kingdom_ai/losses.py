@@ -80,9 +80,13 @@ def policy_loss(logits, *, legal_mask=None, actions=None, old_log_probs=None, ad
     place before that.
 
     Second derivatives and forward-mode ones (a tensor that carries a tangent)
-    are refused.
+    are refused. torch.compile cannot trace the call: keep it outside.
 
     Rows with unit column stride are read in place; others are copied first.
+    Longer rows run fastest where the logits', mask's and target's rows start
+    on the same remainders of 16 bytes as the gradient's, which are contiguous:
+    a view of a padded vocabulary whose width is no multiple of 8 (fp32: 4) is
+    faster copied first.
     """
     global _operator
     if not isinstance(logits, torch.Tensor):

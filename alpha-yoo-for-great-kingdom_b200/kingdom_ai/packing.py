@@ -98,6 +98,8 @@ def packed_activations(min_elements: int = 1 << 16):
     layer outside). Gradients are then those of the held values; the forward
     pass computes with the exact ones. A relu that keeps its output passes no
     gradient where the packed output is zero.
+    A tensor that two operators keep (a relu its output, the convolution behind
+    it its input) is packed for each of them.
     ``linear`` and ``policy_loss`` keep their tensors as they are (``linear``
     has its own ``checkpoint``)."""
     if isinstance(min_elements, bool) or not isinstance(min_elements, int) or min_elements < 1:
