@@ -247,9 +247,8 @@ struct Linear : torch::autograd::Function<Linear> {
                 const size_t size = gk_linear_grad_workspace_bytes(&p);
                 if (size > 0) workspace = bytes_on((int64_t)size, dy);
                 used(dy, stream);
-                ran("gk_linear_backward",
-                    gk_linear_backward(&p, data(workspace), static_cast<uint32_t*>(ctx->saved_data["status"].toTensor().data_ptr()),
-                                       stream.stream()));
+                auto* status = static_cast<uint32_t*>(ctx->saved_data["status"].toTensor().data_ptr());
+                ran("gk_linear_backward", gk_linear_backward(&p, data(workspace), status, stream.stream()));
             }
         }
         return once({dx, dw, db, dr, Tensor(), Tensor(), Tensor()}, "linear");
